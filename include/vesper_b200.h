@@ -394,6 +394,178 @@ VESPER_C_API vesper_status_t vesper_flat_topk_device(vesper_flat_op_t op, const 
 /* Stage times of this thread's last vesper_flat_topk[_device] call. */
 VESPER_C_API vesper_status_t vesper_flat_get_last_timings(vesper_flat_timings_t* out);
 
+/* ---------------------------------------------------------------------------------
+ * Answering from retrieved passages: what a language model needs between a search and
+ * its answer.  The passages a search returns are one long prompt that many questions
+ * share; its keys and values sit in a paged cache [pages, page_size, kv_heads, head_dim].
+ *
+ *   vesper_page_tables_device             pages, slots and positions of a batch, from lengths
+ *   vesper_norm_rotate_device             per-head norm, position rotation, write by slot
+ *   vesper_prompt_attention_device        attention over packed prompts
+ *   vesper_shared_prefix_attention_device one token a request, over the shared prefix's
+ *                                         pages and then the request's own
+ *
+ * All pointers are device memory of the current device, all work is queued on
+ * cuda_stream (NULL: the default stream) and nothing is synchronised: inputs must be
+ * ready in that stream's order, and an input or workspace may be reused only in it too.
+ * No call allocates, so all of them can be captured in a CUDA graph.  16-bit data is
+ * dtype VESPER_BF16 or VESPER_F16; arithmetic is in 32 bits with one rounding at the
+ * output, but the attention probabilities are rounded to dtype before they meet the
+ * values (the sums they are divided by are not).
+ * Strides are in elements.  Data pointers are 16-byte aligned, strides multiples of 8
+ * elements, and the last dimension is contiguous.  page_size is a power of two from 16
+ * to 256.  heads is a multiple of kv_heads, at most 128 times of it; query head h reads
+ * key head h / (heads / kv_heads).
+ * Refusals return VESPER_ERROR_INVALID_PARAM with a message, before any work is queued.
+ * What only the device knows (lengths, page numbers, slots, positions) is bounded there:
+ * see each call.
+ * ------------------------------------------------------------------------------- */
+typedef enum vesper_dtype_e { VESPER_BF16 = 0, VESPER_F16 = 1 } vesper_dtype_t;
+
+/* Request b holds d_cached[b] tokens and gets d_fresh[b] more (negative counts as 0).
+ *   d_table [n_requests, table_width], row stride table_stride: entries below
+ *     ceil(cached / page_size) are read; the entries its new tokens need are written, from
+ *     d_free [n_free] in request order; the others stay.
+ *   d_lengths [n_requests] = cached + fresh; d_starts [n_requests + 1]: running sum of fresh.
+ *   d_positions [n_tokens], d_slots [n_tokens]: token t of the batch has position
+ *     base + n and slot table[b, n / page_size] * page_size + n % page_size, n its place
+ *     in its request.  Tokens past the last request: position 0, slot -1.
+ *   d_used [1]: pages the batch needs.  More than n_free: the pages that were missing are
+ *     -1 in the table, and so are the slots in them; entries past table_width are not
+ *     written and their tokens' slots are -1.
+ * n_requests at most 16384, n_tokens below 2^31.  The outputs do not depend on what an
+ * earlier call left in them, so the call may be repeated. */
+typedef struct vesper_page_tables_params_s {
+  size_t struct_size;
+  const int32_t* d_cached;
+  const int32_t* d_fresh;
+  size_t n_requests;
+  const int32_t* d_free;
+  size_t n_free;
+  int32_t* d_table;
+  size_t table_width;
+  size_t table_stride;
+  size_t page_size;
+  size_t n_tokens;
+  int64_t base;            /* 0 .. 2^31 - 1 */
+  int32_t* d_lengths;
+  int32_t* d_starts;
+  int32_t* d_positions;
+  int64_t* d_slots;
+  int32_t* d_used;
+} vesper_page_tables_params_t;
+
+VESPER_C_API vesper_status_t vesper_page_tables_device(const vesper_page_tables_params_t* params, void* cuda_stream);
+
+/* y = x * rsqrt(mean(x^2) + eps) * weight over each head of q and k, then the first
+ * `turned` values are rotated: pair i is (y[i], y[i + turned / 2]), or (y[2i], y[2i + 1])
+ * with `pairs`; (a, b) becomes (a cos - b sin, b cos + a sin) with the cosine and sine of
+ * row d_positions[t] of d_turns [n_positions, turned] (turned / 2 cosines, then sines).
+ * A NULL weight leaves that side without its norm.  Writes d_out_q [n_tokens, heads,
+ * head_dim] and, unless NULL, d_out_k [n_tokens, kv_heads, head_dim], both contiguous.
+ * With d_slots, the new keys and the values v (copied) also go to the caches at
+ * slot / page_size, slot % page_size; a slot that is negative or past n_pages *
+ * page_size is skipped.  Two tokens with one slot: either one's row is kept.
+ * A position outside the table gives NaN in the rotated values.
+ * head_dim a multiple of 8 up to 256; turned a multiple of 16, 0 to head_dim.
+ * Without d_slots, v and the caches are not read and may be NULL. */
+typedef struct vesper_norm_rotate_params_s {
+  size_t struct_size;
+  size_t dtype;            /* vesper_dtype_t */
+  size_t n_tokens, heads, kv_heads, head_dim, turned;
+  size_t pairs;            /* 0 or 1 */
+  double eps;
+  const void* d_q;
+  size_t q_token_stride, q_head_stride;
+  const void* d_k;
+  size_t k_token_stride, k_head_stride;
+  const void* d_v;
+  size_t v_token_stride, v_head_stride;
+  const int32_t* d_positions;
+  const float* d_turns;
+  size_t n_positions;
+  const void* d_q_weight;
+  const void* d_k_weight;
+  const int64_t* d_slots;
+  void* d_k_cache;
+  size_t k_page_stride, k_slot_stride, k_cache_head_stride;
+  void* d_v_cache;
+  size_t v_page_stride, v_slot_stride, v_cache_head_stride;
+  size_t n_pages, page_size;
+  void* d_out_q;
+  void* d_out_k;
+} vesper_norm_rotate_params_t;
+
+VESPER_C_API vesper_status_t vesper_norm_rotate_device(const vesper_norm_rotate_params_t* params, void* cuda_stream);
+
+/* out[i] = sum_j softmax_j(scale q_i . k_j) v_j.  Request b's queries are rows
+ * d_starts[b] .. d_starts[b + 1] of q and its keys rows d_starts_k[b] .. [b + 1] of k and v
+ * (d_starts_k NULL: d_starts).  With causal, query i of lq sees key j of lk when
+ * j <= i + lk - lq: the last query sees every key, which continues a prompt whose earlier
+ * keys are given.  A row that sees no key, and rows of q past d_starts[n_requests], give
+ * zeros and lse -inf; what is in keys and values that a row does not see, infinities and
+ * NaN included, does not reach it.  d_lse, unless NULL: [n_q, heads] log-sum-exp.
+ * starts are bounded to [0, n_q] and [0, n_k].  d_out [n_q, heads, head_dim] contiguous.
+ * head_dim a multiple of 8 up to 128; scale > 0; n_q, n_k below 2^31; d_workspace:
+ * vesper_prompt_attention_workspace bytes (16-byte aligned, NULL when that is 0). */
+typedef struct vesper_prompt_attention_params_s {
+  size_t struct_size;
+  size_t dtype;
+  size_t n_requests, n_q, n_k, heads, kv_heads, head_dim;
+  size_t causal;
+  double scale;
+  const void* d_q;
+  size_t q_token_stride, q_head_stride;
+  const void* d_k;
+  size_t k_token_stride, k_head_stride;
+  const void* d_v;
+  size_t v_token_stride, v_head_stride;
+  const int32_t* d_starts;
+  const int32_t* d_starts_k;
+  void* d_out;
+  float* d_lse;
+  void* d_workspace;
+  size_t workspace_bytes;
+} vesper_prompt_attention_params_t;
+
+VESPER_C_API size_t vesper_prompt_attention_workspace(const vesper_prompt_attention_params_t* params);
+VESPER_C_API vesper_status_t vesper_prompt_attention_device(const vesper_prompt_attention_params_t* params,
+                                                            void* cuda_stream);
+
+/* One query row a request, q [n_requests, heads, head_dim].  Its keys are the first
+ * prefix_len slots of d_prefix_pages [ceil(prefix_len / page_size)], the same for every
+ * request and read once for all of them, then the first d_lengths[b] slots of
+ * d_table[b, 0 .. table_width).  Softmax and outputs as above, joined over both parts.
+ * Lengths are bounded to [0, table_width * page_size]; a page number outside
+ * [0, n_pages) reads as zero keys and values.  Slots past the lengths are not used,
+ * whatever is in them. */
+typedef struct vesper_shared_prefix_attention_params_s {
+  size_t struct_size;
+  size_t dtype;
+  size_t n_requests, heads, kv_heads, head_dim;
+  double scale;
+  const void* d_q;
+  size_t q_token_stride, q_head_stride;
+  const void* d_k_cache;
+  size_t k_page_stride, k_slot_stride, k_cache_head_stride;
+  const void* d_v_cache;
+  size_t v_page_stride, v_slot_stride, v_cache_head_stride;
+  size_t n_pages, page_size;
+  const int32_t* d_prefix_pages;
+  size_t prefix_len;
+  const int32_t* d_table;
+  size_t table_width, table_stride;
+  const int32_t* d_lengths;
+  void* d_out;
+  float* d_lse;
+  void* d_workspace;
+  size_t workspace_bytes;
+} vesper_shared_prefix_attention_params_t;
+
+VESPER_C_API size_t vesper_shared_prefix_attention_workspace(const vesper_shared_prefix_attention_params_t* params);
+VESPER_C_API vesper_status_t vesper_shared_prefix_attention_device(
+    const vesper_shared_prefix_attention_params_t* params, void* cuda_stream);
+
 /* Number of CUDA devices visible to the library. */
 VESPER_C_API int vesper_b200_device_count(void);
 

@@ -46,6 +46,9 @@ EXPORTED = [
     "vesper_kmeans_shard_pp_update", "vesper_kmeans_shard_accumulate", "vesper_kmeans_shard_finish",
     "vesper_kmeans_shard_running_inertia", "vesper_kmeanspp_sampler_create", "vesper_kmeanspp_sampler_next",
     "vesper_kmeanspp_sampler_destroy",
+    "vesper_page_tables_device", "vesper_norm_rotate_device", "vesper_prompt_attention_workspace",
+    "vesper_prompt_attention_device", "vesper_shared_prefix_attention_workspace",
+    "vesper_shared_prefix_attention_device",
     "vesper_mgr_create", "vesper_mgr_destroy", "vesper_mgr_build", "vesper_mgr_add_batch", "vesper_mgr_update",
     "vesper_mgr_update_batch", "vesper_mgr_remove", "vesper_mgr_remove_batch", "vesper_mgr_search",
     "vesper_mgr_search_batch", "vesper_mgr_save", "vesper_mgr_load", "vesper_mgr_memory_usage",
@@ -248,6 +251,12 @@ def load(path: str = LIB_PATH) -> C.CDLL:
             "vesper_kmeanspp_sampler_create": (st, [C.c_uint32, C.c_size_t, C.POINTER(vp), C.POINTER(C.c_size_t)]),
             "vesper_kmeanspp_sampler_next": (st, [vp, f32p, C.POINTER(C.c_size_t)]),
             "vesper_kmeanspp_sampler_destroy": (None, [vp]),
+            "vesper_page_tables_device": (st, [vp, vp]),
+            "vesper_norm_rotate_device": (st, [vp, vp]),
+            "vesper_prompt_attention_workspace": (C.c_size_t, [vp]),
+            "vesper_prompt_attention_device": (st, [vp, vp]),
+            "vesper_shared_prefix_attention_workspace": (C.c_size_t, [vp]),
+            "vesper_shared_prefix_attention_device": (st, [vp, vp]),
             "vesper_mgr_create": (st, [C.c_size_t, C.POINTER(vp)]),
             "vesper_mgr_destroy": (st, [vp]),
             "vesper_mgr_build": (st, [vp, f32p, C.c_size_t, C.POINTER(ManagerBuildConfig)]),
