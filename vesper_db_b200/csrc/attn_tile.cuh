@@ -1,0 +1,588 @@
+// Attention of query tiles on the tensor cores (tcgen05): the kernel that prompts and the
+// shared prefix both run.
+//
+//   S = Q K^T, P = exp2(scale' S - m) with scale' = scale log2(e), O = sum P V / sum P,
+// one pass over the keys with a running maximum m and sum l of each row in 32 bits.
+//
+// A tile is 128 rows: floor(128 / group) tokens with the `group` query heads of one key
+// head each, so that one key tile serves the whole group.  A block holds two query tiles
+// and takes the keys 128 at a time:
+//   * warp 8 copies Q, then K and V tiles by TMA into a ring of shared-memory slots;
+//   * warp 9 issues the products: S_t = Q_t K^T (both operands from shared memory) and
+//     O_t += P_t V (P from tensor memory);
+//   * warps 0-3 and 4-7 hold one row a thread of tile 0 and tile 1: they read S, keep m and
+//     l, and write P over S as 16-bit values;
+//   * warps 10 and 11 clean the value tiles that hold keys some row must not see.
+// The two query tiles alternate: while one is in the tensor cores the other is in the
+// exponentials.  Tensor memory: S0, S1 (128 columns each), O0, O1.
+//
+// m only moves when a row's maximum has grown by more than 2^8: until then P may reach 2^8,
+// which both types hold at full relative precision, and O need not be rescaled.
+//
+// Masked scores become -inf by selection, so what unseen keys hold does not matter; unseen
+// values meet P = 0, and 0 * NaN is NaN: value rows past the last key are zeroed in shared
+// memory, and where a later token of the same prompt holds a non-finite value (checked on
+// the diagonal tiles) the block recomputes its rows one key at a time.
+//
+// Every wait is bounded; a block whose wait ran out issues no further work, gives NaN rows
+// and frees its tensor memory.
+#pragma once
+
+#include <cuda.h>
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "half_types.cuh"
+#include "tc_common.cuh"
+
+namespace vgpu {
+namespace attn {
+
+constexpr int kRows = 128;     // query rows of a tile
+constexpr int kKeys = 128;     // keys of a tile
+constexpr int kThreads = 384;  // two softmax warpgroups, one of service warps
+constexpr int kSlots = 4;      // K and V tiles in flight
+constexpr float kGrow = 8.0f;  // log2 of how far P may pass 1 before O is rescaled
+constexpr int kSoftmaxRegs = 224, kServiceRegs = 40;  // 2 * 128 * 224 + 128 * 40 <= 384 * 168
+
+struct TileParams {
+    CUtensorMap mq, mk, mv;
+    int heads, kv_heads, group, dim;
+    int tile_tokens;  // tokens of one query tile
+    int n_q, n_k;     // rows of q; rows of k and v, or keys of the prefix
+    // Packed prompts: requests' first rows.  Shared prefix: one request of all rows.
+    const int32_t* starts;
+    const int32_t* starts_k;
+    int n_requests;
+    bool causal;
+    // Paged keys: pages of the prefix.
+    const int32_t* pages;
+    int page_shift;
+    // Packed keys again, for the rows recomputed one key at a time.
+    HeadsView q, k, v;
+    float scale_log2;
+    int splits;
+    bool part;       // results of each split for a later join, in 32 bits
+    void* out;       // otherwise: [n_q, heads, dim]
+    float* lse;
+    float* part_o;   // [splits, n_q * heads, dim], and their log2-sum-exp
+    float* part_lse;
+};
+
+template <int D>
+constexpr int smem_bytes() {
+    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 256;
+}
+
+// Bounded wait for the barrier's phase; false when it ran out (a tile takes microseconds).
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+    const uint32_t a = tc::smem_u32(bar);
+    for (uint32_t i = 0; i < (1u << 20); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(map), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+// Operand whose 64-value blocks run along the output dimension (values: rows are keys),
+// 128-byte swizzle: 8-key groups 1024 bytes apart, 64-value blocks `block_bytes` apart.
+__device__ __forceinline__ uint64_t values_desc(uint32_t saddr, uint32_t block_bytes) {
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(block_bytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// What a block works on.
+struct Work {
+    int q0;        // first row of q of the block's first tile
+    int tokens;    // rows of the request from there on (at most 2 tiles of them count)
+    int k0, len_k; // first key row, keys of the request
+    int first_lim; // keys that the first of these rows sees; each later one sees `step` more
+    int step;
+    int split;
+};
+
+// Tile `idx` (two query tiles each) of the packed requests, last ones first: the rows of a
+// causal prompt's end see the most keys.  Run by one whole warp; tokens = 0: no such tile.
+// Rows before the first and after the last request are requests without keys.
+__device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane) {
+    Work w{};
+    const int n = p.n_requests + 2, per = (n + 31) / 32, span = 2 * p.tile_tokens;
+    const int b0 = lane * per, b1 = min(n, b0 + per);
+    auto bound = [&](int b) {  // first row of piece b
+        if (b == 0) return 0;
+        if (b >= n) return p.n_q;
+        return min(max(p.starts[b - 1], 0), p.n_q);
+    };
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (max(bound(b + 1) - bound(b), 0) + span - 1) / span;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    const int want = total - 1 - idx;
+    const bool here = want >= 0 && want >= incl - mine && want < incl;
+    if (here) {
+        int at = incl - mine, b = b0;
+        for (;; ++b) {
+            const int t = (max(bound(b + 1) - bound(b), 0) + span - 1) / span;
+            if (want < at + t) break;
+            at += t;
+        }
+        const int q0 = bound(b), len_q = bound(b + 1) - q0, tok = (want - at) * span;
+        int k0 = 0, k1 = 0;
+        if (b > 0 && b <= p.n_requests) {
+            k0 = min(max(p.starts_k[b - 1], 0), p.n_k);
+            k1 = min(max(p.starts_k[b], k0), p.n_k);
+        }
+        w.q0 = q0 + tok;
+        w.tokens = len_q - tok;
+        w.k0 = k0;
+        w.len_k = k1 - k0;
+        w.step = p.causal ? 1 : 0;
+        w.first_lim = p.causal ? tok + 1 + w.len_k - len_q : w.len_k;
+    }
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    const int src = who ? __ffs(who) - 1 : 0;
+    w.q0 = __shfl_sync(0xffffffffu, w.q0, src);
+    w.tokens = __shfl_sync(0xffffffffu, w.tokens, src);
+    w.k0 = __shfl_sync(0xffffffffu, w.k0, src);
+    w.len_k = __shfl_sync(0xffffffffu, w.len_k, src);
+    w.step = __shfl_sync(0xffffffffu, w.step, src);
+    w.first_lim = __shfl_sync(0xffffffffu, w.first_lim, src);
+    return w;
+}
+
+template <class H>
+__device__ __forceinline__ bool not_finite(uint4 u) {
+    constexpr uint32_t lo = sizeof(H) && std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & lo) == lo || (w[i] & hi) == hi;
+    return bad;
+}
+
+template <class H, int D, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_constant__ TileParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    constexpr int kHalves = D / 64, kHalfBytes = kKeys * 128, kTileBytes = kHalves * kHalfBytes;
+    const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw);
+    const uint32_t s_q = base, s_kv = base + 2 * kTileBytes;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + (2 + kSlots) * kTileBytes);
+    uint64_t* const q_full = bars;                // [2]
+    uint64_t* const kv_full = bars + 2;           // [kSlots]
+    uint64_t* const kv_empty = kv_full + kSlots;  // [kSlots]
+    uint64_t* const s_full = kv_empty + kSlots;   // [2]
+    uint64_t* const p_full = s_full + 2;          // [2]
+    uint64_t* const o_full = p_full + 2;          // [2]
+    uint64_t* const drained = o_full + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    int* const s_leak = reinterpret_cast<int*>(tmem_slot + 1);
+    Work* const s_work = reinterpret_cast<Work*>(tmem_slot + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int block = blockIdx.x;
+    const int kh = block % p.kv_heads;
+    block /= p.kv_heads;
+    const int split = block % p.splits;
+    block /= p.splits;
+
+    if (warp == 0) {
+        Work w{};
+        if (PAGED) {  // every row sees the whole prefix
+            w.q0 = block * 2 * p.tile_tokens;
+            w.tokens = p.n_q - w.q0;
+            w.len_k = w.first_lim = p.n_k;
+        } else {
+            w = find_work(p, block, lane);
+        }
+        w.split = split;
+        if (lane == 0) *s_work = w;
+    } else if (warp == 9) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; ++i) {
+                tc::mbar_init(&q_full[i], 1);
+                tc::mbar_init(&s_full[i], 1);
+                tc::mbar_init(&p_full[i], 128);
+                tc::mbar_init(&o_full[i], 1);
+            }
+            for (int i = 0; i < kSlots; ++i) {
+                tc::mbar_init(&kv_full[i], 1);
+                tc::mbar_init(&kv_empty[i], 1);
+            }
+            tc::mbar_init(drained, 1);
+            *s_leak = 0;
+            tc::mbar_init_fence();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const Work w = *s_work;
+
+    // Key tiles of each query tile in this split: [j0, j0 + n_t).
+    const int tt = p.tile_tokens;
+    int tok[2], nt[2];  // indexed by constants only: they stay in registers
+    const int all = (w.len_k + kKeys - 1) / kKeys, per = (all + p.splits - 1) / p.splits, j0 = w.split * per;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        tok[t] = min(max(w.tokens - t * tt, 0), tt);
+        const int last = min(w.len_k, w.first_lim + w.step * (t * tt + tok[t] - 1));  // keys its last row sees
+        const int tiles = tok[t] > 0 ? (max(last, 0) + kKeys - 1) / kKeys : 0;
+        nt[t] = min(max(tiles - j0, 0), per);
+    }
+    const int n = max(nt[0], nt[1]);
+    // From this key on some valid row of the block does not see the keys.
+    const int min_lim = min(max(w.first_lim, 0), w.len_k);
+    auto guarded_tile = [&](int j) { return (j0 + j + 1) * kKeys > min_lim; };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+        if (warp == 8) {
+            // ---------------------------------------------------------------- copies
+            if (n > 0) {
+                if (lane == 0) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (nt[t] == 0) continue;
+                        const uint32_t rows = (uint32_t)(tt * p.group);
+                        tc::mbar_expect_tx(&q_full[t], rows * 128 * kHalves);
+                        for (int h = 0; h < kHalves; ++h)
+                            tma4(s_q + t * kTileBytes + h * kHalfBytes, &p.mq, h * 64, 0, kh, w.q0 + t * tt, &q_full[t]);
+                    }
+                }
+                bool ok = true;
+                int i = 0;
+                for (; i < 2 * n; ++i) {  // K, V, K, V, ...
+                    const int slot = i % kSlots, round = i / kSlots, key = (j0 + (i >> 1)) * kKeys;
+                    if (round > 0) ok = mbar_wait(&kv_empty[slot], (round - 1) & 1);
+                    if (!ok) break;
+                    const CUtensorMap* map = (i & 1) ? &p.mv : &p.mk;
+                    const uint32_t dst = s_kv + slot * kTileBytes;
+                    if (!PAGED) {
+                        if (lane == 0) {
+                            tc::mbar_expect_tx(&kv_full[slot], kTileBytes);
+                            for (int h = 0; h < kHalves; ++h)
+                                tma4(dst + h * kHalfBytes, map, h * 64, kh, w.k0 + key, 0, &kv_full[slot]);
+                        }
+                    } else {
+                        const int page = 1 << p.page_shift, box = min(page, kKeys);
+                        const int boxes = (min(w.len_k - key, kKeys) + box - 1) / box;  // those that hold keys
+                        if (lane == 0) tc::mbar_expect_tx(&kv_full[slot], (uint32_t)(boxes * box) * 128 * kHalves);
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const int at = key + lane * box, pg = p.pages[at >> p.page_shift];
+                            for (int h = 0; h < kHalves; ++h)
+                                tma4(dst + h * kHalfBytes + lane * box * 128, map, h * 64, kh, at & (page - 1), pg,
+                                     &kv_full[slot]);
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (!ok)  // nothing may land after the block has gone
+                    for (int e = max(i - kSlots, 0); e < i; ++e) mbar_wait(&kv_full[e % kSlots], (e / kSlots) & 1);
+            }
+        } else if (warp == 9) {
+            // ---------------------------------------------------------------- products
+            constexpr uint32_t fmt = std::is_same<H, Bf16>::value ? 1u : 0u;
+            constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
+            constexpr uint32_t id_s = common | ((uint32_t)(kKeys >> 3) << 17);
+            constexpr uint32_t id_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+            const int steps = (p.dim + 15) / 16;  // of the score product: columns past dim are zero
+            bool ok = true;
+            auto wait = [&](uint64_t* b, uint32_t parity) {
+                if (ok) ok = mbar_wait(b, parity);
+                return ok;
+            };
+            auto scores = [&](int t, int slot) {
+                if (lane == 0) {
+                    const uint32_t a = s_q + t * kTileBytes, b = s_kv + slot * kTileBytes;
+                    for (int k = 0; k < steps; ++k) {
+                        const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                        mma_ss(tmem + t * 128, tc::sw128_kmajor_desc(a + off), tc::sw128_kmajor_desc(b + off), id_s, k > 0);
+                    }
+                    tc::commit(&s_full[t]);
+                }
+                __syncwarp();
+            };
+            // Hands slot of item i back to the copies, unless they are done with it: an arrival
+            // that nobody waits for could come after the block has gone.
+            auto release = [&](int i) {
+                if (ok && i + kSlots < 2 * n && lane == 0) tc::commit(&kv_empty[i % kSlots]);
+                __syncwarp();
+            };
+            if (n > 0) {
+                wait(&kv_full[0], 0);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (nt[t] > 0 && wait(&q_full[t], 0)) {
+                        tc::fence_after_sync();
+                        scores(t, 0);
+                    }
+                release(0);
+            }
+            for (int j = 0; j < n; ++j) {
+                const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % kSlots, sk = ik % kSlots;
+                wait(&kv_full[sv], (iv / kSlots) & 1);
+                if (guarded_tile(j)) {
+                    asm volatile("bar.sync 1, 96;" ::: "memory");
+                    asm volatile("bar.sync 2, 96;" ::: "memory");
+                }
+                const bool more = j + 1 < n;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (j < nt[t] && wait(&p_full[t], j & 1)) {
+                        tc::fence_after_sync();
+                        if (lane == 0) {
+                            const uint32_t b = s_kv + sv * kTileBytes;
+                            for (int k = 0; k < kKeys / 16; ++k)
+                                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, values_desc(b + k * 2048, kHalfBytes),
+                                       id_o, (j > 0 || k > 0) ? 1u : 0u);
+                            if (j + 1 == nt[t]) tc::commit(&o_full[t]);
+                        }
+                        __syncwarp();
+                    }
+                    if (more && t == 0) wait(&kv_full[sk], (ik / kSlots) & 1);
+                    if (ok && j + 1 < nt[t]) scores(t, sk);
+                }
+                release(iv);
+                if (more) release(ik);
+            }
+            if (!ok) {
+                if (lane == 0) tc::commit(drained);
+                __syncwarp();
+                mbar_wait(drained, 0);
+            }
+        } else {
+            // ---------------------------------------------------------------- value rows that not every row sees
+            const int g = tid - 320;
+            for (int j = 0; j < n; ++j) {
+                if (!guarded_tile(j)) continue;
+                asm volatile("bar.sync 1, 96;" ::: "memory");
+                uint8_t* const v = smem + (2 + (2 * j + 1) % kSlots) * kTileBytes;
+                const int key = (j0 + j) * kKeys;
+                const int end = min(max(w.len_k - key, 0), kKeys), from = max(min_lim - key, 0);
+                bool bad = false;
+                if (!PAGED)
+                    for (int i = g; i < (end - from) * 8; i += 64)
+                        for (int h = 0; h < kHalves; ++h)
+                            bad |= not_finite<H>(*reinterpret_cast<const uint4*>(v + h * kHalfBytes + from * 128 + i * 16));
+                for (int i = g; i < (kKeys - end) * 8; i += 64)
+                    for (int h = 0; h < kHalves; ++h)
+                        *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                if (bad) *s_leak = 1;
+                tc::fence_proxy_async_smem();
+                asm volatile("bar.sync 2, 96;" ::: "memory");
+            }
+        }
+    } else {
+        // -------------------------------------------------------------------- softmax: one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int t = warp >> 2, row = tid & 127;
+        const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+        const int my_tiles = t ? nt[1] : nt[0];
+        const bool valid = row_tok < (t ? tok[1] : tok[0]);
+        const int lim = valid ? min(max(w.first_lim + w.step * (t * tt + row_tok), 0), w.len_k) : w.len_k;
+        const int tile_lim = min(max(w.first_lim + w.step * t * tt, 0), w.len_k);  // the tile's first row's
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + t * 128 + lane_base, to = tmem + 256 + t * 128 + lane_base;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < my_tiles && ok; ++j) {
+            ok = mbar_wait(&s_full[t], j & 1);
+            if (!ok) break;
+            tc::fence_after_sync();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::tmem_ld32(ts + c * 32, s[c]);
+            tc::tmem_ld_wait();
+            const int key = (j0 + j) * kKeys;
+            if (key + kKeys > tile_lim) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (key + c * 32 + i >= lim) s[c][i] = 0xff800000u;  // -inf
+            }
+            float mx[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+            if (j == 0) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, top - m > kGrow)) {
+                const float up = top - m > kGrow ? top : m;
+                const float f = top - m > kGrow ? ex2(m - up) : 1.0f;
+                m = up;
+                l *= f;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tc::tmem_ld32(to + c * 32, o);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc::tmem_st32(to + c * 32, o);
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float a = ex2(fmaf(__uint_as_float(s[c + i / 16][(2 * i) & 31]), p.scale_log2, -ref));
+                    const float b = ex2(fmaf(__uint_as_float(s[c + i / 16][(2 * i + 1) & 31]), p.scale_log2, -ref));
+                    sum[i & 3] += a + b;
+                    pk[i] = H::pack(a, b);
+                }
+                tc::tmem_st32(ts + c * 16, pk);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            tc::mbar_arrive(&p_full[t]);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        if (ok && my_tiles > 0) ok = mbar_wait(&o_full[t], 0);
+        tc::fence_after_sync();
+        // ---- results
+        const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + kh * p.group + row_head);
+        const bool leak = !PAGED && my_tiles > 0 && *reinterpret_cast<volatile int*>(s_leak) != 0;
+        const bool part = p.part;
+        const long long rows = (long long)p.n_q * p.heads;
+        float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        if (!ok) inv = __int_as_float(0x7fc00000);
+        using T = typename H::type;
+        if (!leak) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                if (my_tiles > 0) {
+                    tc::tmem_ld32(to + c * 32, o);
+                    tc::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (!valid || c * 32 + i >= p.dim) continue;
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f && ok ? 0.0f : __uint_as_float(o[i + e]) * inv;
+                    if (part) {
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + (split * rows + at) * p.dim + c * 32 + i);
+                        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+                    } else {
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + c * 32 + i) = pack8<H>(x);
+                    }
+                }
+                __syncwarp();
+            }
+        } else if (valid) {
+            // One key at a time, eight output values a pass, with the maximum and sum that the
+            // scores gave: only where an unseen value row is not finite.
+            const T* q = static_cast<const T*>(p.q.p) + (w.q0 + t * tt + row_tok) * p.q.tok + (kh * p.group + row_head) * p.q.head;
+            const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + kh * p.k.head;
+            const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + kh * p.v.head;
+            const int from = j0 * kKeys, to_key = min(lim, (j0 + per) * kKeys);
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+            for (int c = 0; c < p.dim; c += 8) {
+                float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+                for (int key = from; key < to_key; ++key) {
+                    float s = 0.0f;
+#pragma unroll 1
+                    for (int e = 0; e < p.dim; e += 8) {
+                        float a[8], b[8];
+                        unpack8<H>(*reinterpret_cast<const uint4*>(q + e), a);
+                        unpack8<H>(*reinterpret_cast<const uint4*>(k + key * p.k.tok + e), b);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+                    }
+                    const float x = ex2(fmaf(s, p.scale_log2, -ref));
+                    float val[8];
+                    unpack8<H>(*reinterpret_cast<const uint4*>(v + key * p.v.tok + c), val);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] += x * val[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= inv;
+                if (part) {
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + (split * rows + at) * p.dim + c);
+                    dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+                    dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+                } else {
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + c) = pack8<H>(o);
+                }
+            }
+        }
+        if (valid) {
+            const float lse2 = ok ? m + log2f(l) : __int_as_float(0x7fc00000);
+            if (part) p.part_lse[split * rows + at] = lse2;
+            else if (p.lse) p.lse[at] = lse2 * 0.6931471805599453f;
+        }
+        tc::fence_before_sync();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc::fence_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace attn
+}  // namespace vgpu
