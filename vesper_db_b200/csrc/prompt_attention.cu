@@ -102,53 +102,258 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 }
 
 // ---------------------------------------------------------------------------------
-// Own pages of each request: one warp a query row.
+// Own pages of each request: bound by reading keys and values once.  A block takes one
+// request, one key head, up to 16 of its query heads and a range of keys; each of its
+// warps takes 16 keys at a time, with its own running maximum and sum, and the four are
+// joined at the end.  The products are m16n8k16 steps of one warp: 16 query heads by 8
+// keys, then by 8 values.  Operands go from global memory to registers in 16-byte loads,
+// without a stop in shared memory:
+//   * keys: the order of the contraction index is free, so lane (g, t) = (lane / 4,
+//     lane % 4) holds chunks t, t + 4, ... (eight values each) of key g, and the queries are
+//     laid out the same way;
+//   * values: the order of the output columns is free, so lane (g, t) holds chunks g and
+//     g + 8 of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and column n of step (i, e) is value
+//     (8 i + n) 8 + e: one byte permutation makes each operand register.
+// The next keys are loaded while the scores become probabilities, the next values while
+// the next scores are made.
 // ---------------------------------------------------------------------------------
-constexpr int kWarps = 4;
+constexpr int kOwnWarps = 4;
 
-// A lane holds values lane * 4 .. lane * 4 + 3 of a row of up to 128.
 template <class H>
-__device__ __forceinline__ float4 load4(const void* p, long long at, bool live) {
-    if (!live) return make_float4(0, 0, 0, 0);
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const typename H::type*>(p) + at);
-    const float2 a = H::unpack(u.x), b = H::unpack(u.y);
-    return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (std::is_same<H, Bf16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+
+template <class H, int D>
+__global__ void __launch_bounds__(kOwnWarps * 32) own_pages_kernel(const __grid_constant__ SharedArgs a, int splits, int chunk,
+                                                                   float* __restrict__ part_o, float* __restrict__ part_lse) {
+    using T = typename H::type;
+    constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key row, of a value row
+    constexpr int kPad = D + 4;
+    __shared__ float s_o[kOwnWarps][16][kPad];
+    __shared__ float s_m[kOwnWarps][16], s_l[kOwnWarps][16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads, mt = (group + 15) / 16;
+    int x = blockIdx.x;  // key heads fastest: blocks that run together read neighbouring memory
+    const int kh = x % a.kv_heads;
+    x /= a.kv_heads;
+    const int m0 = (x % mt) * 16;
+    x /= mt;
+    const int split = x % splits, b = x / splits;
+    const int rows_here = min(16, group - m0);
+    const long long rows = (long long)a.n_requests * a.heads;
+    const long long row0 = (long long)b * a.heads + kh * group + m0;
+
+    const int n = min(max(a.lengths[b], 0), a.table_width << a.page_shift);
+    const int begin = min((long long)split * chunk, (long long)n), end = min(n, begin + chunk);
+    if (begin >= end) {
+        if (tid < rows_here) part_lse[split * rows + row0 + tid] = -INFINITY;
+        return;
+    }
+    const int blocks = (end - begin + 15) / 16;
+    const int32_t* pages = a.table + (long long)b * a.table_stride;
+    const int mask = (1 << a.page_shift) - 1;
+
+    // Queries, laid out as the keys are.
+    uint32_t qa[2 * KC][4];
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+        const int c = (i * 4 + t) * 8;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        const T* q = static_cast<const T*>(a.q.p) + b * a.q.tok + (kh * group + m0) * a.q.head;
+        if (c < a.dim && g < rows_here) lo = *reinterpret_cast<const uint4*>(q + g * a.q.head + c);
+        if (c < a.dim && g + 8 < rows_here) hi = *reinterpret_cast<const uint4*>(q + (g + 8) * a.q.head + c);
+        qa[2 * i][0] = lo.x; qa[2 * i][1] = hi.x; qa[2 * i][2] = lo.y; qa[2 * i][3] = hi.y;
+        qa[2 * i + 1][0] = lo.z; qa[2 * i + 1][1] = hi.z; qa[2 * i + 1][2] = lo.w; qa[2 * i + 1][3] = hi.w;
+    }
+
+    uint4 kf[2][KC], vf[4][VC];
+    // 16 keys lie in one page.  Rows past the end are not read: they may hold anything.
+    auto load_k = [&](int ib, int pg) {
+        const int key = begin + ib * 16;
+        const bool ok = ib < blocks && pg >= 0 && pg < a.n_pages;
+        const T* p = static_cast<const T*>(a.k_cache.p) + pg * a.k_cache.page + (key & mask) * a.k_cache.tok + kh * a.k_cache.head;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < KC; ++i) {
+                const int c = (i * 4 + t) * 8;
+                kf[r][i] = make_uint4(0, 0, 0, 0);
+                if (ok && c < a.dim && key + r * 8 + g < end)
+                    kf[r][i] = *reinterpret_cast<const uint4*>(p + (r * 8 + g) * a.k_cache.tok + c);
+            }
+    };
+    auto load_v = [&](int ib, int pg) {
+        const int key = begin + ib * 16;
+        const bool ok = ib < blocks && pg >= 0 && pg < a.n_pages;
+        const T* p = static_cast<const T*>(a.v_cache.p) + pg * a.v_cache.page + (key & mask) * a.v_cache.tok + kh * a.v_cache.head;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VC; ++i) {
+                const int c = (i * 8 + g) * 8, k = 2 * t + (r & 1) + (r >> 1) * 8;
+                vf[r][i] = make_uint4(0, 0, 0, 0);
+                if (ok && c < a.dim && key + k < end) vf[r][i] = *reinterpret_cast<const uint4*>(p + k * a.v_cache.tok + c);
+            }
+    };
+    auto page_of = [&](int ib) { return ib < blocks ? pages[(begin + ib * 16) >> a.page_shift] : -1; };
+
+    float o[VC][8][4];
+#pragma unroll
+    for (int i = 0; i < VC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[i][e][c] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const float scale = a.scale * kLog2e;
+    int ib = warp, pg = page_of(ib), pg_next = page_of(ib + kOwnWarps);
+    load_k(ib, pg);
+    load_v(ib, pg);
+    for (; ib < blocks; ib += kOwnWarps) {
+        float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                mma16816<H>(s[r], qa[2 * i], kf[r][i].x, kf[r][i].y);
+                mma16816<H>(s[r], qa[2 * i + 1], kf[r][i].z, kf[r][i].w);
+            }
+        const int pg_after = page_of(ib + 2 * kOwnWarps);
+        load_k(ib + kOwnWarps, pg_next);
+        const int key = begin + ib * 16;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                s[r][c] = key + r * 8 + 2 * t + (c & 1) < end ? s[r][c] * scale : -INFINITY;
+                top[c >> 1] = fmaxf(top[c >> 1], s[r][c]);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float up = fmaxf(m[h], top[h]), f = up == -INFINITY ? 1.0f : attn::ex2(m[h] - up);
+                m[h] = up;
+                l[h] *= f;
+#pragma unroll
+                for (int i = 0; i < VC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        o[i][e][2 * h] *= f;
+                        o[i][e][2 * h + 1] *= f;
+                    }
+            }
+        }
+        const float ref0 = m[0] == -INFINITY ? 0.0f : m[0], ref1 = m[1] == -INFINITY ? 0.0f : m[1];
+        uint32_t pa[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float p0 = attn::ex2(s[r][0] - ref0), p1 = attn::ex2(s[r][1] - ref0);
+            const float p2 = attn::ex2(s[r][2] - ref1), p3 = attn::ex2(s[r][3] - ref1);
+            l[0] += p0 + p1;
+            l[1] += p2 + p3;
+            pa[2 * r] = H::pack(p0, p1);
+            pa[2 * r + 1] = H::pack(p2, p3);
+        }
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+                const uint32_t b0 = __byte_perm(word(vf[0][i], e / 2), word(vf[1][i], e / 2), sel);
+                const uint32_t b1 = __byte_perm(word(vf[2][i], e / 2), word(vf[3][i], e / 2), sel);
+                mma16816<H>(o[i][e], pa, b0, b1);
+            }
+        load_v(ib + kOwnWarps, pg_next);
+        pg_next = pg_after;
+    }
+
+    // Join of the four warps.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = g + 8 * h;
+        if (t == 0) {
+            s_m[warp][r] = m[h];
+            s_l[warp][r] = l[h];
+        }
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float4* dst = reinterpret_cast<float4*>(&s_o[warp][r][(i * 8 + 2 * t + c) * 8]);
+                dst[0] = make_float4(o[i][0][2 * h + c], o[i][1][2 * h + c], o[i][2][2 * h + c], o[i][3][2 * h + c]);
+                dst[1] = make_float4(o[i][4][2 * h + c], o[i][5][2 * h + c], o[i][6][2 * h + c], o[i][7][2 * h + c]);
+            }
+    }
+    __syncthreads();
+    const int r = tid >> 3;
+    if (r >= rows_here) return;
+    float top = -INFINITY, total = 0.0f, w[kOwnWarps];
+#pragma unroll
+    for (int i = 0; i < kOwnWarps; ++i) top = fmaxf(top, s_m[i][r]);
+#pragma unroll
+    for (int i = 0; i < kOwnWarps; ++i) {
+        w[i] = s_m[i][r] == -INFINITY ? 0.0f : attn::ex2(s_m[i][r] - top);
+        if (i >= blocks) w[i] = 0.0f;  // a warp without keys
+        total += s_l[i][r] * w[i];
+    }
+    const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
+    for (int d = (tid & 7) * 4; d < a.dim; d += 32) {
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kOwnWarps; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[i][r][d]);
+            acc = make_float4(acc.x + w[i] * v.x, acc.y + w[i] * v.y, acc.z + w[i] * v.z, acc.w + w[i] * v.w);
+        }
+        *reinterpret_cast<float4*>(part_o + (split * rows + row0 + r) * a.dim + d) =
+            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    if ((tid & 7) == 0) part_lse[split * rows + row0 + r] = top + log2f(total);
+}
+
+struct OwnPlan {
+    int splits, chunk;  // ranges of `chunk` keys
+};
+// The lengths are on the device: ranges are cut for what the table can hold.  Six blocks an
+// SM fill the GPU; no range is below 128 keys, none above 1,024, so that the longest request
+// does not run on alone.  A range past a request's length costs one write a row.
+OwnPlan own_plan(const SharedArgs& a) {
+    const long long cap = (long long)a.table_width << a.page_shift;
+    const long long base = (long long)a.n_requests * a.kv_heads * ((a.heads / a.kv_heads + 15) / 16);
+    long long s = std::max<long long>(ceil_div(6 * kSms, base), ceil_div(cap, 1024));
+    s = std::max<long long>(1, std::min<long long>({s, (cap + 127) / 128, 256}));
+    OwnPlan p;
+    p.chunk = (int)((ceil_div(cap, s) + 63) / 64 * 64);
+    p.splits = p.chunk ? (int)((cap + p.chunk - 1) / p.chunk) : 0;
+    return p;
 }
 
 template <class H>
-__global__ void __launch_bounds__(kWarps * 32) own_rows_kernel(const __grid_constant__ SharedArgs a, float* part_o,
-                                                               float* part_lse) {
-    const int lane = threadIdx.x & 31;
-    const long long row = blockIdx.x * (long long)kWarps + (threadIdx.x >> 5);
-    if (row >= (long long)a.n_requests * a.heads) return;
-    const int b = (int)(row / a.heads), h = (int)(row % a.heads), kh = h / (a.heads / a.kv_heads);
-    const bool live = lane * 4 < a.dim;
-    float4 q = load4<H>(a.q.p, b * a.q.tok + h * a.q.head + lane * 4, live);
-    const float f = a.scale * kLog2e;
-    q = make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    const int mask = (1 << a.page_shift) - 1;
-    const int32_t* pages = a.table + (long long)b * a.table_stride;
-    const long long n = min((long long)max(a.lengths[b], 0), (long long)a.table_width << a.page_shift);
-    for (long long j = 0; j < n; ++j) {
-        const long long p = pages[j >> a.page_shift];
-        const bool ok = live && p >= 0 && p < a.n_pages;
-        const float4 k = load4<H>(
-            a.k_cache.p, p * a.k_cache.page + (j & mask) * a.k_cache.tok + kh * a.k_cache.head + lane * 4, ok);
-        float s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
-#pragma unroll
-        for (int e = 16; e > 0; e >>= 1) s += __shfl_xor_sync(0xffffffffu, s, e);
-        const float4 v = load4<H>(
-            a.v_cache.p, p * a.v_cache.page + (j & mask) * a.v_cache.tok + kh * a.v_cache.head + lane * 4, ok);
-        const float up = fmaxf(m, s), c = exp2f(m - up), x = exp2f(s - up);
-        m = up;
-        l = l * c + x;
-        o = make_float4(o.x * c + x * v.x, o.y * c + x * v.y, o.z * c + x * v.z, o.w * c + x * v.w);
-    }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    if (live) *reinterpret_cast<float4*>(part_o + row * a.dim + lane * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (lane == 0) part_lse[row] = m + log2f(l);
+void launch_own(const SharedArgs& a, const OwnPlan& pl, float* part_o, float* part_lse, cudaStream_t st) {
+    const long long blocks = (long long)a.n_requests * a.kv_heads * ((a.heads / a.kv_heads + 15) / 16) * pl.splits;
+    if (blocks > 0x7fffffffLL) throw CudaError("attention: too many requests for one launch");
+    if (a.dim <= 64)
+        own_pages_kernel<H, 64><<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl.splits, pl.chunk, part_o, part_lse);
+    else
+        own_pages_kernel<H, 128><<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl.splits, pl.chunk, part_o, part_lse);
+    VGPU_LAUNCH("own_pages_kernel");
 }
 
 // ---------------------------------------------------------------------------------
@@ -260,14 +465,15 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
 
 size_t shared_attention_workspace(const SharedArgs& a) {
     if (a.n_requests == 0) return 0;
-    return part_bytes(1 + (a.prefix_len ? shared_splits(a) : 0), (long long)a.n_requests * a.heads, a.dim);
+    return part_bytes(own_plan(a).splits + (a.prefix_len ? shared_splits(a) : 0), (long long)a.n_requests * a.heads, a.dim);
 }
 
 void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
     const long long rows = (long long)a.n_requests * a.heads;
     const int splits = a.prefix_len ? shared_splits(a) : 0;
+    const OwnPlan own = own_plan(a);
     float* part_o = static_cast<float*>(a.workspace);
-    float* part_lse = part_o + (splits + 1) * rows * a.dim;
+    float* part_lse = part_o + (splits + own.splits) * rows * a.dim;
     if (splits) {
         TileParams p{};
         fill_queries(p, a.f16, a.q, a.heads, a.kv_heads, a.dim, a.n_requests);
@@ -285,13 +491,13 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
         p.part_lse = part_lse;
         launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * splits, st);
     }
-    const int blocks = ceil_div(rows, kWarps);
-    float* own_o = part_o + splits * rows * a.dim;
-    float* own_lse = part_lse + splits * rows;
-    if (a.f16) own_rows_kernel<F16><<<blocks, kWarps * 32, 0, st>>>(a, own_o, own_lse);
-    else own_rows_kernel<Bf16><<<blocks, kWarps * 32, 0, st>>>(a, own_o, own_lse);
-    VGPU_LAUNCH("own_rows_kernel");
-    launch_join(a.f16, splits + 1, rows, a.dim, part_o, part_lse, a.out, a.lse, st);
+    if (own.splits) {
+        float* own_o = part_o + splits * rows * a.dim;
+        float* own_lse = part_lse + splits * rows;
+        if (a.f16) launch_own<F16>(a, own, own_o, own_lse, st);
+        else launch_own<Bf16>(a, own, own_o, own_lse, st);
+    }
+    launch_join(a.f16, splits + own.splits, rows, a.dim, part_o, part_lse, a.out, a.lse, st);
 }
 
 }  // namespace vgpu
