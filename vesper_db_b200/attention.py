@@ -14,6 +14,7 @@ from torch's allocator in that stream's order.  Arguments that do not fit raise 
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import NamedTuple
 
@@ -40,22 +41,31 @@ class PageTables(NamedTuple):
     used: torch.Tensor       # [1] int32: pages that the batch takes from the free list
 
 
+# Entry points of the library, resolved on the first call.
+_lib = None
+
+
+def _entries():
+    global _lib
+    _lib = N.load()
+    return _lib
+
+
 def _refuse(why: str):
     raise VesperError(N.VESPER_ERROR_INVALID_PARAM, why)
 
 
-def _on(t: torch.Tensor, device: torch.device, dtype: torch.dtype, name: str) -> torch.Tensor:
+def _wrong(t: torch.Tensor, device: torch.device, dtype: torch.dtype, name: str):
     if t.device != device:
         _refuse(f"{name} is on {t.device}, not on {device}")
-    if t.dtype != dtype:
-        _refuse(f"{name} is {t.dtype}, {dtype} expected")
-    return t
+    _refuse(f"{name} is {t.dtype}, {dtype} expected")
 
 
 def _ints(t: torch.Tensor, device: torch.device, name: str, n: int | None = None, dtype=torch.int32) -> int:
-    """Address of a contiguous vector of whole numbers."""
-    _on(t, device, dtype, name)
-    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+    """Address of a contiguous vector, of whole numbers unless dtype says otherwise."""
+    if t.dtype is not dtype or t.device != device:
+        _wrong(t, device, dtype, name)
+    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
         _refuse(f"{name} must be a contiguous vector" + ("" if n is None else f" of {n}"))
     return t.data_ptr()
 
@@ -66,47 +76,87 @@ def _cuda(t: torch.Tensor, name: str) -> torch.device:
     return t.device
 
 
-def _strides(t: torch.Tensor, name: str) -> tuple[int, ...]:
+def _odd_strides(t: torch.Tensor, name: str) -> tuple[int, ...]:
     """All strides but the last, which must be 1; those of single-element dims do not matter."""
-    shape, st = t.shape, t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         _refuse(f"{name}: the last dimension must be contiguous")
-    return tuple(s if n > 1 else 8 for n, s in zip(shape[:-1], st))
+    return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:-1], t.stride()))
 
 
 def _heads(t: torch.Tensor, device, dtype, name: str, tokens: int | None, heads: int | None, dim: int):
     """(address, token stride, head stride) of a [tokens, heads, dim] tensor."""
-    _on(t, device, dtype, name)
-    if t.dim() != 3 or t.shape[2] != dim or (tokens is not None and t.shape[0] != tokens) or \
-            (heads is not None and t.shape[1] != heads):
-        _refuse(f"{name} has shape {tuple(t.shape)}: [tokens, heads, head_dim] in line with q expected")
-    return (t.data_ptr(), *_strides(t, name))
+    if t.dtype is not dtype or t.device != device:
+        _wrong(t, device, dtype, name)
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or \
+            (heads is not None and shape[1] != heads):
+        _refuse(f"{name} has shape {tuple(shape)}: [tokens, heads, head_dim] in line with q expected")
+    a, b, c = t.stride()
+    if c != 1 or a % 8 or b % 8:
+        a, b = _odd_strides(t, name)
+    return t.data_ptr(), a, b
+
+
+def _queries(q: torch.Tensor):
+    """Device, dtype code, shape and fields of q."""
+    dev, dt = _cuda(q, "q"), _DTYPES.get(q.dtype)
+    if dt is None or q.dim() != 3:
+        _refuse("q must be bf16 or f16, [tokens, heads, head_dim]")
+    t, heads, dim = q.shape
+    a, b, c = q.stride()
+    if c != 1 or a % 8 or b % 8:
+        a, b = _odd_strides(q, "q")
+    return dev, dt, t, heads, dim, (q.data_ptr(), a, b)
 
 
 def _caches(k_cache, v_cache, device, dtype, kv_heads: int | None, dim: int):
     """Fields of both caches, then pages and page size."""
-    _on(k_cache, device, dtype, "k_cache")
-    _on(v_cache, device, dtype, "v_cache")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != dim or \
-            (kv_heads is not None and k_cache.shape[2] != kv_heads):
-        _refuse(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)}: "
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype is not dtype or t.device != device:
+            _wrong(t, device, dtype, name)
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or shape[3] != dim or (kv_heads is not None and shape[2] != kv_heads):
+        _refuse(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)}: "
                 "[pages, page_size, kv_heads, head_dim] in line with q expected")
-    return (k_cache.data_ptr(), *_strides(k_cache, "k_cache"), v_cache.data_ptr(), *_strides(v_cache, "v_cache"),
-            k_cache.shape[0], k_cache.shape[1])
+    a, b, c, d = k_cache.stride()
+    e, f, g, h = v_cache.stride()
+    if d != 1 or h != 1 or (a | b | c | e | f | g) % 8:
+        a, b, c = _odd_strides(k_cache, "k_cache")
+        e, f, g = _odd_strides(v_cache, "v_cache")
+    return k_cache.data_ptr(), a, b, c, v_cache.data_ptr(), e, f, g, shape[0], shape[1]
+
+
+def _table(table: torch.Tensor, device, n: int):
+    """Address, width and row stride of a [n, width] table."""
+    if table.dtype is not torch.int32 or table.device != device:
+        _wrong(table, device, torch.int32, "table")
+    if table.dim() != 2 or table.shape[0] != n or (table.shape[1] > 1 and table.stride(1) != 1):
+        _refuse("table must be [requests, width] with contiguous rows")
+    width = table.shape[1]
+    return table.data_ptr(), width, table.stride(0) if n > 1 else width
 
 
 def _call(fn, params: bytes, device: torch.device) -> None:
-    if device.index == torch.cuda.current_device():
-        status = fn(params, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)  # the address of torch.cuda.current_stream(device)
+    if index == torch.cuda.current_device():
+        status = fn(params, stream)
     else:  # the library launches on the calling thread's device
         with torch.cuda.device(device):
-            status = fn(params, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(params, stream)
     if status != N.VESPER_OK:
-        _check(N.load(), status)
+        _check(_lib, status)
 
 
-def _workspace(need: int, device: torch.device):
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+@functools.lru_cache(maxsize=4096)
+def _prompt_workspace(*sizes) -> int:
+    return _lib.vesper_prompt_attention_workspace(_PROMPT.pack(*sizes, *(0,) * 15))
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace(head: tuple, n_pages: int, page_size: int, prefix_len: int, width: int) -> int:
+    return _lib.vesper_shared_prefix_attention_workspace(
+        _SHARED.pack(*head, *(0,) * 11, n_pages, page_size, 0, prefix_len, 0, width, *(0,) * 6))
 
 
 def page_tables(cached: torch.Tensor, fresh: torch.Tensor, free: torch.Tensor, table: torch.Tensor, page_size: int,
@@ -120,21 +170,16 @@ def page_tables(cached: torch.Tensor, fresh: torch.Tensor, free: torch.Tensor, t
     """
     dev = _cuda(cached, "cached")
     n = cached.shape[0] if cached.dim() == 1 else _refuse("cached must be a vector")
-    c, f = _ints(cached, dev, "cached", n), _ints(fresh, dev, "fresh", n)
-    fr = _ints(free, dev, "free")
-    _on(table, dev, torch.int32, "table")
-    if table.dim() != 2 or table.shape[0] != n or (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse("table must be [requests, width] with contiguous rows")
+    c, f, fr = _ints(cached, dev, "cached", n), _ints(fresh, dev, "fresh", n), _ints(free, dev, "free")
     if total < 0 or page_size < 0:
         _refuse("total and page_size must not be negative")
-    width = table.shape[1]
-    ints = torch.empty(2 * n + 2 + total, dtype=torch.int32, device=dev)
-    lengths, starts, positions, used = ints[:n], ints[n:2 * n + 1], ints[2 * n + 1:-1], ints[-1:]
-    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    ints = cached.new_empty(2 * n + 2 + total)
+    slots = cached.new_empty(total, dtype=torch.int64)
     p = ints.data_ptr()
-    _call(N.load().vesper_page_tables_device, _TABLES.pack(
-        _TABLES.size, c, f, n, fr, free.shape[0], table.data_ptr(), width, table.stride(0) if n > 1 else width,
-        page_size, total, base, p, p + 4 * n, p + 8 * n + 4, slots.data_ptr(), p + 8 * n + 4 + 4 * total), dev)
+    _call((_lib or _entries()).vesper_page_tables_device, _TABLES.pack(
+        _TABLES.size, c, f, n, fr, free.shape[0], *_table(table, dev, n), page_size, total, base, p, p + 4 * n,
+        p + 8 * n + 4, slots.data_ptr(), p + 8 * n + 4 + 4 * total), dev)
+    lengths, starts, positions, used = ints.split((n, n + 1, total, 1))
     return PageTables(table, lengths, starts, positions, slots, used)
 
 
@@ -150,24 +195,15 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positi
     With slots (int64 [tokens], -1: skip), keys and values go to the caches.  Returns (q, k) as new contiguous tensors,
     k None without keep_k.
     """
-    dev = _cuda(q, "q")
-    dt = _DTYPES.get(q.dtype)
-    if dt is None or q.dim() != 3:
-        _refuse("q must be bf16 or f16, [tokens, heads, head_dim]")
-    t, heads, dim = q.shape
-    fq = _heads(q, dev, q.dtype, "q", t, heads, dim)
+    dev, dt, t, heads, dim, fq = _queries(q)
     fk = _heads(k, dev, q.dtype, "k", t, None, dim)
     kv = k.shape[1]
+    if turns.dtype is not torch.float32 or turns.device != dev:
+        _wrong(turns, dev, torch.float32, "turns")
     if turns.dim() != 2 or not turns.is_contiguous():
         _refuse("turns must be [positions, turned], contiguous")
-    _on(turns, dev, torch.float32, "turns")
-    weights = []
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _on(w, dev, q.dtype, name)
-            if w.shape != (dim,) or not w.is_contiguous():
-                _refuse(f"{name} must be a contiguous vector of head_dim")
-        weights.append(0 if w is None else w.data_ptr())
+    wq = 0 if q_weight is None else _ints(q_weight, dev, "q_weight", dim, q.dtype)
+    wk = 0 if k_weight is None else _ints(k_weight, dev, "k_weight", dim, q.dtype)
     if slots is not None:
         if v is None or k_cache is None or v_cache is None:
             _refuse("slots need v, k_cache and v_cache")
@@ -176,11 +212,11 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positi
         fc = _caches(k_cache, v_cache, dev, q.dtype, kv, dim)
     else:
         fs, fv, fc = 0, (0, 0, 0), (0,) * 10
-    out_q = torch.empty((t, heads, dim), dtype=q.dtype, device=dev)
-    out_k = torch.empty((t, kv, dim), dtype=q.dtype, device=dev) if keep_k else None
-    _call(N.load().vesper_norm_rotate_device, _ROTATE.pack(
+    out_q = q.new_empty((t, heads, dim))
+    out_k = q.new_empty((t, kv, dim)) if keep_k else None
+    _call((_lib or _entries()).vesper_norm_rotate_device, _ROTATE.pack(
         _ROTATE.size, dt, t, heads, kv, dim, turns.shape[1], 1 if pairs else 0, eps, *fq, *fk, *fv,
-        _ints(positions, dev, "positions", t), turns.data_ptr(), turns.shape[0], *weights, fs, *fc, out_q.data_ptr(),
+        _ints(positions, dev, "positions", t), turns.data_ptr(), turns.shape[0], wq, wk, fs, *fc, out_q.data_ptr(),
         out_k.data_ptr() if keep_k else 0), dev)
     return out_q, out_k
 
@@ -196,12 +232,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     [tokens, heads, head_dim], with stats (out, lse): the float32 [tokens, heads] log-sum-exp.  Rows that see no key
     are zero, their lse -inf.
     """
-    dev = _cuda(q, "q")
-    dt = _DTYPES.get(q.dtype)
-    if dt is None or q.dim() != 3:
-        _refuse("q must be bf16 or f16, [tokens, heads, head_dim]")
-    t, heads, dim = q.shape
-    fq = _heads(q, dev, q.dtype, "q", t, heads, dim)
+    dev, dt, t, heads, dim, fq = _queries(q)
     fk = _heads(k, dev, q.dtype, "k", None, None, dim)
     n_k, kv = k.shape[0], k.shape[1]
     fv = _heads(v, dev, q.dtype, "v", n_k, kv, dim)
@@ -210,17 +241,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     if n < 0:
         _refuse("starts must hold at least one entry")
     sk = 0 if starts_k is None else _ints(starts_k, dev, "starts_k", n + 1)
-    out = torch.empty((t, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((t, heads), dtype=torch.float32, device=dev) if stats else None
-    fields = [_PROMPT.size, dt, n, t, n_k, heads, kv, dim, 1 if causal else 0,
-              dim ** -0.5 if scale is None else scale, *fq, *fk, *fv, s, sk, out.data_ptr(),
-              lse.data_ptr() if stats else 0, 0, 0]
-    lib = N.load()
-    need = lib.vesper_prompt_attention_workspace(_PROMPT.pack(*fields))
-    if need:
-        ws = _workspace(need, dev)
-        fields[-2:] = ws.data_ptr(), need
-    _call(lib.vesper_prompt_attention_device, _PROMPT.pack(*fields), dev)
+    out = q.new_empty((t, heads, dim))
+    lse = q.new_empty((t, heads), dtype=torch.float32) if stats else None
+    lib = _lib or _entries()
+    sizes = (_PROMPT.size, dt, n, t, n_k, heads, kv, dim, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
+    need = _prompt_workspace(*sizes)
+    space = q.new_empty(need, dtype=torch.uint8) if need else None
+    _call(lib.vesper_prompt_attention_device, _PROMPT.pack(
+        *sizes, *fq, *fk, *fv, s, sk, out.data_ptr(), lse.data_ptr() if stats else 0, space.data_ptr() if need else 0,
+        need), dev)
     return (out, lse) if stats else out
 
 
@@ -233,29 +262,19 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     hold the prefix_len tokens all requests begin with; table int32 [requests, width] and lengths int32 [requests]: the
     pages and the count of each request's own tokens.  Returns out [requests, heads, head_dim], with stats (out, lse).
     """
-    dev = _cuda(q, "q")
-    dt = _DTYPES.get(q.dtype)
-    if dt is None or q.dim() != 3:
-        _refuse("q must be bf16 or f16, [requests, heads, head_dim]")
-    b, heads, dim = q.shape
-    fq = _heads(q, dev, q.dtype, "q", b, heads, dim)
+    dev, dt, b, heads, dim, fq = _queries(q)
     fc = _caches(k_cache, v_cache, dev, q.dtype, None, dim)
     pages = _ints(prefix_pages, dev, "prefix_pages")
-    if prefix_len < 0 or prefix_pages.shape[0] * fc[-1] < prefix_len:
+    if prefix_len < 0 or prefix_pages.shape[0] * fc[9] < prefix_len:
         _refuse("prefix_pages do not hold prefix_len tokens")
-    _on(table, dev, torch.int32, "table")
-    if table.dim() != 2 or table.shape[0] != b or (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse("table must be [requests, width] with contiguous rows")
-    width = table.shape[1]
-    out = torch.empty((b, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((b, heads), dtype=torch.float32, device=dev) if stats else None
-    fields = [_SHARED.size, dt, b, heads, k_cache.shape[2], dim, dim ** -0.5 if scale is None else scale, *fq, *fc,
-              pages, prefix_len, table.data_ptr(), width, table.stride(0) if b > 1 else width,
-              _ints(lengths, dev, "lengths", b), out.data_ptr(), lse.data_ptr() if stats else 0, 0, 0]
-    lib = N.load()
-    need = lib.vesper_shared_prefix_attention_workspace(_SHARED.pack(*fields))
-    if need:
-        ws = _workspace(need, dev)
-        fields[-2:] = ws.data_ptr(), need
-    _call(lib.vesper_shared_prefix_attention_device, _SHARED.pack(*fields), dev)
+    ft = _table(table, dev, b)
+    out = q.new_empty((b, heads, dim))
+    lse = q.new_empty((b, heads), dtype=torch.float32) if stats else None
+    lib = _lib or _entries()
+    head = (_SHARED.size, dt, b, heads, k_cache.shape[2], dim, dim ** -0.5 if scale is None else scale)
+    need = _shared_workspace(head, fc[8], fc[9], prefix_len, ft[1])
+    space = q.new_empty(need, dtype=torch.uint8) if need else None
+    _call(lib.vesper_shared_prefix_attention_device, _SHARED.pack(
+        *head, *fq, *fc, pages, prefix_len, *ft, _ints(lengths, dev, "lengths", b), out.data_ptr(),
+        lse.data_ptr() if stats else 0, space.data_ptr() if need else 0, need), dev)
     return (out, lse) if stats else out

@@ -242,7 +242,8 @@ void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
 
 void launch_page_tables(const PageTablesArgs& a, cudaStream_t st) {
     const size_t smem = 2 * ((size_t)a.n_requests + 1) * sizeof(int);
-    VGPU_CHECK(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024)
+        VGPU_CHECK(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const long long per_block = kScanThreads * 4;
     const long long want = std::max<long long>((a.n_tokens + per_block - 1) / per_block, (a.n_requests + 63) / 64);
     const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 2);
