@@ -115,18 +115,28 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t saddr, uint32_t block_b
     return d;
 }
 
+// Issued by one elected lane of a converged warp: the election inside the statement keeps
+// the operands in uniform registers.  (Under `if (lane == 0)` each product took 120 cycles
+// to issue, twice what it takes to run.)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar))
+        : "memory");
+}
+
 // What a block works on.
 struct Work {
     int q0;        // first row of q of the block's first tile
@@ -334,28 +344,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t id_s = common | ((uint32_t)(kKeys >> 3) << 17);
             constexpr uint32_t id_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-            const int steps = (p.dim + 15) / 16;  // of the score product: columns past dim are zero
             bool ok = true;
             auto wait = [&](uint64_t* b, uint32_t parity) {
                 if (ok) ok = mbar_wait(b, parity);
                 return ok;
             };
             auto scores = [&](int t, int slot) {
-                if (lane == 0) {
-                    const uint32_t a = s_q + t * kTileBytes, b = s_kv + slot * kTileBytes;
-                    for (int k = 0; k < steps; ++k) {
-                        const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                        mma_ss(tmem + t * 128, tc::sw128_kmajor_desc(a + off), tc::sw128_kmajor_desc(b + off), id_s, k > 0);
-                    }
-                    tc::commit(&s_full[t]);
+                const uint64_t a = tc::sw128_kmajor_desc(s_q + t * kTileBytes);
+                const uint64_t b = tc::sw128_kmajor_desc(s_kv + slot * kTileBytes);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {  // columns past dim are zero
+                    const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+                    mma_ss(tmem + t * 128, a + off, b + off, id_s, k > 0);
                 }
-                __syncwarp();
+                commit(&s_full[t]);
             };
             // Hands slot of item i back to the copies, unless they are done with it: an arrival
             // that nobody waits for could come after the block has gone.
             auto release = [&](int i) {
-                if (ok && i + kSlots < 2 * n && lane == 0) tc::commit(&kv_empty[i % kSlots]);
-                __syncwarp();
+                if (ok && i + kSlots < 2 * n) commit(&kv_empty[i % kSlots]);
             };
             if (n > 0) {
                 wait(&kv_full[0], 0);
@@ -379,14 +386,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 for (int t = 0; t < 2; ++t) {
                     if (j < nt[t] && wait(&p_full[t], j & 1)) {
                         tc::fence_after_sync();
-                        if (lane == 0) {
-                            const uint32_t b = s_kv + sv * kTileBytes;
-                            for (int k = 0; k < kKeys / 16; ++k)
-                                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, values_desc(b + k * 2048, kHalfBytes),
-                                       id_o, (j > 0 || k > 0) ? 1u : 0u);
-                            if (j + 1 == nt[t]) tc::commit(&o_full[t]);
-                        }
-                        __syncwarp();
+                        const uint64_t b = values_desc(s_kv + sv * kTileBytes, kHalfBytes);
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), id_o,
+                                   (j > 0 || k > 0) ? 1u : 0u);
+                        if (j + 1 == nt[t]) commit(&o_full[t]);
                     }
                     if (more && t == 0) wait(&kv_full[sk], (ik / kSlots) & 1);
                     if (ok && j + 1 < nt[t]) scores(t, sk);
@@ -395,8 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 if (more) release(ik);
             }
             if (!ok) {
-                if (lane == 0) tc::commit(drained);
-                __syncwarp();
+                commit(drained);
                 mbar_wait(drained, 0);
             }
         } else {

@@ -128,102 +128,121 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
 // Norm of each head, rotation, cache write.  x of one head (dim values):
 //   y = x * rsqrt(mean(x^2) + eps) * w, then for each pair (a, b) of the first `turned`
 //   values, a' = a cos - b sin, b' = b cos + a sin.
-// All of it in 32 bits, one rounding at the store.  A group of W lanes holds one head,
-// eight values (16 bytes) a lane; the partner of a half-split pair is in another lane of
-// the group.  One block a token: a lane's cosines, sines and weights serve all heads.
+// All of it in 32 bits, one rounding at the store.  Bound by reading and writing each row
+// once.  A group of W lanes holds one head, eight values (16 bytes) a lane; the partner of
+// a half-split pair is in another lane of the group.  A block takes whole tokens, so that a
+// lane's cosines and sines serve all heads and its weights all tokens; the rows of kBatch
+// heads are requested before the first of them is used.
 // ---------------------------------------------------------------------------------
 constexpr int kRotThreads = 256;
+constexpr int kBatch = 4;
 
 template <class H, int W, bool PAIRS>
-__global__ void __launch_bounds__(kRotThreads) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
-    const int t = blockIdx.x;
+__global__ void __launch_bounds__(kRotThreads, 3) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
+    using T = typename H::type;
     const int c = threadIdx.x % W;  // this lane's chunk of eight values
     const int group = threadIdx.x / W;
     constexpr int kGroups = kRotThreads / W;
-    const int chunks = a.dim / 8, half = a.turned / 2;
-    const bool live = c < chunks;
+    const int half = a.turned / 2, total = a.heads + 2 * a.kv_heads;
+    const bool live = c * 8 < a.dim, turns_here = c * 8 < a.turned;
+    // Angles of the chunk: half-split pairs use angle i % (turned / 2), neighbouring pairs
+    // angle i / 2.
+    const int angle = PAIRS ? c * 4 : (c * 8 < half ? c * 8 : c * 8 - half);
+    const int mate = !turns_here || PAIRS ? c : (c * 8 < half ? c + half / 8 : c - half / 8);
+    const float sign = c * 8 < half ? -1.0f : 1.0f;
+    uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+    if (live && a.q_weight) wq = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q_weight) + c * 8);
+    if (live && a.k_weight) wk = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_weight) + c * 8);
 
-    // Angles of the chunk: half-split pairs use angle i % (turned / 2), neighbouring
-    // pairs use angle i / 2.
-    float cs[8], sn[8], wq[8], wk[8];
-    const int pos = a.positions[t];
-    const bool known = pos >= 0 && pos < a.n_positions;
-    const bool turns_here = live && c * 8 < a.turned;
+    for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x) {
+        const int pos = a.positions[t];
+        int64_t slot = a.slots ? a.slots[t] : -1;
+        const bool known = pos >= 0 && pos < a.n_positions;
+        if (slot >= (a.n_pages << a.page_shift)) slot = -1;
+        const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
+        constexpr int kAngles = PAIRS ? 4 : 8;
+        float cs[kAngles], sn[kAngles];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = c * 8 + i;
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-        if (turns_here) {
-            const int ang = PAIRS ? e / 2 : (e < half ? e : e - half);
-            cs[i] = known ? a.turns[(long long)pos * a.turned + ang] : __int_as_float(0x7fc00000);
-            sn[i] = known ? a.turns[(long long)pos * a.turned + half + ang] : __int_as_float(0x7fc00000);
-        }
-        wq[i] = wk[i] = 1.0f;
-    }
-    using T = typename H::type;
-    if (live) {
-        if (a.q_weight) unpack8<H>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q_weight) + c * 8), wq);
-        if (a.k_weight) unpack8<H>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_weight) + c * 8), wk);
-    }
-    int64_t slot = a.slots ? a.slots[t] : -1;
-    if (slot >= (a.n_pages << a.page_shift)) slot = -1;
-    const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
-
-    const int total = a.heads + 2 * a.kv_heads;
-    for (int u0 = 0; u0 < total; u0 += kGroups) {  // uniform trip count: shuffles below
-        const int u = u0 + group;
-        const bool is_q = u < a.heads, is_k = !is_q && u < a.heads + a.kv_heads, is_v = !is_q && !is_k && u < total;
-        const int h = is_q ? u : (is_k ? u - a.heads : u - a.heads - a.kv_heads);
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live && u < total && !(is_v && slot < 0)) {
-            const HeadsView& x = is_q ? a.q : (is_k ? a.k : a.v);
-            raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(x.p) + t * x.tok + h * x.head + c * 8);
-        }
-        if (is_v) {  // values are copied as they are
-            if (live && slot >= 0)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok +
-                                          h * a.v_cache.head + c * 8) = raw;
-        }
-        float x[8];
-        unpack8<H>(raw, x);
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, W);
-        const bool scaled = is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
-        const float inv = scaled ? rsqrtf(ss / a.dim + a.eps) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (is_q ? wq[i] : wk[i]);
-        float y[8];
-        if (PAIRS) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                y[i] = turns_here ? x[i] * cs[i] - x[i + 1] * sn[i] : x[i];
-                y[i + 1] = turns_here ? x[i + 1] * cs[i] + x[i] * sn[i] : x[i + 1];
+        for (int i = 0; i < kAngles; i += 4) {
+            float4 x = make_float4(1, 1, 1, 1), y = make_float4(0, 0, 0, 0);
+            if (turns_here) {
+                const float nan = __int_as_float(0x7fc00000);
+                x = y = make_float4(nan, nan, nan, nan);
+                if (known) {
+                    const float* row = a.turns + (long long)pos * a.turned + angle + i;
+                    x = __ldg(reinterpret_cast<const float4*>(row));
+                    y = __ldg(reinterpret_cast<const float4*>(row + half));
+                }
             }
-        } else {
-            const int hc = half / 8;  // chunks of one half
-            const bool first = c < hc;
-            const int mate = turns_here ? (first ? c + hc : c - hc) : c;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float o = __shfl_sync(0xffffffffu, x[i], mate, W);
-                y[i] = turns_here ? (first ? x[i] * cs[i] - o * sn[i] : x[i] * cs[i] + o * sn[i]) : x[i];
-            }
+            cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
+            sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
         }
-        if (!live || u >= total || is_v) continue;
-        const uint4 r = pack8<H>(y);
-        if (is_q) {
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.out_q) + ((long long)t * a.heads + h) * a.dim + c * 8) = r;
-        } else {
-            if (a.out_k)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out_k) + ((long long)t * a.kv_heads + h) * a.dim + c * 8) =
-                    r;
-            if (slot >= 0)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok +
-                                          h * a.k_cache.head + c * 8) = r;
+        for (int u0 = group; u0 - group < total; u0 += kGroups * kBatch) {  // uniform trip count: shuffles below
+            uint4 raw[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int u = u0 + b * kGroups;
+                raw[b] = make_uint4(0, 0, 0, 0);
+                if (!live || u >= total) continue;
+                const T* src;
+                if (u < a.heads) src = static_cast<const T*>(a.q.p) + t * a.q.tok + u * a.q.head;
+                else if (u < a.heads + a.kv_heads) src = static_cast<const T*>(a.k.p) + t * a.k.tok + (u - a.heads) * a.k.head;
+                else if (slot < 0) continue;
+                else src = static_cast<const T*>(a.v.p) + t * a.v.tok + (u - a.heads - a.kv_heads) * a.v.head;
+                raw[b] = *reinterpret_cast<const uint4*>(src + c * 8);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int u = u0 + b * kGroups;
+                if (u0 - group + b * kGroups >= total) break;  // the same for the whole block
+                const bool is_q = u < a.heads, is_k = !is_q && u < a.heads + a.kv_heads;
+                float x[8], w[8];
+                unpack8<H>(raw[b], x);
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+                for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, W);
+                if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
+                    const float inv = rsqrtf(ss / a.dim + a.eps);
+                    unpack8<H>(is_q ? wq : wk, w);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+                }
+                float y[8];
+                if (PAIRS) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        y[i] = turns_here ? x[i] * cs[i / 2] - x[i + 1] * sn[i / 2] : x[i];
+                        y[i + 1] = turns_here ? x[i + 1] * cs[i / 2] + x[i] * sn[i / 2] : x[i + 1];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float o = __shfl_sync(0xffffffffu, x[i], mate, W);
+                        y[i] = turns_here ? x[i] * cs[i % kAngles] + sign * o * sn[i % kAngles] : x[i];
+                    }
+                }
+                if (!live || u >= total) continue;
+                if (!is_q && !is_k) {  // values are copied as they are
+                    if (slot >= 0)
+                        *reinterpret_cast<uint4*>(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok +
+                                                  (u - a.heads - a.kv_heads) * a.v_cache.head + c * 8) = raw[b];
+                    continue;
+                }
+                const uint4 r = pack8<H>(y);
+                if (is_q) {
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out_q) + ((long long)t * a.heads + u) * a.dim + c * 8) = r;
+                    continue;
+                }
+                const int h = u - a.heads;
+                if (a.out_k)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out_k) + ((long long)t * a.kv_heads + h) * a.dim + c * 8) = r;
+                if (slot >= 0)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok +
+                                              h * a.k_cache.head + c * 8) = r;
+            }
+            __syncwarp();
         }
     }
 }
@@ -231,7 +250,7 @@ __global__ void __launch_bounds__(kRotThreads) norm_rotate_kernel(const __grid_c
 template <class H, bool PAIRS>
 void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
     const int chunks = a.dim / 8;
-    const dim3 grid((unsigned)a.n_tokens);
+    const unsigned grid = (unsigned)std::min(a.n_tokens, 148 * 3 * 8);  // a few tokens a block where there are many
     if (chunks <= 8) norm_rotate_kernel<H, 8, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
     else if (chunks <= 16) norm_rotate_kernel<H, 16, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
     else norm_rotate_kernel<H, 32, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
