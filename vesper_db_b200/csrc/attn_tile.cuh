@@ -8,13 +8,18 @@
 // head each, so that one key tile serves the whole group.  A block holds two query tiles
 // and takes the keys 128 at a time:
 //   * warp 8 copies Q, then K and V tiles by TMA into a ring of shared-memory slots;
-//   * warp 9 issues the products: S_t = Q_t K^T (both operands from shared memory) and
-//     O_t += P_t V (P from tensor memory);
+//   * warps 9 and 10 issue the products of tile 0 and tile 1: S_t = Q_t K^T (both operands
+//     from shared memory) and O_t += P_t V (P from tensor memory);
 //   * warps 0-3 and 4-7 hold one row a thread of tile 0 and tile 1: they read S, keep m and
-//     l, and write P over S as 16-bit values;
-//   * warps 10 and 11 clean the value tiles that hold keys some row must not see.
-// The two query tiles alternate: while one is in the tensor cores the other is in the
-// exponentials.  Tensor memory: S0, S1 (128 columns each), O0, O1.
+//     l, and write P over S as 16-bit values, in two halves, so that the first half's
+//     product runs while the second half is made;
+//   * warps 12 to 15 clean the value tiles that hold keys some row must not see.
+// The two query tiles are independent of each other: while one is in the tensor cores the
+// other is in the exponentials.  Tensor memory: S0, S1 (128 columns each), O0, O1.
+//
+// What bounds it: a pair of tiles takes 2,048 cycles in the tensor cores (heads of 128) and
+// as many in the special-function units if these make all exponentials (32,768 at 16 a
+// cycle).  So three in eight are made by the FMA units instead, see exp2_pair.
 //
 // m only moves when a row's maximum has grown by more than 2^8: until then P may reach 2^8,
 // which both types hold at full relative precision, and O need not be rescaled.
@@ -30,6 +35,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "half_types.cuh"
@@ -40,10 +47,10 @@ namespace attn {
 
 constexpr int kRows = 128;     // query rows of a tile
 constexpr int kKeys = 128;     // keys of a tile
-constexpr int kThreads = 384;  // two softmax warpgroups, one of service warps
+constexpr int kThreads = 512;  // two softmax warpgroups, two of service warps
 constexpr int kSlots = 4;      // K and V tiles in flight
 constexpr float kGrow = 8.0f;  // log2 of how far P may pass 1 before O is rescaled
-constexpr int kSoftmaxRegs = 224, kServiceRegs = 40;  // 2 * 128 * 224 + 128 * 40 <= 384 * 168
+constexpr int kSoftmaxRegs = 208, kServiceRegs = 40;  // 256 * 208 + 256 * 40 <= 512 * 128
 
 struct TileParams {
     CUtensorMap mq, mk, mv;
@@ -71,7 +78,7 @@ struct TileParams {
 
 template <int D>
 constexpr int smem_bytes() {
-    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 256;
+    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512;
 }
 
 // Bounded wait for the barrier's phase; false when it ran out (a tile takes microseconds).
@@ -95,6 +102,53 @@ __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+// Packed pairs of 32-bit floats: one instruction for two.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Maximum of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two values of at most 2^kGrow on the FMA units: x = n + f with n the nearest whole
+// number (adding and taking away 1.5 * 2^23 rounds to it, and leaves n in the low bits of the
+// sum), 2^f by the polynomial of degree 4 with the least largest relative error on
+// [-1/2, 1/2] (2.6e-6, found by Remez exchange), and n added to the exponent.  Below 2^-126
+// it gives 2^-126, which no sum here notices: it is used on tiles without masked keys only.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+    const float2 h = halves(x);
+    x = pair(fmaxf(h.x, -126.0f), fmaxf(h.y, -126.0f));
+    const uint64_t t = add2(x, pair(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), x);
+    uint64_t r = fma2(f, pair(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    r = fma2(r, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    r = fma2(r, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    r = fma2(r, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    const float2 a = halves(t), b = halves(r);
+    return pair(__int_as_float(__float_as_int(b.x) + (__float_as_int(a.x) << 23)),
+                __int_as_float(__float_as_int(b.y) + (__float_as_int(a.y) << 23)));
 }
 
 __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -223,10 +277,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     uint64_t* const kv_full = bars + 2;           // [kSlots]
     uint64_t* const kv_empty = kv_full + kSlots;  // [kSlots]
     uint64_t* const s_full = kv_empty + kSlots;   // [2]
-    uint64_t* const p_full = s_full + 2;          // [2]
-    uint64_t* const o_full = p_full + 2;          // [2]
-    uint64_t* const drained = o_full + 2;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    uint64_t* const p_full = s_full + 2;          // [2][2]: tile, half of the keys
+    uint64_t* const turn = p_full + 4;            // [2]
+    uint64_t* const o_full = turn + 2;            // [2]
+    uint64_t* const drained = o_full + 2;         // [2]
+    uint64_t* const clean = drained + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(clean + 1);
     int* const s_leak = reinterpret_cast<int*>(tmem_slot + 1);
     Work* const s_work = reinterpret_cast<Work*>(tmem_slot + 2);
 
@@ -253,14 +309,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             for (int i = 0; i < 2; ++i) {
                 tc::mbar_init(&q_full[i], 1);
                 tc::mbar_init(&s_full[i], 1);
-                tc::mbar_init(&p_full[i], 128);
+                tc::mbar_init(&p_full[2 * i], 128);
+                tc::mbar_init(&p_full[2 * i + 1], 128);
+                tc::mbar_init(&turn[i], 1);
                 tc::mbar_init(&o_full[i], 1);
+                tc::mbar_init(&drained[i], 1);
             }
             for (int i = 0; i < kSlots; ++i) {
                 tc::mbar_init(&kv_full[i], 1);
-                tc::mbar_init(&kv_empty[i], 1);
+                tc::mbar_init(&kv_empty[i], 2);  // both warps of products
             }
-            tc::mbar_init(drained, 1);
+            tc::mbar_init(clean, 4);
             *s_leak = 0;
             tc::mbar_init_fence();
         }
@@ -338,91 +397,96 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 if (!ok)  // nothing may land after the block has gone
                     for (int e = max(i - kSlots, 0); e < i; ++e) mbar_wait(&kv_full[e % kSlots], (e / kSlots) & 1);
             }
-        } else if (warp == 9) {
-            // ---------------------------------------------------------------- products
+        } else if (warp == 9 || warp == 10) {
+            // ---------------------------------------------------------------- products of tile t
             constexpr uint32_t fmt = std::is_same<H, Bf16>::value ? 1u : 0u;
             constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t id_s = common | ((uint32_t)(kKeys >> 3) << 17);
             constexpr uint32_t id_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+            const int t = warp - 9, mine = t ? nt[1] : nt[0];
+            const uint32_t t_s = tmem + t * 128, t_o = tmem + 256 + t * 128;
+            const uint64_t q_desc = tc::sw128_kmajor_desc(s_q + t * kTileBytes);
             bool ok = true;
             auto wait = [&](uint64_t* b, uint32_t parity) {
                 if (ok) ok = mbar_wait(b, parity);
                 return ok;
             };
-            auto scores = [&](int t, int slot) {
-                const uint64_t a = tc::sw128_kmajor_desc(s_q + t * kTileBytes);
+            auto scores = [&](int slot) {
                 const uint64_t b = tc::sw128_kmajor_desc(s_kv + slot * kTileBytes);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {  // columns past dim are zero
                     const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-                    mma_ss(tmem + t * 128, a + off, b + off, id_s, k > 0);
+                    mma_ss(t_s, q_desc + off, b + off, id_s, k > 0);
                 }
                 commit(&s_full[t]);
             };
-            // Hands slot of item i back to the copies, unless they are done with it: an arrival
-            // that nobody waits for could come after the block has gone.
+            // Hands the slot of item i back to the copies, unless they are done with it: an
+            // arrival that nobody waits for could come after the block has gone.
             auto release = [&](int i) {
                 if (ok && i + kSlots < 2 * n) commit(&kv_empty[i % kSlots]);
             };
-            if (n > 0) {
-                wait(&kv_full[0], 0);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    if (nt[t] > 0 && wait(&q_full[t], 0)) {
-                        tc::fence_after_sync();
-                        scores(t, 0);
-                    }
-                release(0);
+            // A warp without rows of its own follows the same waits: it hands a slot back only
+            // after what the slot holds has landed.
+            if (mine > 0) wait(&q_full[t], 0);
+            if (n > 0 && wait(&kv_full[0], 0) && mine > 0) {
+                tc::fence_after_sync();
+                scores(0);
             }
+            release(0);
+            // The two warps take turns, one product of values and the next of scores each: left
+            // to themselves the tiles fall into step, both in the exponentials and then both in
+            // the tensor cores, and half the time of each is lost.
+            int cleaned = 0;
             for (int j = 0; j < n; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % kSlots, sk = ik % kSlots;
                 wait(&kv_full[sv], (iv / kSlots) & 1);
                 if (guarded_tile(j)) {
-                    asm volatile("bar.sync 1, 96;" ::: "memory");
-                    asm volatile("bar.sync 2, 96;" ::: "memory");
+                    asm volatile("bar.arrive 1, 192;" ::: "memory");
+                    wait(clean, cleaned++ & 1);
                 }
-                const bool more = j + 1 < n;
+                if (t == 1 || j > 0) wait(&turn[t], t == 1 ? j & 1 : (j - 1) & 1);
+                if (j < mine) {
+                    const uint64_t b = values_desc(s_kv + sv * kTileBytes, kHalfBytes);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (j < nt[t] && wait(&p_full[t], j & 1)) {
+                    for (int h = 0; h < 2; ++h) {  // halves of P
+                        if (!wait(&p_full[2 * t + h], j & 1)) break;
                         tc::fence_after_sync();
-                        const uint64_t b = values_desc(s_kv + sv * kTileBytes, kHalfBytes);
 #pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), id_o,
-                                   (j > 0 || k > 0) ? 1u : 0u);
-                        if (j + 1 == nt[t]) commit(&o_full[t]);
+                        for (int k = h * 4; k < h * 4 + 4; ++k)
+                            mma_ts(t_o, t_s + k * 8, b + k * (2048 >> 4), id_o, (j > 0 || k > 0) ? 1u : 0u);
                     }
-                    if (more && t == 0) wait(&kv_full[sk], (ik / kSlots) & 1);
-                    if (ok && j + 1 < nt[t]) scores(t, sk);
+                    if (ok && j + 1 == mine) commit(&o_full[t]);
                 }
+                if (j + 1 < n && wait(&kv_full[sk], (ik / kSlots) & 1) && j + 1 < mine) scores(sk);
+                if (lane == 0) tc::mbar_arrive(&turn[t ^ 1]);
                 release(iv);
-                if (more) release(ik);
+                if (j + 1 < n) release(ik);
             }
             if (!ok) {
-                commit(drained);
-                mbar_wait(drained, 0);
+                commit(&drained[t]);
+                mbar_wait(&drained[t], 0);
             }
-        } else {
+        } else if (warp >= 12) {
             // ---------------------------------------------------------------- value rows that not every row sees
-            const int g = tid - 320;
+            const int g = tid - 384;
             for (int j = 0; j < n; ++j) {
                 if (!guarded_tile(j)) continue;
-                asm volatile("bar.sync 1, 96;" ::: "memory");
+                asm volatile("bar.sync 1, 192;" ::: "memory");  // both warps of products have seen the tile land
                 uint8_t* const v = smem + (2 + (2 * j + 1) % kSlots) * kTileBytes;
                 const int key = (j0 + j) * kKeys;
                 const int end = min(max(w.len_k - key, 0), kKeys), from = max(min_lim - key, 0);
                 bool bad = false;
                 if (!PAGED)
-                    for (int i = g; i < (end - from) * 8; i += 64)
+                    for (int i = g; i < (end - from) * 8; i += 128)
                         for (int h = 0; h < kHalves; ++h)
                             bad |= not_finite<H>(*reinterpret_cast<const uint4*>(v + h * kHalfBytes + from * 128 + i * 16));
-                for (int i = g; i < (kKeys - end) * 8; i += 64)
+                for (int i = g; i < (kKeys - end) * 8; i += 128)
                     for (int h = 0; h < kHalves; ++h)
                         *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
                 if (bad) *s_leak = 1;
                 tc::fence_proxy_async_smem();
-                asm volatile("bar.sync 2, 96;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(clean);
             }
         }
     } else {
@@ -457,16 +521,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             float mx[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                mx[c] = __uint_as_float(s[c][0]);
+                auto f = [&](int i) { return __uint_as_float(s[c][i]); };
+                mx[c] = max3(f(0), f(1), f(2));
 #pragma unroll
-                for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+                for (int i = 3; i < 31; i += 2) mx[c] = max3(mx[c], f(i), f(i + 1));
+                mx[c] = max3(mx[c], mx[c], f(31));
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
             if (j == 0) {
-                m = top;
-            } else if (__any_sync(0xffffffffu, top - m > kGrow)) {
-                const float up = top - m > kGrow ? top : m;
-                const float f = top - m > kGrow ? ex2(m - up) : 1.0f;
+                m = top == INFINITY ? __int_as_float(0x7fc00000) : top;
+            } else if (__any_sync(0xffffffffu, !(top - m <= kGrow))) {
+                // Grown too far, or NaN (a score is NaN or infinite, or the row has seen no key)
+                float up = !(top - m <= kGrow) ? top : m;
+                if (up == INFINITY) up = __int_as_float(0x7fc00000);
+                const float f = m == up ? 1.0f : ex2(m - up);
                 m = up;
                 l *= f;
 #pragma unroll 1
@@ -480,23 +548,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
             }
             const float ref = m == -INFINITY ? 0.0f : m;
-            float sum[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < 4; c += 2) {
+            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), ref2 = pair(-ref, -ref);
+            uint64_t sum[4] = {0, 0, 0, 0};
+            auto half = [&](auto masked, int c) {  // 64 keys
                 uint32_t pk[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const float a = ex2(fmaf(__uint_as_float(s[c + i / 16][(2 * i) & 31]), p.scale_log2, -ref));
-                    const float b = ex2(fmaf(__uint_as_float(s[c + i / 16][(2 * i + 1) & 31]), p.scale_log2, -ref));
-                    sum[i & 3] += a + b;
-                    pk[i] = H::pack(a, b);
+                    const uint32_t* e = &s[c + i / 16][(2 * i) & 31];
+                    uint64_t x = fma2(pair(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, ref2);
+                    if (!masked && (i % 8 == 1 || i % 8 == 4 || i % 8 == 6)) {
+                        x = exp2_pair(x);
+                    } else {
+                        const float2 h = halves(x);
+                        x = pair(ex2(h.x), ex2(h.y));
+                    }
+                    sum[i & 3] = add2(sum[i & 3], x);
+                    const float2 h = halves(x);
+                    pk[i] = H::pack(h.x, h.y);
                 }
                 tc::tmem_st32(ts + c * 16, pk);
+                tc::tmem_st_wait();
+                tc::fence_before_sync();
+                tc::mbar_arrive(&p_full[2 * t + c / 2]);
+            };
+            if (key + kKeys > tile_lim) {
+                half(std::true_type{}, 0);
+                half(std::true_type{}, 2);
+            } else {
+                half(std::false_type{}, 0);
+                half(std::false_type{}, 2);
             }
-            tc::tmem_st_wait();
-            tc::fence_before_sync();
-            tc::mbar_arrive(&p_full[t]);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float2 s01 = halves(add2(sum[0], sum[1])), s23 = halves(add2(sum[2], sum[3]));
+            l += (s01.x + s01.y) + (s23.x + s23.y);
         }
         if (ok && my_tiles > 0) ok = mbar_wait(&o_full[t], 0);
         tc::fence_after_sync();

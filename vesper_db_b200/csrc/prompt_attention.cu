@@ -79,7 +79,7 @@ void launch_tiles_as(const TileParams& p, long long blocks, cudaStream_t st) {
         cudaFuncAttributes fa;
         VGPU_CHECK(cudaFuncGetAttributes(&fa, kernel));
         // the softmax warps' registers come out of what the block is launched with
-        if (fa.numRegs * kThreads < 256 * attn::kSoftmaxRegs + 128 * attn::kServiceRegs)
+        if (fa.numRegs * kThreads < 256 * (attn::kSoftmaxRegs + attn::kServiceRegs))
             throw CudaError("attn_tile_kernel: launched with too few registers for its split");
         return true;
     }();
