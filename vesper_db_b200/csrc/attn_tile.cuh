@@ -17,9 +17,11 @@
 // The two query tiles are independent of each other: while one is in the tensor cores the
 // other is in the exponentials.  Tensor memory: S0, S1 (128 columns each), O0, O1.
 //
-// What bounds it: a pair of tiles takes 2,048 cycles in the tensor cores (heads of 128) and
-// as many in the special-function units if these make all exponentials (32,768 at 16 a
-// cycle).  So three in eight are made by the FMA units instead, see exp2_pair.
+// What bounds it: a pair of tiles takes 2,048 cycles in the tensor cores (heads of 128), as
+// many in the special-function units (32,768 exponentials, 16 a cycle) and as many in
+// shared memory (256 KB read and written, 128 bytes a cycle).  Making a quarter or three
+// eighths of the exponentials by a polynomial on the FMA units instead cost 1 to 7 %: the
+// issue slots it takes are worth more than the special-function cycles it frees.
 //
 // m only moves when a row's maximum has grown by more than 2^8: until then P may reach 2^8,
 // which both types hold at full relative precision, and O need not be rescaled.
@@ -130,25 +132,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-// 2^x of two values of at most 2^kGrow on the FMA units: x = n + f with n the nearest whole
-// number (adding and taking away 1.5 * 2^23 rounds to it, and leaves n in the low bits of the
-// sum), 2^f by the polynomial of degree 4 with the least largest relative error on
-// [-1/2, 1/2] (2.6e-6, found by Remez exchange), and n added to the exponent.  Below 2^-126
-// it gives 2^-126, which no sum here notices: it is used on tiles without masked keys only.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-    const float2 h = halves(x);
-    x = pair(fmaxf(h.x, -126.0f), fmaxf(h.y, -126.0f));
-    const uint64_t t = add2(x, pair(12582912.0f, 12582912.0f));
-    const uint64_t f = fma2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), x);
-    uint64_t r = fma2(f, pair(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    r = fma2(r, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    r = fma2(r, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    r = fma2(r, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    const float2 a = halves(t), b = halves(r);
-    return pair(__int_as_float(__float_as_int(b.x) + (__float_as_int(a.x) << 23)),
-                __int_as_float(__float_as_int(b.y) + (__float_as_int(a.y) << 23)));
 }
 
 __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -548,35 +531,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
             }
             const float ref = m == -INFINITY ? 0.0f : m;
-            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), ref2 = pair(-ref, -ref);
+            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+            uint64_t ref2 = pair(-ref, -ref);
             uint64_t sum[4] = {0, 0, 0, 0};
-            auto half = [&](auto masked, int c) {  // 64 keys
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {  // halves of 64 keys
                 uint32_t pk[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     const uint32_t* e = &s[c + i / 16][(2 * i) & 31];
-                    uint64_t x = fma2(pair(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, ref2);
-                    if (!masked && (i % 8 == 1 || i % 8 == 4 || i % 8 == 6)) {
-                        x = exp2_pair(x);
-                    } else {
-                        const float2 h = halves(x);
-                        x = pair(ex2(h.x), ex2(h.y));
-                    }
-                    sum[i & 3] = add2(sum[i & 3], x);
-                    const float2 h = halves(x);
-                    pk[i] = H::pack(h.x, h.y);
+                    const float2 x = halves(fma2(pair(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, ref2));
+                    const float a = ex2(x.x), b = ex2(x.y);
+                    sum[i & 3] = add2(sum[i & 3], pair(a, b));
+                    pk[i] = H::pack(a, b);
                 }
                 tc::tmem_st32(ts + c * 16, pk);
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
                 tc::mbar_arrive(&p_full[2 * t + c / 2]);
-            };
-            if (key + kKeys > tile_lim) {
-                half(std::true_type{}, 0);
-                half(std::true_type{}, 2);
-            } else {
-                half(std::false_type{}, 0);
-                half(std::false_type{}, 2);
+                // the second half's exponentials stay behind this arrival
+                asm volatile("" : "+l"(ref2));
             }
             const float2 s01 = halves(add2(sum[0], sum[1])), s23 = halves(add2(sum[2], sum[3]));
             l += (s01.x + s01.y) + (s23.x + s23.y);
