@@ -128,132 +128,190 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
 // Norm of each head, rotation, cache write.  x of one head (dim values):
 //   y = x * rsqrt(mean(x^2) + eps) * w, then for each pair (a, b) of the first `turned`
 //   values, a' = a cos - b sin, b' = b cos + a sin.
-// All of it in 32 bits, one rounding at the store.  Bound by reading and writing each row
-// once.  A group of W lanes holds one head, eight values (16 bytes) a lane; the partner of
-// a half-split pair is in another lane of the group.  A block takes whole tokens, so that a
-// lane's cosines and sines serve all heads and its weights all tokens; the rows of kBatch
-// heads are requested before the first of them is used.
+// All of it in 32 bits, two values an instruction, one rounding at the store.  The bound is
+// reading and writing each row once; getting near it took fewer instructions rather than
+// more loads in flight.  A group of W lanes holds one head; a lane holds two chunks of eight
+// values that rotate into each other (half-split pairs: chunks l and l + turned / 16, which
+// share their eight angles; neighbouring pairs: chunks 2 l and 2 l + 1), so that the partners
+// need no exchange.  A block takes whole tokens: a lane's cosines and sines serve all its
+// heads and its weights all tokens, and the next rows are requested before the current ones
+// are used.
 // ---------------------------------------------------------------------------------
 constexpr int kRotThreads = 256;
-constexpr int kBatch = 4;
+
+using Pairs = uint64_t[4];  // eight 32-bit values
+
+template <class H>
+__device__ __forceinline__ void unpack_pairs(const uint4& u, Pairs& x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = H::unpack(w[i]);
+        x[i] = pair(f.x, f.y);
+    }
+}
+
+template <class H>
+__device__ __forceinline__ uint4 pack_pairs(const Pairs& x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = halves(x[i]);
+        w[i] = H::pack(f.x, f.y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct TwoChunks {
+    uint4 a, b;
+};
 
 template <class H, int W, bool PAIRS>
-__global__ void __launch_bounds__(kRotThreads, 3) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 2) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
     using T = typename H::type;
-    const int c = threadIdx.x % W;  // this lane's chunk of eight values
-    const int group = threadIdx.x / W;
     constexpr int kGroups = kRotThreads / W;
-    const int half = a.turned / 2, total = a.heads + 2 * a.kv_heads;
-    const bool live = c * 8 < a.dim, turns_here = c * 8 < a.turned;
-    // Angles of the chunk: half-split pairs use angle i % (turned / 2), neighbouring pairs
-    // angle i / 2.
-    const int angle = PAIRS ? c * 4 : (c * 8 < half ? c * 8 : c * 8 - half);
-    const int mate = !turns_here || PAIRS ? c : (c * 8 < half ? c + half / 8 : c - half / 8);
-    const float sign = c * 8 < half ? -1.0f : 1.0f;
-    uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
-    if (live && a.q_weight) wq = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q_weight) + c * 8);
-    if (live && a.k_weight) wk = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_weight) + c * 8);
+    const int l = threadIdx.x % W, group = threadIdx.x / W;
+    const unsigned mask = W == 32 ? 0xffffffffu : ((1u << (W & 31)) - 1u) << (threadIdx.x & 31 & ~(W - 1));
+    const int half = a.turned / 2, turning = a.turned / 16;  // lanes whose chunks rotate
+    const bool turns_here = l < turning;
+    // Values at which the lane's chunks start; the second may lie past the head.
+    const int c0 = !PAIRS && turns_here ? l * 8 : (PAIRS ? l * 16 : a.turned + (l - turning) * 16);
+    const int c1 = !PAIRS && turns_here ? c0 + half : c0 + 8;
+    const bool live0 = c0 < a.dim, live1 = c1 < a.dim;
+    const float inv_dim = 1.0f / a.dim;
 
-    for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x) {
-        const int pos = a.positions[t];
-        int64_t slot = a.slots ? a.slots[t] : -1;
-        const bool known = pos >= 0 && pos < a.n_positions;
-        if (slot >= (a.n_pages << a.page_shift)) slot = -1;
-        const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
-        constexpr int kAngles = PAIRS ? 4 : 8;
-        float cs[kAngles], sn[kAngles];
+    auto load2 = [&](const T* row) {
+        TwoChunks x;
+        x.a = x.b = make_uint4(0, 0, 0, 0);
+        if (live0) x.a = __ldcs(reinterpret_cast<const uint4*>(row + c0));
+        if (live1) x.b = __ldcs(reinterpret_cast<const uint4*>(row + c1));
+        return x;
+    };
+    auto store2 = [&](T* row, const TwoChunks& x) {
+        if (live0) __stcs(reinterpret_cast<uint4*>(row + c0), x.a);
+        if (live1) __stcs(reinterpret_cast<uint4*>(row + c1), x.b);
+    };
+    TwoChunks wq = {}, wk = {};
+    if (a.q_weight) wq = load2(static_cast<const T*>(a.q_weight));
+    if (a.k_weight) wk = load2(static_cast<const T*>(a.k_weight));
+
+    // Round r of a token: one query head, one key head and one value head for each group.
+    // Keys and values start at the groups that the queries leave free.
+    const int hk0 = (group + kGroups - a.heads % kGroups) % kGroups;
+    const int hv0 = (group + kGroups - (a.heads + a.kv_heads) % kGroups) % kGroups;
+    const int rounds = max((a.heads + kGroups - 1) / kGroups, (a.kv_heads + kGroups - 1) / kGroups);
+    TwoChunks q = {}, k = {}, v = {};
+    // Values are read even where the slot says to skip them: the read does not wait for it.
+    auto request = [&](int t, int r) {
+        const int hq = group + r * kGroups, hk = hk0 + r * kGroups, hv = hv0 + r * kGroups;
+        if (hq < a.heads) q = load2(static_cast<const T*>(a.q.p) + t * a.q.tok + hq * a.q.head);
+        if (hk < a.kv_heads) k = load2(static_cast<const T*>(a.k.p) + t * a.k.tok + hk * a.k.head);
+        if (hv < a.kv_heads && a.slots) v = load2(static_cast<const T*>(a.v.p) + t * a.v.tok + hv * a.v.head);
+    };
+    const int step = gridDim.x;
+    int pos = a.positions[blockIdx.x];
+    int64_t slot = a.slots ? a.slots[blockIdx.x] : -1;
+    request(blockIdx.x, 0);
+    for (int t = blockIdx.x; t < a.n_tokens; t += step) {
+        Pairs cs, sn;  // of angles l * 8 .. l * 8 + 7
+        if (turns_here) {
+            const bool known = pos >= 0 && pos < a.n_positions;
+            const float nan = __int_as_float(0x7fc00000);
+            float4 x[2], y[2];
+            x[0] = x[1] = y[0] = y[1] = make_float4(nan, nan, nan, nan);
+            if (known) {
+                const float* row = a.turns + (long long)pos * a.turned + l * 8;
 #pragma unroll
-        for (int i = 0; i < kAngles; i += 4) {
-            float4 x = make_float4(1, 1, 1, 1), y = make_float4(0, 0, 0, 0);
-            if (turns_here) {
-                const float nan = __int_as_float(0x7fc00000);
-                x = y = make_float4(nan, nan, nan, nan);
-                if (known) {
-                    const float* row = a.turns + (long long)pos * a.turned + angle + i;
-                    x = __ldg(reinterpret_cast<const float4*>(row));
-                    y = __ldg(reinterpret_cast<const float4*>(row + half));
+                for (int i = 0; i < 2; ++i) {
+                    x[i] = __ldg(reinterpret_cast<const float4*>(row) + i);
+                    y[i] = __ldg(reinterpret_cast<const float4*>(row + half) + i);
                 }
             }
-            cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
-            sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                cs[2 * i] = pair(x[i].x, x[i].y); cs[2 * i + 1] = pair(x[i].z, x[i].w);
+                sn[2 * i] = pair(y[i].x, y[i].y); sn[2 * i + 1] = pair(y[i].z, y[i].w);
+            }
         }
-        for (int u0 = group; u0 - group < total; u0 += kGroups * kBatch) {  // uniform trip count: shuffles below
-            uint4 raw[kBatch];
+        auto rotated = [&](const TwoChunks& in, const TwoChunks& weight, bool norm) {
+            Pairs x, y;
+            unpack_pairs<H>(in.a, x);
+            unpack_pairs<H>(in.b, y);
+            if (norm) {
+                uint64_t s2 = 0, s3 = 0;
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int u = u0 + b * kGroups;
-                raw[b] = make_uint4(0, 0, 0, 0);
-                if (!live || u >= total) continue;
-                const T* src;
-                if (u < a.heads) src = static_cast<const T*>(a.q.p) + t * a.q.tok + u * a.q.head;
-                else if (u < a.heads + a.kv_heads) src = static_cast<const T*>(a.k.p) + t * a.k.tok + (u - a.heads) * a.k.head;
-                else if (slot < 0) continue;
-                else src = static_cast<const T*>(a.v.p) + t * a.v.tok + (u - a.heads - a.kv_heads) * a.v.head;
-                raw[b] = *reinterpret_cast<const uint4*>(src + c * 8);
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int u = u0 + b * kGroups;
-                if (u0 - group + b * kGroups >= total) break;  // the same for the whole block
-                const bool is_q = u < a.heads, is_k = !is_q && u < a.heads + a.kv_heads;
-                float x[8], w[8];
-                unpack8<H>(raw[b], x);
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-                for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, W);
-                if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
-                    const float inv = rsqrtf(ss / a.dim + a.eps);
-                    unpack8<H>(is_q ? wq : wk, w);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+                for (int i = 0; i < 4; ++i) {
+                    s2 = fma2(x[i], x[i], s2);
+                    s3 = fma2(y[i], y[i], s3);
                 }
-                float y[8];
-                if (PAIRS) {
+                const float2 s = halves(add2(s2, s3));
+                float ss = s.x + s.y;
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        y[i] = turns_here ? x[i] * cs[i / 2] - x[i + 1] * sn[i / 2] : x[i];
-                        y[i + 1] = turns_here ? x[i + 1] * cs[i / 2] + x[i] * sn[i / 2] : x[i + 1];
-                    }
-                } else {
+                for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o, W);
+                const float inv = rsqrtf(fmaf(ss, inv_dim, a.eps));
+                const uint64_t inv2 = pair(inv, inv);
+                Pairs w;
+                unpack_pairs<H>(weight.a, w);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float o = __shfl_sync(0xffffffffu, x[i], mate, W);
-                        y[i] = turns_here ? x[i] * cs[i % kAngles] + sign * o * sn[i % kAngles] : x[i];
+                for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], inv2), w[i]);
+                unpack_pairs<H>(weight.b, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(y[i], inv2), w[i]);
+            }
+            if (turns_here) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (PAIRS) {  // chunk a has angles 0 to 3, chunk b angles 4 to 7
+                        const float2 u = halves(x[i]), w = halves(y[i]);
+                        const float2 c_lo = halves(cs[i / 2]), s_lo = halves(sn[i / 2]);
+                        const float2 c_hi = halves(cs[2 + i / 2]), s_hi = halves(sn[2 + i / 2]);
+                        const float c = i & 1 ? c_lo.y : c_lo.x, s = i & 1 ? s_lo.y : s_lo.x;
+                        const float e = i & 1 ? c_hi.y : c_hi.x, f = i & 1 ? s_hi.y : s_hi.x;
+                        x[i] = pair(u.x * c - u.y * s, u.y * c + u.x * s);
+                        y[i] = pair(w.x * e - w.y * f, w.y * e + w.x * f);
+                    } else {
+                        const uint64_t u = x[i], w = y[i];
+                        y[i] = fma2(u, sn[i], mul2(w, cs[i]));
+                        x[i] = fma2(w, mul2(sn[i], pair(-1.0f, -1.0f)), mul2(u, cs[i]));
                     }
                 }
-                if (!live || u >= total) continue;
-                if (!is_q && !is_k) {  // values are copied as they are
-                    if (slot >= 0)
-                        *reinterpret_cast<uint4*>(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok +
-                                                  (u - a.heads - a.kv_heads) * a.v_cache.head + c * 8) = raw[b];
-                    continue;
-                }
-                const uint4 r = pack8<H>(y);
-                if (is_q) {
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out_q) + ((long long)t * a.heads + u) * a.dim + c * 8) = r;
-                    continue;
-                }
-                const int h = u - a.heads;
-                if (a.out_k)
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out_k) + ((long long)t * a.kv_heads + h) * a.dim + c * 8) = r;
-                if (slot >= 0)
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok +
-                                              h * a.k_cache.head + c * 8) = r;
             }
-            __syncwarp();
+            return TwoChunks{pack_pairs<H>(x), pack_pairs<H>(y)};
+        };
+        int64_t at = slot;
+        if (at >= (a.n_pages << a.page_shift)) at = -1;
+        const int64_t page = at >> a.page_shift, off = at & ((1 << a.page_shift) - 1);
+        const int next = t + step;
+        if (next < a.n_tokens) {
+            pos = a.positions[next];
+            if (a.slots) slot = a.slots[next];
+        }
+        for (int r = 0; r < rounds; ++r) {
+            const TwoChunks q_now = q, k_now = k, v_now = v;
+            if (r + 1 < rounds) request(t, r + 1);
+            else if (next < a.n_tokens) request(next, 0);
+            const int hq = group + r * kGroups, hk = hk0 + r * kGroups, hv = hv0 + r * kGroups;
+            if (hv < a.kv_heads && at >= 0)  // values are copied as they are
+                store2(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok + hv * a.v_cache.head, v_now);
+            if (hq < a.heads)  // the same for a whole group
+                store2(static_cast<T*>(a.out_q) + ((long long)t * a.heads + hq) * a.dim,
+                       rotated(q_now, wq, a.q_weight != nullptr));
+            if (hk < a.kv_heads) {
+                const TwoChunks y = rotated(k_now, wk, a.k_weight != nullptr);
+                if (a.out_k) store2(static_cast<T*>(a.out_k) + ((long long)t * a.kv_heads + hk) * a.dim, y);
+                if (at >= 0)
+                    store2(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok + hk * a.k_cache.head, y);
+            }
         }
     }
 }
 
 template <class H, bool PAIRS>
 void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
-    const int chunks = a.dim / 8;
-    const unsigned grid = (unsigned)std::min(a.n_tokens, 148 * 3 * 8);  // a few tokens a block where there are many
-    if (chunks <= 8) norm_rotate_kernel<H, 8, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
-    else if (chunks <= 16) norm_rotate_kernel<H, 16, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
-    else norm_rotate_kernel<H, 32, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
+    const unsigned grid = (unsigned)std::min(a.n_tokens, 148 * 2 * 8);  // a few tokens a block where there are many
+    if (a.dim <= 64) norm_rotate_kernel<H, 4, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
+    else if (a.dim <= 128) norm_rotate_kernel<H, 8, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
+    else norm_rotate_kernel<H, 16, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
     VGPU_LAUNCH("norm_rotate_kernel");
 }
 
