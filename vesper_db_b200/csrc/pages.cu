@@ -133,11 +133,10 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
 // more loads in flight.  A group of W lanes holds one head; a lane holds two chunks of eight
 // values that rotate into each other (half-split pairs: chunks l and l + turned / 16, which
 // share their eight angles; neighbouring pairs: chunks 2 l and 2 l + 1), so that the partners
-// need no exchange.  A block takes whole tokens: a lane's cosines and sines serve all its
-// heads and its weights all tokens, and the next rows are requested before the current ones
-// are used.
+// need no exchange.  Groups step over the (token, head) rows of the batch, neighbouring
+// groups on neighbouring heads, and request the next row before the current one is used.
 // ---------------------------------------------------------------------------------
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 256, kRotBlocks = 3;  // threads a block, blocks an SM
 
 using Pairs = uint64_t[4];  // eight 32-bit values
 
@@ -167,7 +166,7 @@ struct TwoChunks {
 };
 
 template <class H, int W, bool PAIRS>
-__global__ void __launch_bounds__(kRotThreads, 2) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
+__global__ void __launch_bounds__(kRotThreads, kRotBlocks) norm_rotate_kernel(const __grid_constant__ NormRotateArgs a) {
     using T = typename H::type;
     constexpr int kGroups = kRotThreads / W;
     const int l = threadIdx.x % W, group = threadIdx.x / W;
@@ -191,127 +190,122 @@ __global__ void __launch_bounds__(kRotThreads, 2) norm_rotate_kernel(const __gri
         if (live0) __stcs(reinterpret_cast<uint4*>(row + c0), x.a);
         if (live1) __stcs(reinterpret_cast<uint4*>(row + c1), x.b);
     };
-    TwoChunks wq = {}, wk = {};
-    if (a.q_weight) wq = load2(static_cast<const T*>(a.q_weight));
-    if (a.k_weight) wk = load2(static_cast<const T*>(a.k_weight));
-
-    // Round r of a token: one query head, one key head and one value head for each group.
-    // Keys and values start at the groups that the queries leave free.
-    const int hk0 = (group + kGroups - a.heads % kGroups) % kGroups;
-    const int hv0 = (group + kGroups - (a.heads + a.kv_heads) % kGroups) % kGroups;
-    const int rounds = max((a.heads + kGroups - 1) / kGroups, (a.kv_heads + kGroups - 1) / kGroups);
-    TwoChunks q = {}, k = {}, v = {};
-    // Values are read even where the slot says to skip them: the read does not wait for it.
-    auto request = [&](int t, int r) {
-        const int hq = group + r * kGroups, hk = hk0 + r * kGroups, hv = hv0 + r * kGroups;
-        if (hq < a.heads) q = load2(static_cast<const T*>(a.q.p) + t * a.q.tok + hq * a.q.head);
-        if (hk < a.kv_heads) k = load2(static_cast<const T*>(a.k.p) + t * a.k.tok + hk * a.k.head);
-        if (hv < a.kv_heads && a.slots) v = load2(static_cast<const T*>(a.v.p) + t * a.v.tok + hv * a.v.head);
+    // Rows of a token: query heads, key heads, value heads.
+    const int qk = a.heads + a.kv_heads, units = a.slots ? qk + a.kv_heads : qk;
+    const long long first = (long long)blockIdx.x * kGroups + group, stride = (long long)gridDim.x * kGroups;
+    unsigned t = (unsigned)(first / units);  // may pass 2^31 by a stride
+    int u = (int)(first % units);
+    const int dt = (int)(stride / units), du = (int)(stride % units);
+    TwoChunks next = {};
+    int next_pos = 0;
+    int64_t next_slot = -1;
+    const unsigned n_tokens = (unsigned)a.n_tokens;
+    auto request = [&](unsigned t, int u) {
+        if (t >= n_tokens) return;
+        next_pos = a.positions[t];
+        if (a.slots && u >= a.heads) next_slot = a.slots[t];
+        const HeadsView& x = u < a.heads ? a.q : (u < qk ? a.k : a.v);
+        const int h = u < a.heads ? u : (u < qk ? u - a.heads : u - qk);
+        next = load2(static_cast<const T*>(x.p) + t * x.tok + h * x.head);
     };
-    const int step = gridDim.x;
-    int pos = a.positions[blockIdx.x];
-    int64_t slot = a.slots ? a.slots[blockIdx.x] : -1;
-    request(blockIdx.x, 0);
-    for (int t = blockIdx.x; t < a.n_tokens; t += step) {
-        Pairs cs, sn;  // of angles l * 8 .. l * 8 + 7
-        if (turns_here) {
-            const bool known = pos >= 0 && pos < a.n_positions;
-            const float nan = __int_as_float(0x7fc00000);
-            float4 x[2], y[2];
-            x[0] = x[1] = y[0] = y[1] = make_float4(nan, nan, nan, nan);
-            if (known) {
-                const float* row = a.turns + (long long)pos * a.turned + l * 8;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[i] = __ldg(reinterpret_cast<const float4*>(row) + i);
-                    y[i] = __ldg(reinterpret_cast<const float4*>(row + half) + i);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                cs[2 * i] = pair(x[i].x, x[i].y); cs[2 * i + 1] = pair(x[i].z, x[i].w);
-                sn[2 * i] = pair(y[i].x, y[i].y); sn[2 * i + 1] = pair(y[i].z, y[i].w);
-            }
+    request(t, u);
+    while (t < n_tokens) {
+        const TwoChunks in = next;
+        const unsigned here_t = t;
+        const int pos = next_pos, here_u = u;
+        int64_t at = next_slot;
+        // Cosines and sines of angles l * 8 .. l * 8 + 7
+        float4 cs[2], sn[2];
+        const float nan = __int_as_float(0x7fc00000);
+        cs[0] = cs[1] = sn[0] = sn[1] = make_float4(nan, nan, nan, nan);
+        if (turns_here && here_u < qk && pos >= 0 && pos < a.n_positions) {
+            const float4* row = reinterpret_cast<const float4*>(a.turns + (long long)pos * a.turned + l * 8);
+            cs[0] = __ldg(row);
+            cs[1] = __ldg(row + 1);
+            sn[0] = __ldg(row + half / 4);
+            sn[1] = __ldg(row + half / 4 + 1);
         }
-        auto rotated = [&](const TwoChunks& in, const TwoChunks& weight, bool norm) {
-            Pairs x, y;
-            unpack_pairs<H>(in.a, x);
-            unpack_pairs<H>(in.b, y);
-            if (norm) {
-                uint64_t s2 = 0, s3 = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s2 = fma2(x[i], x[i], s2);
-                    s3 = fma2(y[i], y[i], s3);
-                }
-                const float2 s = halves(add2(s2, s3));
-                float ss = s.x + s.y;
-#pragma unroll
-                for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o, W);
-                const float inv = rsqrtf(fmaf(ss, inv_dim, a.eps));
-                const uint64_t inv2 = pair(inv, inv);
-                Pairs w;
-                unpack_pairs<H>(weight.a, w);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], inv2), w[i]);
-                unpack_pairs<H>(weight.b, w);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(y[i], inv2), w[i]);
-            }
-            if (turns_here) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (PAIRS) {  // chunk a has angles 0 to 3, chunk b angles 4 to 7
-                        const float2 u = halves(x[i]), w = halves(y[i]);
-                        const float2 c_lo = halves(cs[i / 2]), s_lo = halves(sn[i / 2]);
-                        const float2 c_hi = halves(cs[2 + i / 2]), s_hi = halves(sn[2 + i / 2]);
-                        const float c = i & 1 ? c_lo.y : c_lo.x, s = i & 1 ? s_lo.y : s_lo.x;
-                        const float e = i & 1 ? c_hi.y : c_hi.x, f = i & 1 ? s_hi.y : s_hi.x;
-                        x[i] = pair(u.x * c - u.y * s, u.y * c + u.x * s);
-                        y[i] = pair(w.x * e - w.y * f, w.y * e + w.x * f);
-                    } else {
-                        const uint64_t u = x[i], w = y[i];
-                        y[i] = fma2(u, sn[i], mul2(w, cs[i]));
-                        x[i] = fma2(w, mul2(sn[i], pair(-1.0f, -1.0f)), mul2(u, cs[i]));
-                    }
-                }
-            }
-            return TwoChunks{pack_pairs<H>(x), pack_pairs<H>(y)};
-        };
-        int64_t at = slot;
+        t += dt;
+        u += du;
+        if (u >= units) {
+            u -= units;
+            ++t;
+        }
+        request(t, u);
         if (at >= (a.n_pages << a.page_shift)) at = -1;
         const int64_t page = at >> a.page_shift, off = at & ((1 << a.page_shift) - 1);
-        const int next = t + step;
-        if (next < a.n_tokens) {
-            pos = a.positions[next];
-            if (a.slots) slot = a.slots[next];
+        if (here_u >= qk) {  // values are copied as they are
+            if (at >= 0)
+                store2(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok + (here_u - qk) * a.v_cache.head, in);
+            continue;
         }
-        for (int r = 0; r < rounds; ++r) {
-            const TwoChunks q_now = q, k_now = k, v_now = v;
-            if (r + 1 < rounds) request(t, r + 1);
-            else if (next < a.n_tokens) request(next, 0);
-            const int hq = group + r * kGroups, hk = hk0 + r * kGroups, hv = hv0 + r * kGroups;
-            if (hv < a.kv_heads && at >= 0)  // values are copied as they are
-                store2(static_cast<T*>(a.v_cache.p) + page * a.v_cache.page + off * a.v_cache.tok + hv * a.v_cache.head, v_now);
-            if (hq < a.heads)  // the same for a whole group
-                store2(static_cast<T*>(a.out_q) + ((long long)t * a.heads + hq) * a.dim,
-                       rotated(q_now, wq, a.q_weight != nullptr));
-            if (hk < a.kv_heads) {
-                const TwoChunks y = rotated(k_now, wk, a.k_weight != nullptr);
-                if (a.out_k) store2(static_cast<T*>(a.out_k) + ((long long)t * a.kv_heads + hk) * a.dim, y);
-                if (at >= 0)
-                    store2(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok + hk * a.k_cache.head, y);
+        const bool is_q = here_u < a.heads;
+        const T* weight = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
+        Pairs x, y;
+        unpack_pairs<H>(in.a, x);
+        unpack_pairs<H>(in.b, y);
+        if (weight) {
+            uint64_t s2 = 0, s3 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s2 = fma2(x[i], x[i], s2);
+                s3 = fma2(y[i], y[i], s3);
+            }
+            const float2 s = halves(add2(s2, s3));
+            float ss = s.x + s.y;
+#pragma unroll
+            for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o, W);
+            const float inv = rsqrtf(fmaf(ss, inv_dim, a.eps));
+            const uint64_t inv2 = pair(inv, inv);
+            uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
+            if (live0) wa = __ldg(reinterpret_cast<const uint4*>(weight + c0));
+            if (live1) wb = __ldg(reinterpret_cast<const uint4*>(weight + c1));
+            Pairs w;
+            unpack_pairs<H>(wa, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], inv2), w[i]);
+            unpack_pairs<H>(wb, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(y[i], inv2), w[i]);
+        }
+        if (turns_here) {
+            const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+            const float s[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (PAIRS) {  // chunk a has angles 0 to 3, chunk b angles 4 to 7
+                    const float2 f = halves(x[i]), g = halves(y[i]);
+                    x[i] = pair(f.x * c[i] - f.y * s[i], f.y * c[i] + f.x * s[i]);
+                    y[i] = pair(g.x * c[4 + i] - g.y * s[4 + i], g.y * c[4 + i] + g.x * s[4 + i]);
+                } else {
+                    const uint64_t f = x[i], g = y[i], c2 = pair(c[2 * i], c[2 * i + 1]), s2 = pair(s[2 * i], s[2 * i + 1]);
+                    y[i] = fma2(f, s2, mul2(g, c2));
+                    x[i] = fma2(g, pair(-s[2 * i], -s[2 * i + 1]), mul2(f, c2));
+                }
             }
         }
+        const TwoChunks out{pack_pairs<H>(x), pack_pairs<H>(y)};
+        if (is_q) {
+            store2(static_cast<T*>(a.out_q) + ((long long)here_t * a.heads + here_u) * a.dim, out);
+            continue;
+        }
+        const int h = here_u - a.heads;
+        if (a.out_k) store2(static_cast<T*>(a.out_k) + ((long long)here_t * a.kv_heads + h) * a.dim, out);
+        if (at >= 0)
+            store2(static_cast<T*>(a.k_cache.p) + page * a.k_cache.page + off * a.k_cache.tok + h * a.k_cache.head, out);
     }
 }
 
 template <class H, bool PAIRS>
 void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
-    const unsigned grid = (unsigned)std::min(a.n_tokens, 148 * 2 * 8);  // a few tokens a block where there are many
-    if (a.dim <= 64) norm_rotate_kernel<H, 4, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
-    else if (a.dim <= 128) norm_rotate_kernel<H, 8, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
-    else norm_rotate_kernel<H, 16, PAIRS><<<grid, kRotThreads, 0, st>>>(a);
+    const long long rows = (long long)a.n_tokens * (a.heads + (a.slots ? 2 : 1) * a.kv_heads);
+    auto launch = [&](auto* kernel, int width) {
+        const long long blocks = (rows * width + kRotThreads - 1) / kRotThreads;
+        kernel<<<(unsigned)std::min<long long>(blocks, 148 * kRotBlocks * 4), kRotThreads, 0, st>>>(a);
+    };
+    if (a.dim <= 64) launch(norm_rotate_kernel<H, 4, PAIRS>, 4);
+    else if (a.dim <= 128) launch(norm_rotate_kernel<H, 8, PAIRS>, 8);
+    else launch(norm_rotate_kernel<H, 16, PAIRS>, 16);
     VGPU_LAUNCH("norm_rotate_kernel");
 }
 
