@@ -17,6 +17,9 @@ using attn::kThreads;
 using attn::TileParams;
 
 constexpr int kSms = 148;
+// Prefix rows in tiles of 8 or 16: up to this many of them, re-reading the prefix for each
+// from L2 is quicker than a tensor-core tile.
+constexpr int kFewRowTiles = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------------------------
@@ -102,79 +105,106 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 }
 
 // ---------------------------------------------------------------------------------
-// Own pages of each request: bound by reading keys and values once.  A block takes one
-// request, one key head, up to 16 of its query heads and a range of keys; each of its
-// warps takes 16 keys at a time, with its own running maximum and sum, and the four are
-// joined at the end.  The products are m16n8k16 steps of one warp: 16 query heads by 8
-// keys, then by 8 values.  Operands go from global memory to registers in 16-byte loads,
-// without a stop in shared memory:
+// Pages of a cache with few query rows: each request's own pages, and the prefix when the
+// whole batch has few rows.  Bound by reading keys and values once.  A block takes one key
+// head, up to 8 * NT query rows and a range of keys; each of its warps takes 16 keys at a
+// time, with its own running maximum and sum, and the four are joined at the end.  The
+// products are m16n8k16 steps of one warp, S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T
+// (16 values by 8 rows): with the rows on the short side few of them waste little.  Operands
+// go from global memory to registers in 16-byte loads, without a stop in shared memory:
 //   * keys: the order of the contraction index is free, so lane (g, t) = (lane / 4,
-//     lane % 4) holds chunks t, t + 4, ... (eight values each) of key g, and the queries are
-//     laid out the same way;
-//   * values: the order of the output columns is free, so lane (g, t) holds chunks g and
-//     g + 8 of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and column n of step (i, e) is value
-//     (8 i + n) 8 + e: one byte permutation makes each operand register.
+//     lane % 4) holds chunks t, t + 4, ... (eight values each) of keys g and g + 8, and the
+//     queries are laid out the same way;
+//   * values: the order of the output rows is free, so lane (g, t) holds chunks g and g + 8
+//     of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and rows g and g + 8 of step (i, e) are values e
+//     and e + 4 of chunk 8 i + g: one byte permutation makes each operand register;
+//   * probabilities: one 8 x 8 transposition between registers turns S^T into P^T.
 // The next keys are loaded while the scores become probabilities, the next values while
 // the next scores are made.
 // ---------------------------------------------------------------------------------
 constexpr int kOwnWarps = 4;
 
 template <class H>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
     if (std::is_same<H, Bf16>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
-template <class H, int D>
-__global__ void __launch_bounds__(kOwnWarps * 32) own_pages_kernel(const __grid_constant__ SharedArgs a, int splits, int chunk,
-                                                                   float* __restrict__ part_o, float* __restrict__ part_lse) {
-    using T = typename H::type;
-    constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key row, of a value row
-    constexpr int kPad = D + 4;
-    __shared__ float s_o[kOwnWarps][16][kPad];
-    __shared__ float s_m[kOwnWarps][16], s_l[kOwnWarps][16];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int group = a.heads / a.kv_heads, mt = (group + 15) / 16;
-    int x = blockIdx.x;  // key heads fastest: blocks that run together read neighbouring memory
-    const int kh = x % a.kv_heads;
-    x /= a.kv_heads;
-    const int m0 = (x % mt) * 16;
-    x /= mt;
-    const int split = x % splits, b = x / splits;
-    const int rows_here = min(16, group - m0);
-    const long long rows = (long long)a.n_requests * a.heads;
-    const long long row0 = (long long)b * a.heads + kh * group + m0;
+// Blocks below `prefix_blocks` take the prefix, the others the requests' own pages; a range
+// is `chunk` keys.  Results of range i go to part i of the prefix's or of the own parts.
+struct PagesPlan {
+    int prefix_blocks, prefix_splits, prefix_chunk;
+    int own_splits, own_chunk;
+    float* prefix_o;
+    float* prefix_lse;
+    float* own_o;
+    float* own_lse;
+};
 
-    const int n = min(max(a.lengths[b], 0), a.table_width << a.page_shift);
-    const int begin = min((long long)split * chunk, (long long)n), end = min(n, begin + chunk);
+template <class H, int D, int NT>
+__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 2)
+    pages_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ PagesPlan pl) {
+    using T = typename H::type;
+    constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key, of a value row
+    constexpr int kRowsHere = 8 * NT;
+    __shared__ float s_o[kOwnWarps][kRowsHere][D + 4];
+    __shared__ float s_m[kOwnWarps][kRowsHere], s_l[kOwnWarps][kRowsHere];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads;
+    const bool prefix = (int)blockIdx.x < pl.prefix_blocks;
+    int x = prefix ? blockIdx.x : blockIdx.x - pl.prefix_blocks;
+    const int kh = x % a.kv_heads;  // key heads fastest: blocks that run together read neighbouring memory
+    x /= a.kv_heads;
+    // Rows of this block: row r is query head kh * group + (m0 + r) % group of request
+    // b + (m0 + r) / group.
+    int b, split, m0, n_rows, n, chunk;
+    const int32_t* pages;
+    if (prefix) {
+        split = x % pl.prefix_splits;
+        m0 = x / pl.prefix_splits * kRowsHere;
+        b = 0;
+        n_rows = min(kRowsHere, a.n_requests * group - m0);
+        n = (int)a.prefix_len;
+        chunk = pl.prefix_chunk;
+        pages = a.prefix_pages;
+    } else {
+        const int mt = (group + kRowsHere - 1) / kRowsHere;
+        m0 = x % mt * kRowsHere;
+        x /= mt;
+        split = x % pl.own_splits;
+        b = x / pl.own_splits;
+        n_rows = min(kRowsHere, group - m0);
+        n = min(max(a.lengths[b], 0), a.table_width << a.page_shift);
+        chunk = pl.own_chunk;
+        pages = a.table + (long long)b * a.table_stride;
+    }
+    const long long rows = (long long)a.n_requests * a.heads;
+    auto row_of = [&](int r) { return (long long)(b + (m0 + r) / group) * a.heads + kh * group + (m0 + r) % group; };
+    float* const out_o = (prefix ? pl.prefix_o : pl.own_o) + split * rows * a.dim;
+    float* const out_lse = (prefix ? pl.prefix_lse : pl.own_lse) + split * rows;
+
+    const int begin = (int)min((long long)split * chunk, (long long)n), end = min(n, begin + chunk);
     if (begin >= end) {
-        if (tid < rows_here) part_lse[split * rows + row0 + tid] = -INFINITY;
+        if (tid < n_rows) out_lse[row_of(tid)] = -INFINITY;
         return;
     }
     const int blocks = (end - begin + 15) / 16;
-    const int32_t* pages = a.table + (long long)b * a.table_stride;
     const int mask = (1 << a.page_shift) - 1;
-
-    // Queries, laid out as the keys are.
-    uint32_t qa[2 * KC][4];
-#pragma unroll
-    for (int i = 0; i < KC; ++i) {
-        const int c = (i * 4 + t) * 8;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        const T* q = static_cast<const T*>(a.q.p) + b * a.q.tok + (kh * group + m0) * a.q.head;
-        if (c < a.dim && g < rows_here) lo = *reinterpret_cast<const uint4*>(q + g * a.q.head + c);
-        if (c < a.dim && g + 8 < rows_here) hi = *reinterpret_cast<const uint4*>(q + (g + 8) * a.q.head + c);
-        qa[2 * i][0] = lo.x; qa[2 * i][1] = hi.x; qa[2 * i][2] = lo.y; qa[2 * i][3] = hi.y;
-        qa[2 * i + 1][0] = lo.z; qa[2 * i + 1][1] = hi.z; qa[2 * i + 1][2] = lo.w; qa[2 * i + 1][3] = hi.w;
-    }
 
     uint4 kf[2][KC], vf[4][VC];
     // 16 keys lie in one page.  Rows past the end are not read: they may hold anything.
@@ -207,77 +237,100 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_pages_kernel(const __grid_
     };
     auto page_of = [&](int ib) { return ib < blocks ? pages[(begin + ib * 16) >> a.page_shift] : -1; };
 
-    float o[VC][8][4];
-#pragma unroll
-    for (int i = 0; i < VC; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[i][e][c] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const float scale = a.scale * kLog2e;
     int ib = warp, pg = page_of(ib), pg_next = page_of(ib + kOwnWarps);
     load_k(ib, pg);
     load_v(ib, pg);
+    // Queries, laid out as the keys are.
+    uint32_t qb[NT][2 * KC][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        const T* q = static_cast<const T*>(a.q.p);
+        if (r < n_rows) q += (long long)(b + (m0 + r) / group) * a.q.tok + (kh * group + (m0 + r) % group) * a.q.head;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            const int c = (i * 4 + t) * 8;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (c < a.dim && r < n_rows) u = *reinterpret_cast<const uint4*>(q + c);
+            qb[nt][2 * i][0] = u.x; qb[nt][2 * i][1] = u.y;
+            qb[nt][2 * i + 1][0] = u.z; qb[nt][2 * i + 1][1] = u.w;
+        }
+    }
+
+    float o[NT][VC][4][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[nt][i][e][c] = 0.0f;
+    float m[NT][2], l[NT][2];  // of rows 2t and 2t + 1; l over this lane's keys only
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+    const float scale = a.scale * kLog2e;
     for (; ib < blocks; ib += kOwnWarps) {
-        float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        float s[NT][4];
 #pragma unroll
-        for (int i = 0; i < KC; ++i)
+        for (int nt = 0; nt < NT; ++nt) {
+            s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                mma16816<H>(s[r], qa[2 * i], kf[r][i].x, kf[r][i].y);
-                mma16816<H>(s[r], qa[2 * i + 1], kf[r][i].z, kf[r][i].w);
+            for (int i = 0; i < KC; ++i) {
+                mma16816<H>(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qb[nt][2 * i][0], qb[nt][2 * i][1]);
+                mma16816<H>(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
             }
+        }
         const int pg_after = page_of(ib + 2 * kOwnWarps);
         load_k(ib + kOwnWarps, pg_next);
-        const int key = begin + ib * 16;
-        float top[2] = {-INFINITY, -INFINITY};
+        const int key = begin + ib * 16 + g;
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int nt = 0; nt < NT; ++nt) {
+            float top[2];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[r][c] = key + r * 8 + 2 * t + (c & 1) < end ? s[r][c] * scale : -INFINITY;
-                top[c >> 1] = fmaxf(top[c >> 1], s[r][c]);
+            for (int c = 0; c < 4; ++c) s[nt][c] = key + (c >> 1) * 8 < end ? s[nt][c] * scale : -INFINITY;
+            top[0] = fmaxf(s[nt][0], s[nt][2]);
+            top[1] = fmaxf(s[nt][1], s[nt][3]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 4; e < 32; e *= 2) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], e));
+            if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float up = fmaxf(m[nt][h], top[h]), f = up == -INFINITY ? 1.0f : attn::ex2(m[nt][h] - up);
+                    m[nt][h] = up;
+                    l[nt][h] *= f;
+#pragma unroll
+                    for (int i = 0; i < VC; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[nt][i][e][h] *= f;
+                            o[nt][i][e][2 + h] *= f;
+                        }
+                }
             }
+            const float ref0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], ref1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float up = fmaxf(m[h], top[h]), f = up == -INFINITY ? 1.0f : attn::ex2(m[h] - up);
-                m[h] = up;
-                l[h] *= f;
-#pragma unroll
-                for (int i = 0; i < VC; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        o[i][e][2 * h] *= f;
-                        o[i][e][2 * h + 1] *= f;
-                    }
+            for (int h = 0; h < 2; ++h) {  // keys g and g + 8
+                const float p0 = attn::ex2(s[nt][2 * h] - ref0), p1 = attn::ex2(s[nt][2 * h + 1] - ref1);
+                l[nt][0] += p0;
+                l[nt][1] += p1;
+                pb[nt][h] = transposed8x8(H::pack(p0, p1));
             }
-        }
-        const float ref0 = m[0] == -INFINITY ? 0.0f : m[0], ref1 = m[1] == -INFINITY ? 0.0f : m[1];
-        uint32_t pa[4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float p0 = attn::ex2(s[r][0] - ref0), p1 = attn::ex2(s[r][1] - ref0);
-            const float p2 = attn::ex2(s[r][2] - ref1), p3 = attn::ex2(s[r][3] - ref1);
-            l[0] += p0 + p1;
-            l[1] += p2 + p3;
-            pa[2 * r] = H::pack(p0, p1);
-            pa[2 * r + 1] = H::pack(p2, p3);
         }
 #pragma unroll
         for (int i = 0; i < VC; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-                const uint32_t b0 = __byte_perm(word(vf[0][i], e / 2), word(vf[1][i], e / 2), sel);
-                const uint32_t b1 = __byte_perm(word(vf[2][i], e / 2), word(vf[3][i], e / 2), sel);
-                mma16816<H>(o[i][e], pa, b0, b1);
+                const uint32_t a0 = __byte_perm(word(vf[0][i], e / 2), word(vf[1][i], e / 2), sel);
+                const uint32_t a1 = __byte_perm(word(vf[0][i], e / 2 + 2), word(vf[1][i], e / 2 + 2), sel);
+                const uint32_t a2 = __byte_perm(word(vf[2][i], e / 2), word(vf[3][i], e / 2), sel);
+                const uint32_t a3 = __byte_perm(word(vf[2][i], e / 2 + 2), word(vf[3][i], e / 2 + 2), sel);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<H>(o[nt][i][e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
         load_v(ib + kOwnWarps, pg_next);
         pg_next = pg_after;
@@ -285,75 +338,71 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_pages_kernel(const __grid_
 
     // Join of the four warps.
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int r = g + 8 * h;
-        if (t == 0) {
-            s_m[warp][r] = m[h];
-            s_l[warp][r] = l[h];
-        }
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < VC; ++i)
+        for (int h = 0; h < 2; ++h) {
+            const int r = nt * 8 + 2 * t + h;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float4* dst = reinterpret_cast<float4*>(&s_o[warp][r][(i * 8 + 2 * t + c) * 8]);
-                dst[0] = make_float4(o[i][0][2 * h + c], o[i][1][2 * h + c], o[i][2][2 * h + c], o[i][3][2 * h + c]);
-                dst[1] = make_float4(o[i][4][2 * h + c], o[i][5][2 * h + c], o[i][6][2 * h + c], o[i][7][2 * h + c]);
+            for (int e = 4; e < 32; e *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], e);
+            if (g == 0) {
+                s_m[warp][r] = m[nt][h];
+                s_l[warp][r] = l[nt][h];
             }
-    }
+#pragma unroll
+            for (int i = 0; i < VC; ++i) {
+                float4* dst = reinterpret_cast<float4*>(&s_o[warp][r][(i * 8 + g) * 8]);
+                dst[0] = make_float4(o[nt][i][0][h], o[nt][i][1][h], o[nt][i][2][h], o[nt][i][3][h]);
+                dst[1] = make_float4(o[nt][i][0][2 + h], o[nt][i][1][2 + h], o[nt][i][2][2 + h], o[nt][i][3][2 + h]);
+            }
+        }
     __syncthreads();
-    const int r = tid >> 3;
-    if (r >= rows_here) return;
+    constexpr int kPerRow = kOwnWarps * 32 / kRowsHere;
+    const int r = tid / kPerRow;
+    if (r >= n_rows) return;
     float top = -INFINITY, total = 0.0f, w[kOwnWarps];
 #pragma unroll
     for (int i = 0; i < kOwnWarps; ++i) top = fmaxf(top, s_m[i][r]);
 #pragma unroll
     for (int i = 0; i < kOwnWarps; ++i) {
+        // a warp without keys has m = -inf, and zeros
         w[i] = s_m[i][r] == -INFINITY ? 0.0f : attn::ex2(s_m[i][r] - top);
-        if (i >= blocks) w[i] = 0.0f;  // a warp without keys
-        total += s_l[i][r] * w[i];
+        total += s_l[i][r] * (i < blocks && s_m[i][r] == -INFINITY ? 1.0f : w[i]);
     }
     const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
-    for (int d = (tid & 7) * 4; d < a.dim; d += 32) {
+    const long long row = row_of(r);
+    for (int d = tid % kPerRow * 4; d < a.dim; d += kPerRow * 4) {
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < kOwnWarps; ++i) {
             const float4 v = *reinterpret_cast<const float4*>(&s_o[i][r][d]);
             acc = make_float4(acc.x + w[i] * v.x, acc.y + w[i] * v.y, acc.z + w[i] * v.z, acc.w + w[i] * v.w);
         }
-        *reinterpret_cast<float4*>(part_o + (split * rows + row0 + r) * a.dim + d) =
-            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        *reinterpret_cast<float4*>(out_o + row * a.dim + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
-    if ((tid & 7) == 0) part_lse[split * rows + row0 + r] = top + log2f(total);
+    if (tid % kPerRow == 0) out_lse[row] = top + log2f(total);
 }
 
-struct OwnPlan {
-    int splits, chunk;  // ranges of `chunk` keys
-};
-// The lengths are on the device: ranges are cut for what the table can hold.  Six blocks an
-// SM fill the GPU; no range is below 128 keys, none above 1,024, so that the longest request
-// does not run on alone.  A range past a request's length costs one write a row.
-OwnPlan own_plan(const SharedArgs& a) {
-    const long long cap = (long long)a.table_width << a.page_shift;
-    const long long base = (long long)a.n_requests * a.kv_heads * ((a.heads / a.kv_heads + 15) / 16);
-    long long s = std::max<long long>(ceil_div(6 * kSms, base), ceil_div(cap, 1024));
-    s = std::max<long long>(1, std::min<long long>({s, (cap + 127) / 128, 256}));
-    OwnPlan p;
-    p.chunk = (int)((ceil_div(cap, s) + 63) / 64 * 64);
-    p.splits = p.chunk ? (int)((cap + p.chunk - 1) / p.chunk) : 0;
-    return p;
+// The lengths are on the device: ranges are cut for what the table can hold.  A range past a
+// request's length costs one write a row.
+int keys_a_range(long long cap, long long blocks_a_range) {
+    // four blocks an SM fill the GPU; 128 keys at least a range, 512 at most, so that the
+    // longest request does not run on alone
+    long long s = std::max<long long>(ceil_div(4 * kSms, std::max<long long>(blocks_a_range, 1)), ceil_div(cap, 512));
+    s = std::max<long long>(1, std::min<long long>(s, (cap + 127) / 128));
+    return (int)((ceil_div(cap, s) + 63) / 64 * 64);
 }
 
 template <class H>
-void launch_own(const SharedArgs& a, const OwnPlan& pl, float* part_o, float* part_lse, cudaStream_t st) {
-    const long long blocks = (long long)a.n_requests * a.kv_heads * ((a.heads / a.kv_heads + 15) / 16) * pl.splits;
+void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, cudaStream_t st) {
+    const int group = a.heads / a.kv_heads;
+    const long long blocks =
+        pl.prefix_blocks + (long long)a.n_requests * a.kv_heads * ((group + 8 * nt - 1) / (8 * nt)) * pl.own_splits;
     if (blocks > 0x7fffffffLL) throw CudaError("attention: too many requests for one launch");
-    if (a.dim <= 64)
-        own_pages_kernel<H, 64><<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl.splits, pl.chunk, part_o, part_lse);
-    else
-        own_pages_kernel<H, 128><<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl.splits, pl.chunk, part_o, part_lse);
-    VGPU_LAUNCH("own_pages_kernel");
+    if (blocks == 0) return;
+    auto launch = [&](auto* kernel) { kernel<<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl); };
+    if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
+    else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
+    VGPU_LAUNCH("pages_kernel");
 }
 
 // ---------------------------------------------------------------------------------
@@ -366,27 +415,42 @@ __global__ void __launch_bounds__(128) join_kernel(int parts, long long rows, in
     const int lane = threadIdx.x & 31;
     const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
     if (row >= rows) return;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int i = 0; i < parts; ++i) {
-        const float x = part_lse[i * rows + row];
-        nan |= isnan(x);
-        m = fmaxf(m, x);
-    }
-    float total = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
     const bool live = lane * 4 < dim;
-    for (int i = 0; i < parts; ++i) {
-        const float x = part_lse[i * rows + row];
-        if (x == -INFINITY) continue;
-        const float w = exp2f(x - m);
-        total += w;
-        if (live) {
-            const float4 v = *reinterpret_cast<const float4*>(part_o + (i * rows + row) * dim + lane * 4);
-            o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+    float m = -INFINITY, total = 0.0f;
+    bool nan = false;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int p0 = 0; p0 < parts; p0 += 32) {  // the weights of 32 parts, one a lane
+        const float x = p0 + lane < parts ? part_lse[(p0 + lane) * rows + row] : -INFINITY;
+        float up = m;
+        nan |= __any_sync(0xffffffffu, isnan(x)) != 0;
+        up = fmaxf(up, x);
+#pragma unroll
+        for (int e = 16; e > 0; e >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, e));
+        const float ref = up == -INFINITY ? 0.0f : up, f = exp2f(m - ref), w = exp2f(x - ref);
+        m = up;
+        total = total * f + w;  // this lane's share
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        unsigned some = __ballot_sync(0xffffffffu, w > 0.0f);  // parts without keys hold no rows
+        while (some) {
+            float4 v[4];
+            float wi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = some ? __ffs(some) - 1 : -1;
+                wi[e] = __shfl_sync(0xffffffffu, w, i < 0 ? 0 : i);
+                v[e] = make_float4(0, 0, 0, 0);
+                if (i < 0) wi[e] = 0.0f;
+                else if (live) v[e] = *reinterpret_cast<const float4*>(part_o + ((p0 + i) * rows + row) * dim + lane * 4);
+                some &= some - 1;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o = make_float4(o.x + wi[e] * v[e].x, o.y + wi[e] * v[e].y, o.z + wi[e] * v[e].z, o.w + wi[e] * v[e].w);
         }
     }
-    const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f && !nan ? 0.0f : __int_as_float(0x7fc00000));
+#pragma unroll
+    for (int e = 16; e > 0; e >>= 1) total += __shfl_xor_sync(0xffffffffu, total, e);
+    const float inv = nan ? __int_as_float(0x7fc00000) : (total > 0.0f ? 1.0f / total : 0.0f);
     if (live)
         *reinterpret_cast<uint2*>(static_cast<typename H::type*>(out) + row * dim + lane * 4) =
             make_uint2(H::pack(o.x * inv, o.y * inv), H::pack(o.z * inv, o.w * inv));
@@ -423,9 +487,31 @@ PromptPlan prompt_plan(const PromptArgs& a) {
     return pl;
 }
 
-int shared_splits(const SharedArgs& a) {
-    const int span = 2 * (kRows / (a.heads / a.kv_heads));
-    return splits_for((long long)ceil_div(a.n_requests, span) * a.kv_heads, a.prefix_len / kKeys);
+// Parts of the prefix, then of the own pages.
+struct SharedPlan {
+    bool tiles;  // the prefix goes to the tensor cores' tiles
+    int prefix_splits, prefix_chunk, own_splits, own_chunk, nt;
+};
+SharedPlan shared_plan(const SharedArgs& a) {
+    SharedPlan p{};
+    const int group = a.heads / a.kv_heads;
+    const long long rows = (long long)a.n_requests * group;  // of one key head
+    p.nt = group > 8 ? 2 : 1;
+    const long long cap = (long long)a.table_width << a.page_shift;
+    const long long own_blocks = (long long)a.n_requests * a.kv_heads * ((group + 8 * p.nt - 1) / (8 * p.nt));
+    p.own_chunk = cap ? keys_a_range(cap, own_blocks) : 0;
+    p.own_splits = cap ? (int)((cap + p.own_chunk - 1) / p.own_chunk) : 0;
+    if (a.prefix_len == 0) return p;
+    const long long row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
+    p.tiles = row_tiles > kFewRowTiles;
+    if (p.tiles) {
+        const int span = 2 * (kRows / group);
+        p.prefix_splits = splits_for((long long)ceil_div(a.n_requests, span) * a.kv_heads, a.prefix_len / kKeys);
+    } else {
+        p.prefix_chunk = keys_a_range(a.prefix_len, row_tiles * a.kv_heads);
+        p.prefix_splits = (int)((a.prefix_len + p.prefix_chunk - 1) / p.prefix_chunk);
+    }
+    return p;
 }
 
 }  // namespace
@@ -465,16 +551,22 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
 
 size_t shared_attention_workspace(const SharedArgs& a) {
     if (a.n_requests == 0) return 0;
-    return part_bytes(own_plan(a).splits + (a.prefix_len ? shared_splits(a) : 0), (long long)a.n_requests * a.heads, a.dim);
+    const SharedPlan sp = shared_plan(a);
+    return part_bytes(sp.prefix_splits + sp.own_splits, (long long)a.n_requests * a.heads, a.dim);
 }
 
 void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
     const long long rows = (long long)a.n_requests * a.heads;
-    const int splits = a.prefix_len ? shared_splits(a) : 0;
-    const OwnPlan own = own_plan(a);
+    const SharedPlan sp = shared_plan(a);
+    const int parts = sp.prefix_splits + sp.own_splits;
     float* part_o = static_cast<float*>(a.workspace);
-    float* part_lse = part_o + (splits + own.splits) * rows * a.dim;
-    if (splits) {
+    float* part_lse = part_o + parts * rows * a.dim;
+    PagesPlan pl{};
+    pl.own_splits = sp.own_splits;
+    pl.own_chunk = sp.own_chunk;
+    pl.own_o = part_o + sp.prefix_splits * rows * a.dim;
+    pl.own_lse = part_lse + sp.prefix_splits * rows;
+    if (sp.tiles) {
         TileParams p{};
         fill_queries(p, a.f16, a.q, a.heads, a.kv_heads, a.dim, a.n_requests);
         const int page = 1 << a.page_shift, box = std::min(page, kKeys);
@@ -485,19 +577,22 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
         p.pages = a.prefix_pages;
         p.page_shift = a.page_shift;
         p.scale_log2 = a.scale * kLog2e;
-        p.splits = splits;
+        p.splits = sp.prefix_splits;
         p.part = true;
         p.part_o = part_o;
         p.part_lse = part_lse;
-        launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * splits, st);
+        launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * p.splits, st);
+    } else if (sp.prefix_splits) {
+        const long long row_tiles = ((long long)a.n_requests * (a.heads / a.kv_heads) + 8 * sp.nt - 1) / (8 * sp.nt);
+        pl.prefix_blocks = (int)(row_tiles * a.kv_heads * sp.prefix_splits);
+        pl.prefix_splits = sp.prefix_splits;
+        pl.prefix_chunk = sp.prefix_chunk;
+        pl.prefix_o = part_o;
+        pl.prefix_lse = part_lse;
     }
-    if (own.splits) {
-        float* own_o = part_o + splits * rows * a.dim;
-        float* own_lse = part_lse + splits * rows;
-        if (a.f16) launch_own<F16>(a, own, own_o, own_lse, st);
-        else launch_own<Bf16>(a, own, own_o, own_lse, st);
-    }
-    launch_join(a.f16, splits + own.splits, rows, a.dim, part_o, part_lse, a.out, a.lse, st);
+    if (a.f16) launch_pages<F16>(a, pl, sp.nt, st);
+    else launch_pages<Bf16>(a, pl, sp.nt, st);
+    launch_join(a.f16, parts, rows, a.dim, part_o, part_lse, a.out, a.lse, st);
 }
 
 }  // namespace vgpu
