@@ -536,6 +536,7 @@ VESPER_C_API vesper_status_t vesper_prompt_attention_device(const vesper_prompt_
  * prefix_len slots of d_prefix_pages [ceil(prefix_len / page_size)], the same for every
  * request and read once for all of them, then the first d_lengths[b] slots of
  * d_table[b, 0 .. table_width).  Softmax and outputs as above, joined over both parts.
+ * n_requests * ceil(heads / kv_heads / 8) * table_width * page_size is at most 2^34.
  * Lengths are bounded to [0, table_width * page_size]; a page number outside
  * [0, n_pages) reads as zero keys and values.  Slots past the lengths are not used,
  * whatever is in them. */

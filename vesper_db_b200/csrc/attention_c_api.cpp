@@ -116,6 +116,8 @@ vgpu::SharedArgs shared_args(const vesper_shared_prefix_attention_params_t& p) {
     a.page_shift = page_shift_of(p.page_size);
     need(p.n_pages <= kMaxInt, "at most 2^31 - 1 pages");
     need(p.table_width <= (kMaxInt >> a.page_shift), "table_width * page_size must be below 2^31");
+    need((p.n_requests * ((p.heads / p.kv_heads + 7) / 8) * p.table_width) <= (((size_t)1 << 34) >> a.page_shift),
+         "n_requests * table_width * page_size must be at most 2^34 for eight query heads a key head");
     a.n_pages = (long long)p.n_pages;
     a.prefix_len = (long long)p.prefix_len;
     a.table_width = (int)p.table_width;

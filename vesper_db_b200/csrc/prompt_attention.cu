@@ -106,12 +106,21 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 
 // ---------------------------------------------------------------------------------
 // Pages of a cache with few query rows: each request's own pages, and the prefix when the
-// whole batch has few rows.  Bound by reading keys and values once.  A block takes one key
-// head, up to 8 * NT query rows and a range of keys; each of its warps takes 16 keys at a
-// time, with its own running maximum and sum, and the four are joined at the end.  The
-// products are m16n8k16 steps of one warp, S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T
-// (16 values by 8 rows): with the rows on the short side few of them waste little.  Operands
-// go from global memory to registers in 16-byte loads, without a stop in shared memory:
+// whole batch has few rows.  Bound by reading keys and values once.
+//
+// A job is up to 8 * NT query rows of one key head with the keys they share: a request's
+// own pages (jobs 0 ..), then the prefix for each tile of the batch's rows.  Requests differ
+// widely in length, so the work is cut by keys, not by requests: the jobs' blocks of 16 keys
+// are laid end to end, and each warp takes the next `range` of them, across jobs.  What it
+// has of a job when the job or the range ends goes to slot job + warp (which grows from one
+// such segment to the next, so it is unique); the join adds up a job's slots.  (A grid of
+// requests by fixed ranges took 67 us for 256 requests of 1 to 1,500 tokens, 175 MB: most
+// of its blocks were empty or short.)
+//
+// The products are m16n8k16 steps of one warp, S^T = K Q^T (16 keys by 8 rows) and
+// O^T = V^T P^T (16 values by 8 rows): with the rows on the short side few of them waste
+// little.  Operands go from global memory to registers in 16-byte loads, without a stop in
+// shared memory:
 //   * keys: the order of the contraction index is free, so lane (g, t) = (lane / 4,
 //     lane % 4) holds chunks t, t + 4, ... (eight values each) of keys g and g + 8, and the
 //     queries are laid out the same way;
@@ -120,7 +129,7 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 //     and e + 4 of chunk 8 i + g: one byte permutation makes each operand register;
 //   * probabilities: one 8 x 8 transposition between registers turns S^T into P^T.
 // The next keys are loaded while the scores become probabilities, the next values while
-// the next scores are made.
+// the next scores are made, the page number after that one block earlier still.
 // ---------------------------------------------------------------------------------
 constexpr int kOwnWarps = 4;
 
@@ -145,132 +154,212 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
 
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
-// Blocks below `prefix_blocks` take the prefix, the others the requests' own pages; a range
-// is `chunk` keys.  Results of range i go to part i of the prefix's or of the own parts.
+constexpr int kBlockKeys = 16;
+constexpr int kMinRange = 4;  // blocks a warp takes at least
+
 struct PagesPlan {
-    int prefix_blocks, prefix_splits, prefix_chunk;
-    int own_splits, own_chunk;
-    float* prefix_o;
-    float* prefix_lse;
-    float* own_o;
-    float* own_lse;
+    int own_jobs, tiles;  // jobs of own pages: `tiles` of them a request
+    int prefix_jobs;      // 0: the prefix is not taken here
+    int warps;            // of each key head
+    // Results: [slots][kv_heads][8 * NT][dim], their log2-sum-exp, and of each job its first
+    // warp and how many warps it has.
+    float* o;
+    float* lse;
+    int2* where;
 };
 
+// A block of keys: its job, the job's keys, its number in the job and in all.
+struct Cursor {
+    int job, keys, block, at;
+};
+
+__device__ __forceinline__ int job_keys(const SharedArgs& a, const PagesPlan& pl, int job) {
+    if (job >= pl.own_jobs) return (int)a.prefix_len;
+    return min(max(a.lengths[job / pl.tiles], 0), a.table_width << a.page_shift);
+}
+
 template <class H, int D, int NT>
-__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
     pages_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ PagesPlan pl) {
     using T = typename H::type;
     constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key, of a value row
-    constexpr int kRowsHere = 8 * NT;
-    __shared__ float s_o[kOwnWarps][kRowsHere][D + 4];
-    __shared__ float s_m[kOwnWarps][kRowsHere], s_l[kOwnWarps][kRowsHere];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int group = a.heads / a.kv_heads;
-    const bool prefix = (int)blockIdx.x < pl.prefix_blocks;
-    int x = prefix ? blockIdx.x : blockIdx.x - pl.prefix_blocks;
-    const int kh = x % a.kv_heads;  // key heads fastest: blocks that run together read neighbouring memory
-    x /= a.kv_heads;
-    // Rows of this block: row r is query head kh * group + (m0 + r) % group of request
-    // b + (m0 + r) / group.
-    int b, split, m0, n_rows, n, chunk;
-    const int32_t* pages;
-    if (prefix) {
-        split = x % pl.prefix_splits;
-        m0 = x / pl.prefix_splits * kRowsHere;
-        b = 0;
-        n_rows = min(kRowsHere, a.n_requests * group - m0);
-        n = (int)a.prefix_len;
-        chunk = pl.prefix_chunk;
-        pages = a.prefix_pages;
-    } else {
-        const int mt = (group + kRowsHere - 1) / kRowsHere;
-        m0 = x % mt * kRowsHere;
-        x /= mt;
-        split = x % pl.own_splits;
-        b = x / pl.own_splits;
-        n_rows = min(kRowsHere, group - m0);
-        n = min(max(a.lengths[b], 0), a.table_width << a.page_shift);
-        chunk = pl.own_chunk;
-        pages = a.table + (long long)b * a.table_stride;
-    }
-    const long long rows = (long long)a.n_requests * a.heads;
-    auto row_of = [&](int r) { return (long long)(b + (m0 + r) / group) * a.heads + kh * group + (m0 + r) % group; };
-    float* const out_o = (prefix ? pl.prefix_o : pl.own_o) + split * rows * a.dim;
-    float* const out_lse = (prefix ? pl.prefix_lse : pl.own_lse) + split * rows;
+    constexpr int kThreadsHere = kOwnWarps * 32;
+    __shared__ int s_sum[kThreadsHere + 1];
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads, jobs = pl.own_jobs + pl.prefix_jobs;
+    const int warp_all = blockIdx.x * kOwnWarps + (tid >> 5);
+    const int kh = warp_all % a.kv_heads, warp = warp_all / a.kv_heads;  // key heads fastest: neighbours in memory
+    auto blocks_of = [&](int job) { return (job_keys(a, pl, job) + kBlockKeys - 1) / kBlockKeys; };
 
-    const int begin = (int)min((long long)split * chunk, (long long)n), end = min(n, begin + chunk);
-    if (begin >= end) {
-        if (tid < n_rows) out_lse[row_of(tid)] = -INFINITY;
-        return;
+    // Blocks before each thread's share of the jobs.
+    const int per = (jobs + kThreadsHere - 1) / kThreadsHere;
+    int mine = 0;
+    for (int j = tid * per; j < min(jobs, (tid + 1) * per); ++j) mine += blocks_of(j);
+    s_sum[tid + 1] = mine;
+    if (tid == 0) s_sum[0] = 0;
+    __syncthreads();
+    if (tid < 32) {  // four entries a lane
+        int v[kThreadsHere / 32], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kThreadsHere / 32; ++i) sum += v[i] = s_sum[1 + lane * (kThreadsHere / 32) + i];
+        int incl = sum;
+#pragma unroll
+        for (int e = 1; e < 32; e <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl, e);
+            if (lane >= e) incl += u;
+        }
+        int run = incl - sum;
+#pragma unroll
+        for (int i = 0; i < kThreadsHere / 32; ++i) s_sum[1 + lane * (kThreadsHere / 32) + i] = run += v[i];
     }
-    const int blocks = (end - begin + 15) / 16;
+    __syncthreads();
+    const int all = s_sum[kThreadsHere], range = max(kMinRange, (all + pl.warps - 1) / pl.warps);
+    const int begin = (int)min((long long)warp * range, (long long)all), end = min(all, begin + range);
+    if (warp >= pl.warps || begin >= end) return;
+
+    // The job of the warp's first block: the share that holds it, then the job in the share.
+    Cursor cur;
+    {
+        int lo = 0, hi = kThreadsHere;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_sum[mid] <= begin) lo = mid; else hi = mid;
+        }
+        int at = s_sum[lo], job = lo * per, n = blocks_of(job);
+        while (at + n <= begin) {
+            at += n;
+            n = blocks_of(++job);
+        }
+        cur = {job, job_keys(a, pl, job), begin - at, begin};
+    }
+    // The block after c; past the warp's range its contents do not matter.
+    auto after = [&](Cursor c) {
+        ++c.at;
+        ++c.block;
+        if (c.block * kBlockKeys >= c.keys && c.at < end) {
+            c.block = 0;
+            do c.keys = job_keys(a, pl, ++c.job);
+            while (c.keys == 0);
+        }
+        return c;
+    };
+    auto page_of = [&](const Cursor& c) {
+        if (c.at >= end) return -1;
+        const int i = (c.block * kBlockKeys) >> a.page_shift;
+        return c.job >= pl.own_jobs ? a.prefix_pages[i] : a.table[(long long)(c.job / pl.tiles) * a.table_stride + i];
+    };
     const int mask = (1 << a.page_shift) - 1;
-
     uint4 kf[2][KC], vf[4][VC];
-    // 16 keys lie in one page.  Rows past the end are not read: they may hold anything.
-    auto load_k = [&](int ib, int pg) {
-        const int key = begin + ib * 16;
-        const bool ok = ib < blocks && pg >= 0 && pg < a.n_pages;
+    // 16 keys lie in one page.  Rows past the job's keys are not read: they may hold anything.
+    auto load_k = [&](const Cursor& c, int pg) {
+        const int key = c.block * kBlockKeys, left = pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - key : 0;
         const T* p = static_cast<const T*>(a.k_cache.p) + pg * a.k_cache.page + (key & mask) * a.k_cache.tok + kh * a.k_cache.head;
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < KC; ++i) {
-                const int c = (i * 4 + t) * 8;
+                const int ch = (i * 4 + t) * 8;
                 kf[r][i] = make_uint4(0, 0, 0, 0);
-                if (ok && c < a.dim && key + r * 8 + g < end)
-                    kf[r][i] = *reinterpret_cast<const uint4*>(p + (r * 8 + g) * a.k_cache.tok + c);
+                if (ch < a.dim && r * 8 + g < left)
+                    kf[r][i] = *reinterpret_cast<const uint4*>(p + (r * 8 + g) * a.k_cache.tok + ch);
             }
     };
-    auto load_v = [&](int ib, int pg) {
-        const int key = begin + ib * 16;
-        const bool ok = ib < blocks && pg >= 0 && pg < a.n_pages;
+    auto load_v = [&](const Cursor& c, int pg) {
+        const int key = c.block * kBlockKeys, left = pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - key : 0;
         const T* p = static_cast<const T*>(a.v_cache.p) + pg * a.v_cache.page + (key & mask) * a.v_cache.tok + kh * a.v_cache.head;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
-                const int c = (i * 8 + g) * 8, k = 2 * t + (r & 1) + (r >> 1) * 8;
+                const int ch = (i * 8 + g) * 8, k = 2 * t + (r & 1) + (r >> 1) * 8;
                 vf[r][i] = make_uint4(0, 0, 0, 0);
-                if (ok && c < a.dim && key + k < end) vf[r][i] = *reinterpret_cast<const uint4*>(p + k * a.v_cache.tok + c);
+                if (ch < a.dim && k < left) vf[r][i] = *reinterpret_cast<const uint4*>(p + k * a.v_cache.tok + ch);
             }
     };
-    auto page_of = [&](int ib) { return ib < blocks ? pages[(begin + ib * 16) >> a.page_shift] : -1; };
-
-    int ib = warp, pg = page_of(ib), pg_next = page_of(ib + kOwnWarps);
-    load_k(ib, pg);
-    load_v(ib, pg);
-    // Queries, laid out as the keys are.
+    // Rows of a job: row r is query head kh * group + (m0 + r) % group of request
+    // b + (m0 + r) / group.
+    auto first_row = [&](int job) {
+        return job >= pl.own_jobs ? make_int2(0, (job - pl.own_jobs) * 8 * NT) : make_int2(job / pl.tiles, job % pl.tiles * 8 * NT);
+    };
+    auto rows_of = [&](int job) {
+        return min(8 * NT, job >= pl.own_jobs ? a.n_requests * group - (job - pl.own_jobs) * 8 * NT
+                                              : group - job % pl.tiles * 8 * NT);
+    };
     uint32_t qb[NT][2 * KC][2];
+    auto load_q = [&](int job) {  // laid out as the keys are
+        const int2 bm = first_row(job);
+        const int n_rows = rows_of(job);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int r = nt * 8 + g;
-        const T* q = static_cast<const T*>(a.q.p);
-        if (r < n_rows) q += (long long)(b + (m0 + r) / group) * a.q.tok + (kh * group + (m0 + r) % group) * a.q.head;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g;
+            const T* q = static_cast<const T*>(a.q.p);
+            if (r < n_rows) q += (long long)(bm.x + (bm.y + r) / group) * a.q.tok + (kh * group + (bm.y + r) % group) * a.q.head;
 #pragma unroll
-        for (int i = 0; i < KC; ++i) {
-            const int c = (i * 4 + t) * 8;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (c < a.dim && r < n_rows) u = *reinterpret_cast<const uint4*>(q + c);
-            qb[nt][2 * i][0] = u.x; qb[nt][2 * i][1] = u.y;
-            qb[nt][2 * i + 1][0] = u.z; qb[nt][2 * i + 1][1] = u.w;
+            for (int i = 0; i < KC; ++i) {
+                const int ch = (i * 4 + t) * 8;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (ch < a.dim && r < n_rows) u = *reinterpret_cast<const uint4*>(q + ch);
+                qb[nt][2 * i][0] = u.x; qb[nt][2 * i][1] = u.y;
+                qb[nt][2 * i + 1][0] = u.z; qb[nt][2 * i + 1][1] = u.w;
+            }
         }
-    }
+    };
 
     float o[NT][VC][4][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < VC; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[nt][i][e][c] = 0.0f;
     float m[NT][2], l[NT][2];  // of rows 2t and 2t + 1; l over this lane's keys only
+    auto clear = [&] {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[nt][i][e][c] = 0.0f;
+        }
+    };
+    auto flush = [&](int job) {
+        const long long slot = ((long long)(job + warp) * a.kv_heads + kh) * (8 * NT);
+        const int n_rows = rows_of(job);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = nt * 8 + 2 * t + h;
+                float sum = l[nt][h];
+#pragma unroll
+                for (int e = 4; e < 32; e *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+                if (r >= n_rows) continue;
+                const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+#pragma unroll
+                for (int i = 0; i < VC; ++i) {
+                    const int d = (i * 8 + g) * 8;
+                    if (d >= a.dim) continue;
+                    float4* dst = reinterpret_cast<float4*>(pl.o + (slot + r) * a.dim + d);
+                    dst[0] = make_float4(o[nt][i][0][h] * inv, o[nt][i][1][h] * inv, o[nt][i][2][h] * inv, o[nt][i][3][h] * inv);
+                    dst[1] = make_float4(o[nt][i][0][2 + h] * inv, o[nt][i][1][2 + h] * inv, o[nt][i][2][2 + h] * inv,
+                                         o[nt][i][3][2 + h] * inv);
+                }
+                if (g == 0) pl.lse[slot + r] = m[nt][h] + log2f(sum);
+            }
+        __syncwarp();
+        clear();
+    };
+
+    Cursor next = after(cur);
+    int pg = page_of(cur), pg_next = page_of(next);
+    load_q(cur.job);
+    load_k(cur, pg);
+    load_v(cur, pg);
+    clear();
     const float scale = a.scale * kLog2e;
-    for (; ib < blocks; ib += kOwnWarps) {
+    while (true) {
+        if (cur.block == 0 && kh == 0 && lane == 0) {
+            const int last = cur.at + (cur.keys + kBlockKeys - 1) / kBlockKeys - 1;
+            pl.where[cur.job] = make_int2(warp, last / range - warp + 1);
+        }
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -281,15 +370,18 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 2)
                 mma16816<H>(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
             }
         }
-        const int pg_after = page_of(ib + 2 * kOwnWarps);
-        load_k(ib + kOwnWarps, pg_next);
-        const int key = begin + ib * 16 + g;
+        const bool ends = next.at >= end || next.job != cur.job;
+        load_k(next, pg_next);
+        if (next.at < end && next.job != cur.job) load_q(next.job);
+        const Cursor then = after(next);
+        const int pg_then = page_of(then);
+        const int key = cur.block * kBlockKeys + g;
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float top[2];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[nt][c] = key + (c >> 1) * 8 < end ? s[nt][c] * scale : -INFINITY;
+            for (int c = 0; c < 4; ++c) s[nt][c] = key + (c >> 1) * 8 < cur.keys ? s[nt][c] * scale : -INFINITY;
             top[0] = fmaxf(s[nt][0], s[nt][2]);
             top[1] = fmaxf(s[nt][1], s[nt][3]);
 #pragma unroll
@@ -332,74 +424,20 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 2)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma16816<H>(o[nt][i][e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
-        load_v(ib + kOwnWarps, pg_next);
-        pg_next = pg_after;
+        load_v(next, pg_next);
+        if (ends) flush(cur.job);
+        if (next.at >= end) break;
+        cur = next;
+        next = then;
+        pg_next = pg_then;
     }
-
-    // Join of the four warps.
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = nt * 8 + 2 * t + h;
-#pragma unroll
-            for (int e = 4; e < 32; e *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], e);
-            if (g == 0) {
-                s_m[warp][r] = m[nt][h];
-                s_l[warp][r] = l[nt][h];
-            }
-#pragma unroll
-            for (int i = 0; i < VC; ++i) {
-                float4* dst = reinterpret_cast<float4*>(&s_o[warp][r][(i * 8 + g) * 8]);
-                dst[0] = make_float4(o[nt][i][0][h], o[nt][i][1][h], o[nt][i][2][h], o[nt][i][3][h]);
-                dst[1] = make_float4(o[nt][i][0][2 + h], o[nt][i][1][2 + h], o[nt][i][2][2 + h], o[nt][i][3][2 + h]);
-            }
-        }
-    __syncthreads();
-    constexpr int kPerRow = kOwnWarps * 32 / kRowsHere;
-    const int r = tid / kPerRow;
-    if (r >= n_rows) return;
-    float top = -INFINITY, total = 0.0f, w[kOwnWarps];
-#pragma unroll
-    for (int i = 0; i < kOwnWarps; ++i) top = fmaxf(top, s_m[i][r]);
-#pragma unroll
-    for (int i = 0; i < kOwnWarps; ++i) {
-        // a warp without keys has m = -inf, and zeros
-        w[i] = s_m[i][r] == -INFINITY ? 0.0f : attn::ex2(s_m[i][r] - top);
-        total += s_l[i][r] * (i < blocks && s_m[i][r] == -INFINITY ? 1.0f : w[i]);
-    }
-    const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
-    const long long row = row_of(r);
-    for (int d = tid % kPerRow * 4; d < a.dim; d += kPerRow * 4) {
-        float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < kOwnWarps; ++i) {
-            const float4 v = *reinterpret_cast<const float4*>(&s_o[i][r][d]);
-            acc = make_float4(acc.x + w[i] * v.x, acc.y + w[i] * v.y, acc.z + w[i] * v.z, acc.w + w[i] * v.w);
-        }
-        *reinterpret_cast<float4*>(out_o + row * a.dim + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    }
-    if (tid % kPerRow == 0) out_lse[row] = top + log2f(total);
-}
-
-// The lengths are on the device: ranges are cut for what the table can hold.  A range past a
-// request's length costs one write a row.
-int keys_a_range(long long cap, long long blocks_a_range) {
-    // four blocks an SM fill the GPU; 128 keys at least a range, 512 at most, so that the
-    // longest request does not run on alone
-    long long s = std::max<long long>(ceil_div(4 * kSms, std::max<long long>(blocks_a_range, 1)), ceil_div(cap, 512));
-    s = std::max<long long>(1, std::min<long long>(s, (cap + 127) / 128));
-    return (int)((ceil_div(cap, s) + 63) / 64 * 64);
 }
 
 template <class H>
 void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, cudaStream_t st) {
-    const int group = a.heads / a.kv_heads;
-    const long long blocks =
-        pl.prefix_blocks + (long long)a.n_requests * a.kv_heads * ((group + 8 * nt - 1) / (8 * nt)) * pl.own_splits;
-    if (blocks > 0x7fffffffLL) throw CudaError("attention: too many requests for one launch");
-    if (blocks == 0) return;
-    auto launch = [&](auto* kernel) { kernel<<<(unsigned)blocks, kOwnWarps * 32, 0, st>>>(a, pl); };
+    if (pl.own_jobs + pl.prefix_jobs == 0) return;
+    const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
+    auto launch = [&](auto* kernel) { kernel<<<blocks, kOwnWarps * 32, 0, st>>>(a, pl); };
     if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
     else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
     VGPU_LAUNCH("pages_kernel");
@@ -407,40 +445,91 @@ void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, cudaStream_t
 
 // ---------------------------------------------------------------------------------
 // Join of partial results: with L_i their log2-sum-exp and M = max L_i, the weights are
-// 2^(L_i - M) and out = sum w_i O_i / sum w_i.  One warp a row.
+// 2^(L_i - M) and out = sum w_i O_i / sum w_i.  One warp a row, one part a lane.  A row's
+// parts are `splits` of the tile kernel ([splits][rows][dim]) and the slots of its jobs in
+// the pages kernel.
 // ---------------------------------------------------------------------------------
+struct JoinArgs {
+    long long rows;  // n * heads
+    int heads, kv_heads, dim;
+    int splits;
+    const float* tile_o;
+    const float* tile_lse;
+    bool paged;
+    int nt;
+    PagesPlan pages;
+    const int32_t* lengths;
+    bool own;  // there are own pages
+    void* out;
+    float* lse;
+};
+
 template <class H>
-__global__ void __launch_bounds__(128) join_kernel(int parts, long long rows, int dim, const float* __restrict__ part_o,
-                                                   const float* __restrict__ part_lse, void* out, float* lse) {
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs a) {
     const int lane = threadIdx.x & 31;
     const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const bool live = lane * 4 < dim;
+    if (row >= a.rows) return;
+    const bool live = lane * 4 < a.dim;
+    // Slots of the row's own job, then of its prefix job.
+    const int head = (int)(row % a.heads), group = a.heads / a.kv_heads, kh = head / group, g = head - kh * group;
+    const int b = (int)(row / a.heads);
+    int own = 0, shared = 0;
+    long long own_at = 0, shared_at = 0;  // rows of slots
+    if (a.paged) {
+        const int tall = 8 * a.nt;
+        if (a.own && a.lengths[b] > 0) {
+            const int job = b * a.pages.tiles + g / tall;
+            const int2 w = a.pages.where[job];
+            own = w.y;
+            own_at = ((long long)(job + w.x) * a.kv_heads + kh) * tall + g % tall;
+        }
+        if (a.pages.prefix_jobs) {
+            const long long r = (long long)b * group + g;
+            const int job = a.pages.own_jobs + (int)(r / tall);
+            const int2 w = a.pages.where[job];
+            shared = w.y;
+            shared_at = ((long long)(job + w.x) * a.kv_heads + kh) * tall + (int)(r % tall);
+        }
+    }
+    const long long slot_rows = (long long)a.kv_heads * 8 * a.nt;
+    const int parts = a.splits + own + shared;
     float m = -INFINITY, total = 0.0f;
     bool nan = false;
     float4 o = make_float4(0, 0, 0, 0);
-    for (int p0 = 0; p0 < parts; p0 += 32) {  // the weights of 32 parts, one a lane
-        const float x = p0 + lane < parts ? part_lse[(p0 + lane) * rows + row] : -INFINITY;
-        float up = m;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        const int p = p0 + lane;
+        const float* src = a.pages.o;  // the lane's part
+        float x = -INFINITY;
+        if (p < a.splits) {
+            x = a.tile_lse[p * a.rows + row];
+            src = a.tile_o + (p * a.rows + row) * a.dim;
+        } else if (p < parts) {
+            const int i = p - a.splits;
+            const long long at = i < own ? own_at + i * slot_rows : shared_at + (i - own) * slot_rows;
+            x = a.pages.lse[at];
+            src = a.pages.o + at * a.dim;
+        }
+        float up = fmaxf(m, x);
         nan |= __any_sync(0xffffffffu, isnan(x)) != 0;
-        up = fmaxf(up, x);
 #pragma unroll
         for (int e = 16; e > 0; e >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, e));
         const float ref = up == -INFINITY ? 0.0f : up, f = exp2f(m - ref), w = exp2f(x - ref);
         m = up;
         total = total * f + w;  // this lane's share
         o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-        unsigned some = __ballot_sync(0xffffffffu, w > 0.0f);  // parts without keys hold no rows
+        unsigned some = __ballot_sync(0xffffffffu, w > 0.0f);  // the others add nothing, and may hold anything
         while (some) {
             float4 v[4];
             float wi[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = some ? __ffs(some) - 1 : -1;
-                wi[e] = __shfl_sync(0xffffffffu, w, i < 0 ? 0 : i);
+                const int i = some ? __ffs(some) - 1 : -1, from = i < 0 ? 0 : i;
+                wi[e] = __shfl_sync(0xffffffffu, w, from);
+                const float* s = reinterpret_cast<const float*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), from));
                 v[e] = make_float4(0, 0, 0, 0);
                 if (i < 0) wi[e] = 0.0f;
-                else if (live) v[e] = *reinterpret_cast<const float4*>(part_o + ((p0 + i) * rows + row) * dim + lane * 4);
+                else if (live) v[e] = *reinterpret_cast<const float4*>(s + lane * 4);
                 some &= some - 1;
             }
 #pragma unroll
@@ -452,16 +541,15 @@ __global__ void __launch_bounds__(128) join_kernel(int parts, long long rows, in
     for (int e = 16; e > 0; e >>= 1) total += __shfl_xor_sync(0xffffffffu, total, e);
     const float inv = nan ? __int_as_float(0x7fc00000) : (total > 0.0f ? 1.0f / total : 0.0f);
     if (live)
-        *reinterpret_cast<uint2*>(static_cast<typename H::type*>(out) + row * dim + lane * 4) =
+        *reinterpret_cast<uint2*>(static_cast<typename H::type*>(a.out) + row * a.dim + lane * 4) =
             make_uint2(H::pack(o.x * inv, o.y * inv), H::pack(o.z * inv, o.w * inv));
-    if (lse && lane == 0) lse[row] = nan ? __int_as_float(0x7fc00000) : (m + log2f(total)) / kLog2e;
+    if (a.lse && lane == 0) a.lse[row] = nan ? __int_as_float(0x7fc00000) : (m + log2f(total)) / kLog2e;
 }
 
-void launch_join(bool f16, int parts, long long rows, int dim, const float* part_o, const float* part_lse, void* out,
-                 float* lse, cudaStream_t st) {
-    const int blocks = ceil_div(rows, 4);
-    if (f16) join_kernel<F16><<<blocks, 128, 0, st>>>(parts, rows, dim, part_o, part_lse, out, lse);
-    else join_kernel<Bf16><<<blocks, 128, 0, st>>>(parts, rows, dim, part_o, part_lse, out, lse);
+void launch_join(bool f16, const JoinArgs& a, cudaStream_t st) {
+    const int blocks = ceil_div(a.rows, 4);
+    if (f16) join_kernel<F16><<<blocks, 128, 0, st>>>(a);
+    else join_kernel<Bf16><<<blocks, 128, 0, st>>>(a);
     VGPU_LAUNCH("join_kernel");
 }
 
@@ -487,30 +575,41 @@ PromptPlan prompt_plan(const PromptArgs& a) {
     return pl;
 }
 
-// Parts of the prefix, then of the own pages.
+// Workspace of a shared-prefix call: the tile kernel's parts, the pages kernel's slots.
 struct SharedPlan {
-    bool tiles;  // the prefix goes to the tensor cores' tiles
-    int prefix_splits, prefix_chunk, own_splits, own_chunk, nt;
+    int splits;  // of the prefix on the tensor cores' tiles; 0: the pages kernel takes it
+    int nt;
+    PagesPlan pages;
+    // In floats: the tiles' rows come first, then the slots' rows (both 16-byte aligned, as
+    // dim is a multiple of 8), then both log2-sum-exps and the jobs' slots.
+    size_t slots_at, tile_lse_at, slot_lse_at, where_at;
+    size_t bytes;
 };
 SharedPlan shared_plan(const SharedArgs& a) {
     SharedPlan p{};
     const int group = a.heads / a.kv_heads;
-    const long long rows = (long long)a.n_requests * group;  // of one key head
     p.nt = group > 8 ? 2 : 1;
-    const long long cap = (long long)a.table_width << a.page_shift;
-    const long long own_blocks = (long long)a.n_requests * a.kv_heads * ((group + 8 * p.nt - 1) / (8 * p.nt));
-    p.own_chunk = cap ? keys_a_range(cap, own_blocks) : 0;
-    p.own_splits = cap ? (int)((cap + p.own_chunk - 1) / p.own_chunk) : 0;
-    if (a.prefix_len == 0) return p;
-    const long long row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
-    p.tiles = row_tiles > kFewRowTiles;
-    if (p.tiles) {
-        const int span = 2 * (kRows / group);
-        p.prefix_splits = splits_for((long long)ceil_div(a.n_requests, span) * a.kv_heads, a.prefix_len / kKeys);
-    } else {
-        p.prefix_chunk = keys_a_range(a.prefix_len, row_tiles * a.kv_heads);
-        p.prefix_splits = (int)((a.prefix_len + p.prefix_chunk - 1) / p.prefix_chunk);
+    const int tall = 8 * p.nt;
+    const long long rows = (long long)a.n_requests * a.heads;
+    const long long row_tiles = ((long long)a.n_requests * group + tall - 1) / tall;
+    p.pages.tiles = (group + tall - 1) / tall;
+    p.pages.own_jobs = a.table_width ? a.n_requests * p.pages.tiles : 0;
+    if (a.prefix_len) {
+        if (row_tiles <= kFewRowTiles) p.pages.prefix_jobs = (int)row_tiles;
+        else p.splits = splits_for((long long)ceil_div(a.n_requests, 2 * (kRows / group)) * a.kv_heads, a.prefix_len / kKeys);
     }
+    const long long jobs = (long long)p.pages.own_jobs + p.pages.prefix_jobs;
+    // as many warps as are resident at once, and no more than the keys can use
+    const long long cap = (((long long)a.table_width << a.page_shift) + kBlockKeys - 1) / kBlockKeys;
+    const long long most = p.pages.own_jobs * cap + p.pages.prefix_jobs * ((a.prefix_len + kBlockKeys - 1) / kBlockKeys);
+    const long long resident = (long long)kSms * (p.nt == 1 ? 3 : 2) * kOwnWarps / a.kv_heads;
+    p.pages.warps = (int)std::max<long long>(1, std::min<long long>(resident, (most + kMinRange - 1) / kMinRange));
+    const size_t slot_rows = jobs ? (size_t)(jobs + p.pages.warps) * a.kv_heads * tall : 0;
+    p.slots_at = (size_t)p.splits * rows * a.dim;
+    p.tile_lse_at = p.slots_at + slot_rows * a.dim;
+    p.slot_lse_at = p.tile_lse_at + (size_t)p.splits * rows;
+    p.where_at = (p.slot_lse_at + slot_rows + 1) / 2 * 2;
+    p.bytes = (p.where_at + 2 * (size_t)jobs) * sizeof(float);
     return p;
 }
 
@@ -546,27 +645,35 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
     p.part_o = static_cast<float*>(a.workspace);
     p.part_lse = p.part_o + pl.splits * rows * a.dim;
     launch_tiles<false>(p, a.f16, pl.tiles * a.kv_heads * pl.splits, st);
-    if (p.part) launch_join(a.f16, pl.splits, rows, a.dim, p.part_o, p.part_lse, a.out, a.lse, st);
+    if (!p.part) return;
+    JoinArgs j{};
+    j.rows = rows;
+    j.heads = a.heads;
+    j.kv_heads = a.kv_heads;
+    j.dim = a.dim;
+    j.splits = pl.splits;
+    j.tile_o = p.part_o;
+    j.tile_lse = p.part_lse;
+    j.out = a.out;
+    j.lse = a.lse;
+    launch_join(a.f16, j, st);
 }
 
-size_t shared_attention_workspace(const SharedArgs& a) {
-    if (a.n_requests == 0) return 0;
-    const SharedPlan sp = shared_plan(a);
-    return part_bytes(sp.prefix_splits + sp.own_splits, (long long)a.n_requests * a.heads, a.dim);
-}
+size_t shared_attention_workspace(const SharedArgs& a) { return a.n_requests == 0 ? 0 : shared_plan(a).bytes; }
 
 void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
+    SharedPlan sp = shared_plan(a);
     const long long rows = (long long)a.n_requests * a.heads;
-    const SharedPlan sp = shared_plan(a);
-    const int parts = sp.prefix_splits + sp.own_splits;
-    float* part_o = static_cast<float*>(a.workspace);
-    float* part_lse = part_o + parts * rows * a.dim;
-    PagesPlan pl{};
-    pl.own_splits = sp.own_splits;
-    pl.own_chunk = sp.own_chunk;
-    pl.own_o = part_o + sp.prefix_splits * rows * a.dim;
-    pl.own_lse = part_lse + sp.prefix_splits * rows;
-    if (sp.tiles) {
+    float* const base = static_cast<float*>(a.workspace);
+    JoinArgs j{};
+    j.rows = rows;
+    j.heads = a.heads;
+    j.kv_heads = a.kv_heads;
+    j.dim = a.dim;
+    j.splits = sp.splits;
+    j.tile_o = base;
+    j.tile_lse = base + sp.tile_lse_at;
+    if (sp.splits) {
         TileParams p{};
         fill_queries(p, a.f16, a.q, a.heads, a.kv_heads, a.dim, a.n_requests);
         const int page = 1 << a.page_shift, box = std::min(page, kKeys);
@@ -577,22 +684,25 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
         p.pages = a.prefix_pages;
         p.page_shift = a.page_shift;
         p.scale_log2 = a.scale * kLog2e;
-        p.splits = sp.prefix_splits;
+        p.splits = sp.splits;
         p.part = true;
-        p.part_o = part_o;
-        p.part_lse = part_lse;
+        p.part_o = base;
+        p.part_lse = base + sp.tile_lse_at;
         launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * p.splits, st);
-    } else if (sp.prefix_splits) {
-        const long long row_tiles = ((long long)a.n_requests * (a.heads / a.kv_heads) + 8 * sp.nt - 1) / (8 * sp.nt);
-        pl.prefix_blocks = (int)(row_tiles * a.kv_heads * sp.prefix_splits);
-        pl.prefix_splits = sp.prefix_splits;
-        pl.prefix_chunk = sp.prefix_chunk;
-        pl.prefix_o = part_o;
-        pl.prefix_lse = part_lse;
     }
-    if (a.f16) launch_pages<F16>(a, pl, sp.nt, st);
-    else launch_pages<Bf16>(a, pl, sp.nt, st);
-    launch_join(a.f16, parts, rows, a.dim, part_o, part_lse, a.out, a.lse, st);
+    sp.pages.o = base + sp.slots_at;
+    sp.pages.lse = base + sp.slot_lse_at;
+    sp.pages.where = reinterpret_cast<int2*>(base + sp.where_at);
+    if (a.f16) launch_pages<F16>(a, sp.pages, sp.nt, st);
+    else launch_pages<Bf16>(a, sp.pages, sp.nt, st);
+    j.paged = true;
+    j.nt = sp.nt;
+    j.pages = sp.pages;
+    j.lengths = a.lengths;
+    j.own = sp.pages.own_jobs > 0;
+    j.out = a.out;
+    j.lse = a.lse;
+    launch_join(a.f16, j, st);
 }
 
 }  // namespace vgpu
