@@ -249,6 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     Work* const s_work = reinterpret_cast<Work*>(tmem_slot + 2);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // The own pages' kernel may be queued behind this one and does not depend on it.
+    if (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int block = blockIdx.x;
     const int kh = block % p.kv_heads;
     block /= p.kv_heads;

@@ -155,7 +155,7 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
 constexpr int kBlockKeys = 16;
-constexpr int kMinRange = 4;  // blocks a warp takes at least
+constexpr int kMinRange = 2;  // blocks a warp takes at least
 
 struct PagesPlan {
     int own_jobs, tiles;  // jobs of own pages: `tiles` of them a request
@@ -434,10 +434,23 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
 }
 
 template <class H>
-void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, cudaStream_t st) {
+void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, bool after_tiles, cudaStream_t st) {
     if (pl.own_jobs + pl.prefix_jobs == 0) return;
     const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
-    auto launch = [&](auto* kernel) { kernel<<<blocks, kOwnWarps * 32, 0, st>>>(a, pl); };
+    // After the prefix's tiles: nothing here depends on them, and they leave SMs idle, so
+    // the blocks may start as soon as all of the tiles' blocks have.
+    auto launch = [&](auto* kernel) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(kOwnWarps * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = after_tiles ? 1 : 0;
+        VGPU_CHECK(cudaLaunchKernelEx(&cfg, kernel, a, pl));
+    };
     if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
     else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
     VGPU_LAUNCH("pages_kernel");
@@ -602,7 +615,8 @@ SharedPlan shared_plan(const SharedArgs& a) {
     // as many warps as are resident at once, and no more than the keys can use
     const long long cap = (((long long)a.table_width << a.page_shift) + kBlockKeys - 1) / kBlockKeys;
     const long long most = p.pages.own_jobs * cap + p.pages.prefix_jobs * ((a.prefix_len + kBlockKeys - 1) / kBlockKeys);
-    const long long resident = (long long)kSms * (p.nt == 1 ? 3 : 2) * kOwnWarps / a.kv_heads;
+    // (four times that after the tiles: their SMs come free one by one)
+    const long long resident = (long long)kSms * (p.nt == 1 ? 3 : 2) * kOwnWarps * (p.splits ? 4 : 1) / a.kv_heads;
     p.pages.warps = (int)std::max<long long>(1, std::min<long long>(resident, (most + kMinRange - 1) / kMinRange));
     const size_t slot_rows = jobs ? (size_t)(jobs + p.pages.warps) * a.kv_heads * tall : 0;
     p.slots_at = (size_t)p.splits * rows * a.dim;
@@ -693,8 +707,8 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
     sp.pages.o = base + sp.slots_at;
     sp.pages.lse = base + sp.slot_lse_at;
     sp.pages.where = reinterpret_cast<int2*>(base + sp.where_at);
-    if (a.f16) launch_pages<F16>(a, sp.pages, sp.nt, st);
-    else launch_pages<Bf16>(a, sp.pages, sp.nt, st);
+    if (a.f16) launch_pages<F16>(a, sp.pages, sp.nt, sp.splits > 0, st);
+    else launch_pages<Bf16>(a, sp.pages, sp.nt, sp.splits > 0, st);
     j.paged = true;
     j.nt = sp.nt;
     j.pages = sp.pages;
