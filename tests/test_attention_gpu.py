@@ -549,3 +549,39 @@ def test_operators_in_a_graph_and_on_a_side_stream(V):
         graph.replay()
         replayed = out.clone()
         assert torch.equal(replayed, step())
+
+
+# Prompts whose mean is above what goes to the small blocks: every head layout on the tensor-memory tiles too.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 128), (4, 4, 64), (7, 1, 128), (6, 2, 96), (2, 1, 40), (3, 3, 8),
+                                        (16, 1, 64), (24, 1, 72), (100, 1, 64), (128, 1, 128)])
+def test_prompt_heads_and_types_long(V, dtype, causal, heads, kv, d):
+    check_prompt(V, [700, 1, 333, 0, 1300], None, heads, kv, d, dtype, causal, seed=heads)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 128), (2, 2, 64)])
+def test_prompt_unseen_values_do_not_leak_long(V, bad, heads, kv, d):
+    """One non-finite value row in the middle of a long prompt, and one neighbouring prompt full of them."""
+    lens = [900, 300, 1100]
+    n = sum(lens)
+    q, k, v = rand(n, heads, d, seed=1), rand(n, kv, d, seed=2), rand(n, kv, d, seed=3)
+    clean = V.prompt_attention(q, k, v, starts_of(lens))
+    v2, k2 = v.clone(), k.clone()
+    v2[500, :, d // 2] = bad
+    v2[900:1200], k2[900:1200] = bad, bad
+    out = V.prompt_attention(q, k2, v2, starts_of(lens))
+    err = (out.double() - clean.double()).abs()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[500:1200] = False
+    assert err[keep].max() <= 2.0 ** -7 * clean.double().abs().max()
+    assert torch.isfinite(out[500:900, :, :d // 2]).all() and not torch.isfinite(out[500:900, :, d // 2]).any()
+
+
+def test_prompt_many_requests(V):
+    """More requests than one step of the search for a block's request looks at, empty ones among them."""
+    lens = [(i * 7919) % 23 if i % 5 else 0 for i in range(1500)] + [2000]
+    check_prompt(V, lens, None, 2, 1, 64, torch.bfloat16, True, seed=3)
+    lens = [1] * 40 + [0] * 40 + [9000]
+    check_prompt(V, lens, None, 2, 1, 64, torch.bfloat16, False, seed=4)

@@ -1,0 +1,260 @@
+// Attention of short prompts: the same rows and masks as attn_tile.cuh, in small blocks.
+//
+// A prompt of a few hundred tokens gives a tensor-memory tile little to overlap: setting it
+// up and draining it takes 8 us of an SM that holds one block.  Here a block is four warps of
+// 16 rows (64 / group tokens with the query heads of one key head), takes the keys 64 at a
+// time through two shared-memory stages filled by asynchronous copies, multiplies with
+// m16n8k16 steps of each warp, and an SM holds three or more such blocks.
+//
+// Rows of the stages are 16-byte chunks XORed with the row, so that the eight rows of a
+// matrix load lie in different banks.  Softmax as in attn_tile.cuh: one pass, running maximum
+// and sum in 32 bits, P rounded to the data's type for the second product.  Value rows past
+// the last key are filled with zeros by the copy; where a later token of the same prompt holds
+// a non-finite value (checked on the diagonal tiles) the block recomputes its rows one key at
+// a time.
+#pragma once
+
+#include "attn_tile.cuh"
+
+namespace vgpu {
+namespace attn {
+
+constexpr int kShortRows = 64, kShortKeys = 64, kShortThreads = 128;
+
+template <class H>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if (std::is_same<H, Bf16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// 16 bytes to shared memory, zeros where `some` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool some) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
+}
+
+template <class H, int D>
+__global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_kernel(const __grid_constant__ TileParams p) {
+    using T = typename H::type;
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int kChunks = D / 8, kRowBytes = D * 2, kTileBytes = kShortKeys * kRowBytes;
+    __shared__ Work s_work;
+    __shared__ int s_leak;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kh = blockIdx.x % p.kv_heads;
+    if (warp == 0) {
+        const Work w = find_work(p, blockIdx.x / p.kv_heads, lane, p.tile_tokens);
+        if (lane == 0) {
+            s_work = w;
+            s_leak = 0;
+        }
+    }
+    __syncthreads();
+    const Work w = s_work;
+    const int tokens = min(w.tokens, p.tile_tokens);
+    if (tokens <= 0) return;
+    const int last = min(w.len_k, w.first_lim + w.step * (tokens - 1));  // keys the last row sees
+    const int n = (max(last, 0) + kShortKeys - 1) / kShortKeys;
+    const int min_lim = min(max(w.first_lim, 0), w.len_k);  // keys that every row sees
+
+    const uint32_t s_kv = tc::smem_u32(smem);
+    auto request = [&](int j) {
+        const uint32_t dst = s_kv + (j & 1) * 2 * kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kShortKeys * kChunks / kShortThreads; ++i) {
+            const int e = i * kShortThreads + tid, row = e / kChunks, c = e % kChunks;
+            const long long key = w.k0 + min(j * kShortKeys + row, w.len_k - 1);
+            const bool some = j * kShortKeys + row < w.len_k && c * 8 < p.dim;
+            const uint32_t at = row * kRowBytes + ((c ^ (row & 7)) << 4);
+            const int d = c * 8 < p.dim ? c * 8 : 0;
+            copy16(dst + at, static_cast<const T*>(p.k.p) + key * p.k.tok + kh * p.k.head + d, some);
+            copy16(dst + kTileBytes + at, static_cast<const T*>(p.v.p) + key * p.v.tok + kh * p.v.head + d, some);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (n > 0) request(0);
+
+    // Rows g and g + 8 of the warp's 16.
+    int lim[2];
+    long long out_row[2];
+    bool valid[2];
+    const T* q_row[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = warp * 16 + g + 8 * h, tok = row / p.group, head = kh * p.group + row - tok * p.group;
+        valid[h] = tok < tokens;
+        lim[h] = valid[h] ? min(max(w.first_lim + w.step * tok, 0), w.len_k) : 0;
+        out_row[h] = (long long)(w.q0 + tok) * p.heads + head;
+        q_row[h] = static_cast<const T*>(p.q.p) + (w.q0 + (valid[h] ? tok : 0)) * p.q.tok + (valid[h] ? head : kh * p.group) * p.q.head;
+    }
+    uint32_t qa[D / 16][4];
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = k * 16 + 2 * t + (i >> 1) * 8;
+            qa[k][i] = d < p.dim ? *reinterpret_cast<const uint32_t*>(q_row[i & 1] + d) : 0u;
+        }
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    // Matrix loads: lane's row and chunk within a 16 x 16 piece.
+    const int r16 = (lane & 7) + ((lane >> 4) << 3), c16 = (lane >> 3) & 1;    // keys: rows 0-7, 8-15 by lane / 16
+    const int rv = (lane & 7) + (((lane >> 3) & 1) << 3), cv = lane >> 4;      // values: rows by lane / 8, columns by lane / 16
+    for (int j = 0; j < n; ++j) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        if (j + 1 < n) request(j + 1);
+        const uint32_t sk = s_kv + (j & 1) * 2 * kTileBytes, sv = sk + kTileBytes;
+        const int key = j * kShortKeys;
+        if (w.step && key + kShortKeys > min_lim) {  // value rows that some row must not see
+            const int from = max(min_lim - key, 0), end = min(w.len_k - key, kShortKeys);
+            bool bad = false;
+            for (int i = from * kChunks + tid; i < end * kChunks; i += kShortThreads)
+                bad |= not_finite<H>(*reinterpret_cast<const uint4*>(smem + (j & 1) * 2 * kTileBytes + kTileBytes + i * 16));
+            if (bad) s_leak = 1;
+        }
+        float s[kShortKeys / 8][4];
+#pragma unroll
+        for (int i = 0; i < kShortKeys / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int i = 0; i < kShortKeys / 16; ++i) {
+                uint32_t b[4];
+                const int row = i * 16 + r16;
+                ldsm4(b, sk + row * kRowBytes + (((2 * k + c16) ^ (row & 7)) << 4));
+                mma16816<H>(s[2 * i], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[0], b[1]);
+                mma16816<H>(s[2 * i + 1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[2], b[3]);
+            }
+        if (key + kShortKeys > min_lim) {
+#pragma unroll
+            for (int i = 0; i < kShortKeys / 8; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (key + i * 8 + 2 * t + (c & 1) >= lim[c >> 1]) s[i][c] = -INFINITY;
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kShortKeys / 8; ++i) {
+            top[0] = max3(top[0], s[i][0], s[i][1]);
+            top[1] = max3(top[1], s[i][2], s[i][3]);
+        }
+        float f[2], ref[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float a = __shfl_xor_sync(0xffffffffu, top[h], 1);
+            const float b = max3(top[h], a, a), c = __shfl_xor_sync(0xffffffffu, b, 2);
+            float up = max3(m[h], b * p.scale_log2, c * p.scale_log2);
+            if (up == INFINITY) up = __int_as_float(0x7fc00000);
+            f[h] = up == m[h] ? 1.0f : ex2(m[h] - up);
+            m[h] = up;
+            ref[h] = up == -INFINITY ? 0.0f : up;
+            l[h] *= f[h];
+        }
+        if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= f[0];
+                o[i][1] *= f[0];
+                o[i][2] *= f[1];
+                o[i][3] *= f[1];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kShortKeys / 16; ++k) {
+            uint32_t pa[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float* x = s[2 * k + e];
+                const float p0 = ex2(fmaf(x[0], p.scale_log2, -ref[0])), p1 = ex2(fmaf(x[1], p.scale_log2, -ref[0]));
+                const float p2 = ex2(fmaf(x[2], p.scale_log2, -ref[1])), p3 = ex2(fmaf(x[3], p.scale_log2, -ref[1]));
+                l[0] += p0 + p1;
+                l[1] += p2 + p3;
+                pa[2 * e] = H::pack(p0, p1);
+                pa[2 * e + 1] = H::pack(p2, p3);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t b[4];
+                const int row = k * 16 + rv;
+                ldsm4_t(b, sv + row * kRowBytes + (((2 * i + cv) ^ (row & 7)) << 4));
+                mma16816<H>(o[2 * i], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+                mma16816<H>(o[2 * i + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+            }
+        }
+    }
+    __syncthreads();
+    const bool leak = *static_cast<volatile int*>(&s_leak) != 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (!valid[h]) continue;
+        const float inv = l[h] > 0.0f ? 1.0f / l[h] : (l[h] == 0.0f ? 0.0f : l[h]);
+        T* const dst = static_cast<T*>(p.out) + out_row[h] * p.dim;
+        if (!leak) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const int d = i * 8 + 2 * t;
+                if (d < p.dim) {
+                    const float x = l[h] == 0.0f ? 0.0f : o[i][2 * h] * inv, y = l[h] == 0.0f ? 0.0f : o[i][2 * h + 1] * inv;
+                    *reinterpret_cast<uint32_t*>(dst + d) = H::pack(x, y);
+                }
+            }
+        } else {
+            // One key at a time, with the maximum and sum that the scores gave; a lane of the
+            // four that hold the row takes every fourth chunk of it.
+            const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + kh * p.k.head;
+            const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + kh * p.v.head;
+            const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll 1
+            for (int c = t * 8; c < p.dim; c += 32) {
+                float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+                for (int key = 0; key < lim[h]; ++key) {
+                    float s = 0.0f, a[8], b[8];
+#pragma unroll 1
+                    for (int e = 0; e < p.dim; e += 8) {
+                        unpack8<H>(*reinterpret_cast<const uint4*>(q_row[h] + e), a);
+                        unpack8<H>(*reinterpret_cast<const uint4*>(k + key * p.k.tok + e), b);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+                    }
+                    const float x = ex2(fmaf(s, p.scale_log2, -ref));
+                    unpack8<H>(*reinterpret_cast<const uint4*>(v + key * p.v.tok + c), b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] += x * b[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] *= inv;
+                *reinterpret_cast<uint4*>(dst + c) = pack8<H>(acc);
+            }
+        }
+        if (p.lse && t == 0) p.lse[out_row[h]] = (m[h] + log2f(l[h])) * 0.6931471805599453f;
+    }
+}
+
+template <int D>
+constexpr int short_smem_bytes() {
+    return 4 * kShortKeys * D * 2;
+}
+
+}  // namespace attn
+}  // namespace vgpu

@@ -156,64 +156,47 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // What a block works on.
 struct Work {
     int q0;        // first row of q of the block's first tile
-    int tokens;    // rows of the request from there on (at most 2 tiles of them count)
+    int tokens;    // rows of the request from there on (those past the block's tiles do not count)
     int k0, len_k; // first key row, keys of the request
     int first_lim; // keys that the first of these rows sees; each later one sees `step` more
     int step;
     int split;
 };
 
-// Tile `idx` (two query tiles each) of the packed requests, last ones first: the rows of a
-// causal prompt's end see the most keys.  Run by one whole warp; tokens = 0: no such tile.
-// Rows before the first and after the last request are requests without keys.
-__device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane) {
-    Work w{};
-    const int n = p.n_requests + 2, per = (n + 31) / 32, span = 2 * p.tile_tokens;
-    const int b0 = lane * per, b1 = min(n, b0 + per);
-    auto bound = [&](int b) {  // first row of piece b
+// Piece `idx` of the packed requests, each cut into `span` tokens.  Run by one whole warp;
+// tokens <= 0: no such piece.  Request b's pieces have the numbers from starts[b] / span + b
+// on, which leaves room for each (some numbers stay unused) and can be searched without
+// adding up lengths: 32 candidates a step.  Rows before the first and after the last request
+// are requests without keys.  Last pieces come first: the rows of a causal prompt's end see
+// the most keys.
+__device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane, int span) {
+    const int n = p.n_requests + 2;
+    auto bound = [&](int b) {  // first row of request b
         if (b == 0) return 0;
         if (b >= n) return p.n_q;
         return min(max(p.starts[b - 1], 0), p.n_q);
     };
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (max(bound(b + 1) - bound(b), 0) + span - 1) / span;
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
+    const int want = p.n_q / span + n - 1 - idx;
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, c = lo + (lane + 1) * step;
+        const bool before = c < hi && bound(c) / span + c <= want;
+        lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+        hi = min(hi, lo + step);
     }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
-    const int want = total - 1 - idx;
-    const bool here = want >= 0 && want >= incl - mine && want < incl;
-    if (here) {
-        int at = incl - mine, b = b0;
-        for (;; ++b) {
-            const int t = (max(bound(b + 1) - bound(b), 0) + span - 1) / span;
-            if (want < at + t) break;
-            at += t;
-        }
-        const int q0 = bound(b), len_q = bound(b + 1) - q0, tok = (want - at) * span;
-        int k0 = 0, k1 = 0;
-        if (b > 0 && b <= p.n_requests) {
-            k0 = min(max(p.starts_k[b - 1], 0), p.n_k);
-            k1 = min(max(p.starts_k[b], k0), p.n_k);
-        }
-        w.q0 = q0 + tok;
-        w.tokens = len_q - tok;
-        w.k0 = k0;
-        w.len_k = k1 - k0;
-        w.step = p.causal ? 1 : 0;
-        w.first_lim = p.causal ? tok + 1 + w.len_k - len_q : w.len_k;
+    Work w{};
+    const int q0 = bound(lo), len_q = bound(lo + 1) - q0, tok = (want - q0 / span - lo) * span;
+    w.q0 = q0 + tok;
+    w.tokens = tok >= 0 ? len_q - tok : 0;
+    int k0 = 0, k1 = 0;
+    if (lo > 0 && lo <= p.n_requests) {
+        k0 = min(max(p.starts_k[lo - 1], 0), p.n_k);
+        k1 = min(max(p.starts_k[lo], k0), p.n_k);
     }
-    const unsigned who = __ballot_sync(0xffffffffu, here);
-    const int src = who ? __ffs(who) - 1 : 0;
-    w.q0 = __shfl_sync(0xffffffffu, w.q0, src);
-    w.tokens = __shfl_sync(0xffffffffu, w.tokens, src);
-    w.k0 = __shfl_sync(0xffffffffu, w.k0, src);
-    w.len_k = __shfl_sync(0xffffffffu, w.len_k, src);
-    w.step = __shfl_sync(0xffffffffu, w.step, src);
-    w.first_lim = __shfl_sync(0xffffffffu, w.first_lim, src);
+    w.k0 = k0;
+    w.len_k = k1 - k0;
+    w.step = p.causal ? 1 : 0;
+    w.first_lim = p.causal ? tok + 1 + w.len_k - len_q : w.len_k;
     return w;
 }
 
@@ -264,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             w.tokens = p.n_q - w.q0;
             w.len_k = w.first_lim = p.n_k;
         } else {
-            w = find_work(p, block, lane);
+            w = find_work(p, block, lane, 2 * p.tile_tokens);
         }
         w.split = split;
         if (lane == 0) *s_work = w;

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "attention.cuh"
+#include "attn_short.cuh"
 #include "attn_tile.cuh"
 #include "common.cuh"
 #include "half_types.cuh"
@@ -17,6 +18,12 @@ using attn::kThreads;
 using attn::TileParams;
 
 constexpr int kSms = 148;
+// Prompts go to the small blocks when their mean is at most this many query rows (tokens
+// times group: a tensor-memory block's 256) and keys.  30,000 tokens of one length, us in
+// small blocks / tiles: 32 + 8 heads of 128, 64 tokens (256 rows) 283 / 333, 128 tokens
+// 324 / 292; 12 heads of 64, 200 tokens 113 / 147, 300 tokens 112 / 159, 600 tokens 167 / 154.
+constexpr int kShortMeanRows = 256, kShortMeanKeys = 512;
+
 // Prefix rows in tiles of 8 or 16: up to this many of them, re-reading the prefix for each
 // from L2 is quicker than a tensor-core tile.
 constexpr int kFewRowTiles = 4;
@@ -104,6 +111,29 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
     }
 }
 
+template <class H, int D>
+void launch_short_as(const TileParams& p, long long blocks, cudaStream_t st) {
+    constexpr int smem = attn::short_smem_bytes<D>();
+    static const bool ready = [&] {
+        VGPU_CHECK(cudaFuncSetAttribute(attn::attn_short_kernel<H, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        return true;
+    }();
+    (void)ready;
+    attn::attn_short_kernel<H, D><<<(unsigned)blocks, attn::kShortThreads, smem, st>>>(p);
+    VGPU_LAUNCH("attn_short_kernel");
+}
+
+void launch_short(const TileParams& p, bool f16, long long blocks, cudaStream_t st) {
+    if (blocks > 0x7fffffffLL) throw CudaError("attention: too many tiles for one launch");
+    if (f16) {
+        if (p.dim <= 64) launch_short_as<F16, 64>(p, blocks, st);
+        else launch_short_as<F16, 128>(p, blocks, st);
+    } else {
+        if (p.dim <= 64) launch_short_as<Bf16, 64>(p, blocks, st);
+        else launch_short_as<Bf16, 128>(p, blocks, st);
+    }
+}
+
 // ---------------------------------------------------------------------------------
 // Pages of a cache with few query rows: each request's own pages, and the prefix when the
 // whole batch has few rows.  Bound by reading keys and values once.
@@ -132,19 +162,6 @@ void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 // the next scores are made, the page number after that one block earlier still.
 // ---------------------------------------------------------------------------------
 constexpr int kOwnWarps = 4;
-
-template <class H>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    if (std::is_same<H, Bf16>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
     uint32_t r;
@@ -366,8 +383,8 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
             s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
             for (int i = 0; i < KC; ++i) {
-                mma16816<H>(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qb[nt][2 * i][0], qb[nt][2 * i][1]);
-                mma16816<H>(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
+                attn::mma16816<H>(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qb[nt][2 * i][0], qb[nt][2 * i][1]);
+                attn::mma16816<H>(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
             }
         }
         const bool ends = next.at >= end || next.job != cur.job;
@@ -422,7 +439,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
                 const uint32_t a2 = __byte_perm(word(vf[2][i], e / 2), word(vf[3][i], e / 2), sel);
                 const uint32_t a3 = __byte_perm(word(vf[2][i], e / 2 + 2), word(vf[3][i], e / 2 + 2), sel);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816<H>(o[nt][i][e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) attn::mma16816<H>(o[nt][i][e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
         load_v(next, pg_next);
         if (ends) flush(cur.job);
@@ -576,13 +593,22 @@ int splits_for(long long blocks, long long key_tiles) {
 }
 
 struct PromptPlan {
+    bool small;       // small blocks, see attn_short.cuh
     long long tiles;  // upper bound of block tiles: the requests' lengths are on the device
     int splits;
 };
 PromptPlan prompt_plan(const PromptArgs& a) {
-    const int span = 2 * (kRows / (a.heads / a.kv_heads));
+    const int group = a.heads / a.kv_heads;
     PromptPlan pl;
-    pl.tiles = a.n_q / span + std::min<long long>(a.n_requests + 2, a.n_q);
+    pl.small = group <= attn::kShortRows && a.n_q * group <= (long long)kShortMeanRows * a.n_requests &&
+               a.n_k <= (long long)kShortMeanKeys * a.n_requests;
+    if (pl.small) {
+        pl.tiles = a.n_q / (attn::kShortRows / group) + a.n_requests + 2;
+        pl.splits = 1;
+        return pl;
+    }
+    const int span = 2 * (kRows / group);
+    pl.tiles = a.n_q / span + a.n_requests + 2;
     const long long likely = (a.n_q + span - 1) / span + std::max(a.n_requests - 1, 0);
     pl.splits = splits_for(likely * a.kv_heads, a.n_k / kKeys / std::max(a.n_requests, 1));
     return pl;
@@ -639,9 +665,19 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
     const PromptPlan pl = prompt_plan(a);
     const long long rows = a.n_q * a.heads;
     TileParams p{};
-    fill_queries(p, a.f16, a.q, a.heads, a.kv_heads, a.dim, a.n_q);
+    if (pl.small) {
+        p.heads = a.heads;
+        p.kv_heads = a.kv_heads;
+        p.group = a.heads / a.kv_heads;
+        p.dim = a.dim;
+        p.tile_tokens = attn::kShortRows / p.group;
+        p.n_q = (int)a.n_q;
+        p.q = a.q;
+    } else {
+        fill_queries(p, a.f16, a.q, a.heads, a.kv_heads, a.dim, a.n_q);
+    }
     p.n_k = (int)a.n_k;
-    if (a.n_k) {
+    if (a.n_k && !pl.small) {
         p.mk = make_map(a.f16, a.k.p, {a.dim, a.kv_heads, a.n_k, 1}, {a.k.head, a.k.tok, a.k.tok}, {64, 1, kKeys, 1});
         p.mv = make_map(a.f16, a.v.p, {a.dim, a.kv_heads, a.n_k, 1}, {a.v.head, a.v.tok, a.v.tok}, {64, 1, kKeys, 1});
     }
@@ -658,6 +694,10 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
     p.lse = a.lse;
     p.part_o = static_cast<float*>(a.workspace);
     p.part_lse = p.part_o + pl.splits * rows * a.dim;
+    if (pl.small) {
+        launch_short(p, a.f16, pl.tiles * a.kv_heads, st);
+        return;
+    }
     launch_tiles<false>(p, a.f16, pl.tiles * a.kv_heads * pl.splits, st);
     if (!p.part) return;
     JoinArgs j{};
