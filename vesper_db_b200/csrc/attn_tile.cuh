@@ -7,13 +7,16 @@
 // A tile is 128 rows: floor(128 / group) tokens with the `group` query heads of one key
 // head each, so that one key tile serves the whole group.  A block holds two query tiles
 // and takes the keys 128 at a time:
-//   * warp 8 copies Q, then K and V tiles by TMA into a ring of shared-memory slots;
-//   * warps 9 and 10 issue the products of tile 0 and tile 1: S_t = Q_t K^T (both operands
+//   * warps 0-7 and 8-15 make the probabilities of tile 0 and tile 1, one row of 64 keys a
+//     thread: they read S, exchange the two halves' maxima of a row, keep m and l, and write P
+//     over S as 16-bit values, 32 keys at a time, so that the first products with the values
+//     run while the rest is made.  (With whole rows of 128 keys in four warps a tile, each
+//     scheduler had one warp to hide every latency with: 1,900 cycles from S to P.)
+//   * warp 16 picks what the block works on next, and copies Q, K and V tiles by TMA, K and V
+//     into a ring of shared-memory slots;
+//   * warps 17 and 18 issue the products of tile 0 and tile 1: S_t = Q_t K^T (both operands
 //     from shared memory) and O_t += P_t V (P from tensor memory);
-//   * warps 0-3 and 4-7 hold one row a thread of tile 0 and tile 1: they read S, keep m and
-//     l, and write P over S as 16-bit values, in two halves, so that the first half's
-//     product runs while the second half is made;
-//   * warps 12 to 15 clean the value tiles that hold keys some row must not see.
+//   * warp 19 cleans the value tiles that hold keys some row must not see.
 // The two query tiles are independent of each other: while one is in the tensor cores the
 // other is in the exponentials.  Tensor memory: S0, S1 (128 columns each), O0, O1.
 //
@@ -30,6 +33,9 @@
 // values meet P = 0, and 0 * NaN is NaN: value rows past the last key are zeroed in shared
 // memory, and where a later token of the same prompt holds a non-finite value (checked on
 // the diagonal tiles) the block recomputes its rows one key at a time.
+//
+// A block runs from one piece of work to the next (there is one an SM): the copies of the
+// next one, and its first scores, go on while the results of the last one are written.
 //
 // Every wait is bounded; a block whose wait ran out issues no further work, gives NaN rows
 // and frees its tensor memory.
@@ -49,10 +55,11 @@ namespace attn {
 
 constexpr int kRows = 128;     // query rows of a tile
 constexpr int kKeys = 128;     // keys of a tile
-constexpr int kThreads = 512;  // two softmax warpgroups, two of service warps
+constexpr int kSoftmaxWarps = 16, kThreads = kSoftmaxWarps * 32 + 128;  // and four service warps
 constexpr int kSlots = 4;      // K and V tiles in flight
+constexpr int kAhead = 4;      // pieces of work known ahead
 constexpr float kGrow = 8.0f;  // log2 of how far P may pass 1 before O is rescaled
-constexpr int kSoftmaxRegs = 208, kServiceRegs = 40;  // 256 * 208 + 256 * 40 <= 512 * 128
+constexpr int kSoftmaxRegs = 104, kServiceRegs = 56;  // 512 * 104 + 128 * 56 <= 640 * 96
 
 struct TileParams {
     CUtensorMap mq, mk, mv;
@@ -70,6 +77,8 @@ struct TileParams {
     // Packed keys again, for the rows recomputed one key at a time.
     HeadsView q, k, v;
     float scale_log2;
+    int items;     // pieces of work at most (two query tiles, key head, split)
+    int* counter;  // zero at launch: pieces are taken as blocks come free; null: in turn
     int splits;
     bool part;       // results of each split for a later join, in 32 bits
     void* out;       // otherwise: [n_q, heads, dim]
@@ -80,7 +89,7 @@ struct TileParams {
 
 template <int D>
 constexpr int smem_bytes() {
-    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512;
+    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512 + 2 * 2 * 2 * kRows * 4;
 }
 
 // Bounded wait for the barrier's phase; false when it ran out (a tile takes microseconds).
@@ -106,11 +115,27 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Maximum of three; NaN if one of them is.
+// Maximum of three; NaN is passed over.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// 16 columns of tensor memory, one lane's row a thread.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 
 __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -160,8 +185,34 @@ struct Work {
     int k0, len_k; // first key row, keys of the request
     int first_lim; // keys that the first of these rows sees; each later one sees `step` more
     int step;
-    int split;
+    int kh, split;
+    int stop;      // no more work
 };
+
+// What follows from it: tokens and key tiles of each query tile, [j0, j0 + nt) of the keys'.
+struct Tiles {
+    int tok0, tok1, nt0, nt1, n, j0, per, min_lim;
+    // Tiles that hold keys which some valid row does not see.
+    __device__ __forceinline__ bool guarded(int j) const { return (j0 + j + 1) * kKeys > min_lim; }
+};
+__device__ __forceinline__ Tiles tiles_of(const Work& w, int tt, int splits) {
+    Tiles x;
+    const int all = (w.len_k + kKeys - 1) / kKeys;
+    x.per = (all + splits - 1) / splits;
+    x.j0 = w.split * x.per;
+    auto count = [&](int first, int tok) {
+        const int last = min(w.len_k, w.first_lim + w.step * (first + tok - 1));  // keys its last row sees
+        const int tiles = tok > 0 ? (max(last, 0) + kKeys - 1) / kKeys : 0;
+        return min(max(tiles - x.j0, 0), x.per);
+    };
+    x.tok0 = min(max(w.tokens, 0), tt);
+    x.tok1 = min(max(w.tokens - tt, 0), tt);
+    x.nt0 = count(0, x.tok0);
+    x.nt1 = count(tt, x.tok1);
+    x.n = max(x.nt0, x.nt1);
+    x.min_lim = min(max(w.first_lim, 0), w.len_k);
+    return x;
+}
 
 // Piece `idx` of the packed requests, each cut into `span` tokens.  Run by one whole warp;
 // tokens <= 0: no such piece.  Request b's pieces have the numbers from starts[b] / span + b
@@ -210,6 +261,24 @@ __device__ __forceinline__ bool not_finite(uint4 u) {
     return bad;
 }
 
+// Piece of work number `item`: key heads fastest, then splits.  Run by one whole warp.
+template <bool PAGED>
+__device__ __forceinline__ Work item_work(const TileParams& p, int item, int lane) {
+    Work w{};
+    const int kh = item % p.kv_heads, rest = item / p.kv_heads, split = rest % p.splits, block = rest / p.splits;
+    if (PAGED) {  // every row sees the whole prefix
+        w.q0 = block * 2 * p.tile_tokens;
+        w.tokens = p.n_q - w.q0;
+        w.len_k = w.first_lim = p.n_k;
+    } else {
+        w = find_work(p, block, lane, 2 * p.tile_tokens);
+    }
+    w.kh = kh;
+    w.split = split;
+    w.stop = 0;
+    return w;
+}
+
 template <class H, int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_constant__ TileParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -218,46 +287,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     uint8_t* const smem = smem_raw + (base - raw);
     const uint32_t s_q = base, s_kv = base + 2 * kTileBytes;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + (2 + kSlots) * kTileBytes);
-    uint64_t* const q_full = bars;                // [2]
-    uint64_t* const kv_full = bars + 2;           // [kSlots]
-    uint64_t* const kv_empty = kv_full + kSlots;  // [kSlots]
-    uint64_t* const s_full = kv_empty + kSlots;   // [2]
-    uint64_t* const p_full = s_full + 2;          // [2][2]: tile, half of the keys
-    uint64_t* const turn = p_full + 4;            // [2]
-    uint64_t* const o_full = turn + 2;            // [2]
-    uint64_t* const drained = o_full + 2;         // [2]
-    uint64_t* const clean = drained + 2;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(clean + 1);
-    int* const s_leak = reinterpret_cast<int*>(tmem_slot + 1);
-    Work* const s_work = reinterpret_cast<Work*>(tmem_slot + 2);
+    uint64_t* const q_full = bars;                   // [2]
+    uint64_t* const q_empty = q_full + 2;            // [2]
+    uint64_t* const kv_full = q_empty + 2;           // [kSlots]
+    uint64_t* const kv_empty = kv_full + kSlots;     // [kSlots]
+    uint64_t* const s_full = kv_empty + kSlots;      // [2]
+    uint64_t* const p_full = s_full + 2;             // [2][2]: tile, part of the keys
+    uint64_t* const o_full = p_full + 4;             // [2]
+    uint64_t* const turn = o_full + 2;               // [2]
+    uint64_t* const drained = turn + 2;              // [2]
+    uint64_t* const landed = drained + 2;
+    uint64_t* const clean = landed + 1;
+    uint64_t* const work_full = clean + 1;           // [kAhead]
+    uint64_t* const work_empty = work_full + kAhead; // [kAhead]
+    Work* const s_work = reinterpret_cast<Work*>(work_empty + kAhead);  // [kAhead]
+    int* const s_leak = reinterpret_cast<int*>(s_work + kAhead);        // [kAhead]
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(s_leak + kAhead);
+    // Rows' maxima (and sums) of each half of the keys: [turn][tile][half][row]
+    float* const s_half = reinterpret_cast<float*>(bars + 64);
+    static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + kAhead * (sizeof(Work) + 4) + 4 <= 512, "");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // The own pages' kernel may be queued behind this one and does not depend on it.
     if (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    int block = blockIdx.x;
-    const int kh = block % p.kv_heads;
-    block /= p.kv_heads;
-    const int split = block % p.splits;
-    block /= p.splits;
 
-    if (warp == 0) {
-        Work w{};
-        if (PAGED) {  // every row sees the whole prefix
-            w.q0 = block * 2 * p.tile_tokens;
-            w.tokens = p.n_q - w.q0;
-            w.len_k = w.first_lim = p.n_k;
-        } else {
-            w = find_work(p, block, lane, 2 * p.tile_tokens);
-        }
-        w.split = split;
-        if (lane == 0) *s_work = w;
-    } else if (warp == 9) {
+    if (warp == 17) {
         if (lane == 0) {
             for (int i = 0; i < 2; ++i) {
                 tc::mbar_init(&q_full[i], 1);
+                tc::mbar_init(&q_empty[i], 1);
                 tc::mbar_init(&s_full[i], 1);
-                tc::mbar_init(&p_full[2 * i], 128);
-                tc::mbar_init(&p_full[2 * i + 1], 128);
+                tc::mbar_init(&p_full[2 * i], 256);
+                tc::mbar_init(&p_full[2 * i + 1], 256);
                 tc::mbar_init(&turn[i], 1);
                 tc::mbar_init(&o_full[i], 1);
                 tc::mbar_init(&drained[i], 1);
@@ -266,8 +327,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 tc::mbar_init(&kv_full[i], 1);
                 tc::mbar_init(&kv_empty[i], 2);  // both warps of products
             }
-            tc::mbar_init(clean, 4);
-            *s_leak = 0;
+            for (int i = 0; i < kAhead; ++i) {
+                tc::mbar_init(&work_full[i], 1);
+                tc::mbar_init(&work_empty[i], kSoftmaxWarps + 3);  // all warps but the one that fills it
+            }
+            tc::mbar_init(landed, 2);
+            tc::mbar_init(clean, 1);
             tc::mbar_init_fence();
         }
         __syncwarp();
@@ -280,52 +345,78 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    const Work w = *s_work;
-
-    // Key tiles of each query tile in this split: [j0, j0 + n_t).
     const int tt = p.tile_tokens;
-    int tok[2], nt[2];  // indexed by constants only: they stay in registers
-    const int all = (w.len_k + kKeys - 1) / kKeys, per = (all + p.splits - 1) / p.splits, j0 = w.split * per;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        tok[t] = min(max(w.tokens - t * tt, 0), tt);
-        const int last = min(w.len_k, w.first_lim + w.step * (t * tt + tok[t] - 1));  // keys its last row sees
-        const int tiles = tok[t] > 0 ? (max(last, 0) + kKeys - 1) / kKeys : 0;
-        nt[t] = min(max(tiles - j0, 0), per);
-    }
-    const int n = max(nt[0], nt[1]);
-    // From this key on some valid row of the block does not see the keys.
-    const int min_lim = min(max(w.first_lim, 0), w.len_k);
-    auto guarded_tile = [&](int j) { return (j0 + j + 1) * kKeys > min_lim; };
 
-    if (warp >= 8) {
+    bool ok = true;  // sticky: after a wait that ran out a warp waits no more
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(b, parity)) != 0;
+        return ok;
+    };
+    // The piece of work number `it` of the block; false when a wait ran out.  `done` hands its
+    // place back; whoever reads the leak flag does that at the end.
+    auto work_done = [&](uint32_t it) {
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&work_empty[it % kAhead]);
+    };
+    auto next_work = [&](Work& w, uint32_t it) {
+        if (!wait(&work_full[it % kAhead], (it / kAhead) & 1)) return false;
+        w = s_work[it % kAhead];
+        return true;
+    };
+
+    if (warp >= kSoftmaxWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
-        if (warp == 8) {
-            // ---------------------------------------------------------------- copies
-            if (n > 0) {
+        if (warp == 16) {
+            // ---------------------------------------------------------------- work and copies
+            uint32_t it = 0, kv = 0, qn0 = 0, qn1 = 0;
+            auto load_q = [&](const Work& w, int t, uint32_t& qn) {
+                if (qn > 0 && !wait(&q_empty[t], (qn - 1) & 1)) return;
+                ++qn;
                 if (lane == 0) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (nt[t] == 0) continue;
-                        const uint32_t rows = (uint32_t)(tt * p.group);
-                        tc::mbar_expect_tx(&q_full[t], rows * 128 * kHalves);
-                        for (int h = 0; h < kHalves; ++h)
-                            tma4(s_q + t * kTileBytes + h * kHalfBytes, &p.mq, h * 64, 0, kh, w.q0 + t * tt, &q_full[t]);
+                    tc::mbar_expect_tx(&q_full[t], (uint32_t)(tt * p.group) * 128 * kHalves);
+                    for (int h = 0; h < kHalves; ++h)
+                        tma4(s_q + t * kTileBytes + h * kHalfBytes, &p.mq, h * 64, 0, w.kh, w.q0 + t * tt, &q_full[t]);
+                }
+            };
+            int item = blockIdx.x;
+            while (ok) {
+                Work w{};
+                w.stop = 1;
+                // pieces that turn out to be empty are passed over
+                while (item < p.items) {
+                    w = item_work<PAGED>(p, item, lane);
+                    if (w.tokens > 0) break;
+                    w.stop = 1;
+                    if (p.counter) {
+                        if (lane == 0) item = gridDim.x + atomicAdd(p.counter, 1);
+                        item = __shfl_sync(0xffffffffu, item, 0);
+                    } else {
+                        item += gridDim.x;
                     }
                 }
-                bool ok = true;
-                int i = 0;
-                for (; i < 2 * n; ++i) {  // K, V, K, V, ...
-                    const int slot = i % kSlots, round = i / kSlots, key = (j0 + (i >> 1)) * kKeys;
-                    if (round > 0) ok = mbar_wait(&kv_empty[slot], (round - 1) & 1);
-                    if (!ok) break;
+                const int r = it % kAhead;
+                if (it >= kAhead && !wait(&work_empty[r], (it / kAhead - 1) & 1)) break;
+                if (lane == 0) {
+                    s_work[r] = w;
+                    s_leak[r] = 0;
+                    tc::mbar_arrive(&work_full[r]);
+                }
+                __syncwarp();
+                ++it;
+                if (w.stop) break;
+                int after = item + gridDim.x;
+                if (p.counter && lane == 0) after = gridDim.x + atomicAdd(p.counter, 1);
+                const Tiles x = tiles_of(w, tt, p.splits);
+                for (int i = 0; i < 2 * x.n; ++i, ++kv) {  // K, V, K, V, ...
+                    const int slot = kv % kSlots, round = kv / kSlots, key = (x.j0 + (i >> 1)) * kKeys;
+                    if (round > 0 && !wait(&kv_empty[slot], (round - 1) & 1)) break;
                     const CUtensorMap* map = (i & 1) ? &p.mv : &p.mk;
                     const uint32_t dst = s_kv + slot * kTileBytes;
                     if (!PAGED) {
                         if (lane == 0) {
                             tc::mbar_expect_tx(&kv_full[slot], kTileBytes);
                             for (int h = 0; h < kHalves; ++h)
-                                tma4(dst + h * kHalfBytes, map, h * 64, kh, w.k0 + key, 0, &kv_full[slot]);
+                                tma4(dst + h * kHalfBytes, map, h * 64, w.kh, w.k0 + key, 0, &kv_full[slot]);
                         }
                     } else {
                         const int page = 1 << p.page_shift, box = min(page, kKeys);
@@ -335,29 +426,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         if (lane < boxes) {
                             const int at = key + lane * box, pg = p.pages[at >> p.page_shift];
                             for (int h = 0; h < kHalves; ++h)
-                                tma4(dst + h * kHalfBytes + lane * box * 128, map, h * 64, kh, at & (page - 1), pg,
+                                tma4(dst + h * kHalfBytes + lane * box * 128, map, h * 64, w.kh, at & (page - 1), pg,
                                      &kv_full[slot]);
                         }
                         __syncwarp();
                     }
+                    if (i == 0) {
+                        if (x.nt0 > 0) load_q(w, 0, qn0);
+                        if (x.nt1 > 0) load_q(w, 1, qn1);
+                    }
                 }
-                if (!ok)  // nothing may land after the block has gone
-                    for (int e = max(i - kSlots, 0); e < i; ++e) mbar_wait(&kv_full[e % kSlots], (e / kSlots) & 1);
+                item = __shfl_sync(0xffffffffu, after, 0);
             }
-        } else if (warp == 9 || warp == 10) {
+            // Nothing may land, or arrive, after the block has gone.
+            const bool sound = ok;
+            ok = true;
+            for (uint32_t e = kv > kSlots ? kv - kSlots : 0; e < kv; ++e) {
+                wait(&kv_full[e % kSlots], (e / kSlots) & 1);
+                if (sound) wait(&kv_empty[e % kSlots], (e / kSlots) & 1);
+            }
+            if (sound && qn0 > 0) wait(&q_empty[0], (qn0 - 1) & 1);
+            if (sound && qn1 > 0) wait(&q_empty[1], (qn1 - 1) & 1);
+        } else if (warp == 17 || warp == 18) {
             // ---------------------------------------------------------------- products of tile t
             constexpr uint32_t fmt = std::is_same<H, Bf16>::value ? 1u : 0u;
             constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t id_s = common | ((uint32_t)(kKeys >> 3) << 17);
             constexpr uint32_t id_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-            const int t = warp - 9, mine = t ? nt[1] : nt[0];
+            const int t = warp - 17;
             const uint32_t t_s = tmem + t * 128, t_o = tmem + 256 + t * 128;
             const uint64_t q_desc = tc::sw128_kmajor_desc(s_q + t * kTileBytes);
-            bool ok = true;
-            auto wait = [&](uint64_t* b, uint32_t parity) {
-                if (ok) ok = mbar_wait(b, parity);
-                return ok;
-            };
             auto scores = [&](int slot) {
                 const uint64_t b = tc::sw128_kmajor_desc(s_kv + slot * kTileBytes);
 #pragma unroll
@@ -367,100 +465,141 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
                 commit(&s_full[t]);
             };
-            // Hands the slot of item i back to the copies, unless they are done with it: an
-            // arrival that nobody waits for could come after the block has gone.
-            auto release = [&](int i) {
-                if (ok && i + kSlots < 2 * n) commit(&kv_empty[i % kSlots]);
-            };
-            // A warp without rows of its own follows the same waits: it hands a slot back only
-            // after what the slot holds has landed.
-            if (mine > 0) wait(&q_full[t], 0);
-            if (n > 0 && wait(&kv_full[0], 0) && mine > 0) {
-                tc::fence_after_sync();
-                scores(0);
-            }
-            release(0);
-            // The two warps take turns, one product of values and the next of scores each: left
-            // to themselves the tiles fall into step, both in the exponentials and then both in
-            // the tensor cores, and half the time of each is lost.
-            int cleaned = 0;
-            for (int j = 0; j < n; ++j) {
-                const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % kSlots, sk = ik % kSlots;
-                wait(&kv_full[sv], (iv / kSlots) & 1);
-                if (guarded_tile(j)) {
-                    asm volatile("bar.arrive 1, 192;" ::: "memory");
-                    wait(clean, cleaned++ & 1);
+            // Counts over all pieces of work: items of the ring, turns, tiles, Q tiles, cleanings.
+            uint32_t kv = 0, turns = 0, tiles = 0, qn = 0, cleaned = 0;
+            Work w;
+            for (uint32_t it = 0; next_work(w, it); ++it) {
+                work_done(it);
+                if (w.stop) break;
+                const Tiles x = tiles_of(w, tt, p.splits);
+                const int n = x.n, mine = t ? x.nt1 : x.nt0;
+                if (n == 0) continue;
+                auto slot_of = [&](int i) { return (int)((kv + i) % kSlots); };
+                auto arrived = [&](int i) { return wait(&kv_full[slot_of(i)], ((kv + i) / kSlots) & 1); };
+                auto release = [&](int i) {
+                    if (ok) commit(&kv_empty[slot_of(i)]);
+                };
+                // A warp without rows of its own follows the same waits: it hands a slot back only
+                // after what the slot holds has landed.
+                if (mine > 0) wait(&q_full[t], qn++ & 1);
+                if (arrived(0) && mine > 0) {
+                    tc::fence_after_sync();
+                    scores(slot_of(0));
+                    if (mine == 1) commit(&q_empty[t]);
                 }
-                if (t == 1 || j > 0) wait(&turn[t], t == 1 ? j & 1 : (j - 1) & 1);
-                if (j < mine) {
-                    const uint64_t b = values_desc(s_kv + sv * kTileBytes, kHalfBytes);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {  // halves of P
-                        if (!wait(&p_full[2 * t + h], j & 1)) break;
-                        tc::fence_after_sync();
-#pragma unroll
-                        for (int k = h * 4; k < h * 4 + 4; ++k)
-                            mma_ts(t_o, t_s + k * 8, b + k * (2048 >> 4), id_o, (j > 0 || k > 0) ? 1u : 0u);
+                release(0);
+                // The two warps take turns, one product of values and the next of scores each:
+                // left to themselves the tiles fall into step, both in the exponentials and then
+                // both in the tensor cores, and half the time of each is lost.
+                for (int j = 0; j < n && ok; ++j, ++turns) {
+                    const int iv = 2 * j + 1, ik = 2 * j + 2;
+                    arrived(iv);
+                    if (x.guarded(j)) {
+                        if (lane == 0) tc::mbar_arrive(landed);
+                        wait(clean, cleaned++ & 1);
                     }
-                    if (ok && j + 1 == mine) commit(&o_full[t]);
+                    if (j + 1 < n) arrived(ik);
+                    if (t == 1 || turns > 0) wait(&turn[t], t == 1 ? turns & 1 : (turns - 1) & 1);
+                    if (j < mine) {
+                        const uint64_t b = values_desc(s_kv + slot_of(iv) * kTileBytes, kHalfBytes);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {  // keys 0-31 and 64-95, then the others
+                            if (!wait(&p_full[2 * t + h], tiles & 1)) break;
+                            tc::fence_after_sync();
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int k = 2 * h + (e & 1) + (e >> 1) * 4;
+                                mma_ts(t_o, t_s + k * 8, b + k * (2048 >> 4), id_o, (j > 0 || h > 0 || e > 0) ? 1u : 0u);
+                            }
+                        }
+                        ++tiles;
+                        if (ok && j + 1 == mine) commit(&o_full[t]);
+                    }
+                    if (ok && j + 1 < mine) {
+                        scores(slot_of(ik));
+                        if (j + 2 == mine) commit(&q_empty[t]);
+                    }
+                    if (lane == 0) tc::mbar_arrive(&turn[t ^ 1]);
+                    release(iv);
+                    if (j + 1 < n) release(ik);
                 }
-                if (j + 1 < n && wait(&kv_full[sk], (ik / kSlots) & 1) && j + 1 < mine) scores(sk);
-                if (lane == 0) tc::mbar_arrive(&turn[t ^ 1]);
-                release(iv);
-                if (j + 1 < n) release(ik);
+                kv += 2 * n;
             }
             if (!ok) {
                 commit(&drained[t]);
                 mbar_wait(&drained[t], 0);
             }
-        } else if (warp >= 12) {
+        } else {
             // ---------------------------------------------------------------- value rows that not every row sees
-            const int g = tid - 384;
-            for (int j = 0; j < n; ++j) {
-                if (!guarded_tile(j)) continue;
-                asm volatile("bar.sync 1, 192;" ::: "memory");  // both warps of products have seen the tile land
-                uint8_t* const v = smem + (2 + (2 * j + 1) % kSlots) * kTileBytes;
-                const int key = (j0 + j) * kKeys;
-                const int end = min(max(w.len_k - key, 0), kKeys), from = max(min_lim - key, 0);
-                bool bad = false;
-                if (!PAGED)
-                    for (int i = g; i < (end - from) * 8; i += 128)
+            uint32_t kv = 0, seen = 0;
+            Work w;
+            for (uint32_t it = 0; next_work(w, it); ++it) {
+                work_done(it);
+                if (w.stop) break;
+                const Tiles x = tiles_of(w, tt, p.splits);
+                for (int j = 0; j < x.n; ++j) {
+                    if (!x.guarded(j)) continue;
+                    if (!wait(landed, seen++ & 1)) break;  // both warps of products have seen the tile land
+                    uint8_t* const v = smem + (2 + (kv + 2 * j + 1) % kSlots) * kTileBytes;
+                    const int key = (x.j0 + j) * kKeys;
+                    const int end = min(max(w.len_k - key, 0), kKeys), from = max(x.min_lim - key, 0);
+                    bool bad = false;
+                    if (!PAGED)
+                        for (int i = lane; i < (end - from) * 8; i += 32)
+                            for (int h = 0; h < kHalves; ++h)
+                                bad |= not_finite<H>(*reinterpret_cast<const uint4*>(v + h * kHalfBytes + from * 128 + i * 16));
+                    for (int i = lane; i < (kKeys - end) * 8; i += 32)
                         for (int h = 0; h < kHalves; ++h)
-                            bad |= not_finite<H>(*reinterpret_cast<const uint4*>(v + h * kHalfBytes + from * 128 + i * 16));
-                for (int i = g; i < (kKeys - end) * 8; i += 128)
-                    for (int h = 0; h < kHalves; ++h)
-                        *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-                if (bad) *s_leak = 1;
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(clean);
+                            *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    if (bad) s_leak[it % kAhead] = 1;
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(clean);
+                }
+                kv += 2 * x.n;
             }
         }
     } else {
-        // -------------------------------------------------------------------- softmax: one row a thread
+        // -------------------------------------------------------------------- softmax: 64 keys of a row a thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const int t = warp >> 2, row = tid & 127;
+        const int t = warp >> 3, half = (warp >> 2) & 1, row = tid & 127;
         const int row_tok = row / p.group, row_head = row - row_tok * p.group;
-        const int my_tiles = t ? nt[1] : nt[0];
-        const bool valid = row_tok < (t ? tok[1] : tok[0]);
-        const int lim = valid ? min(max(w.first_lim + w.step * (t * tt + row_tok), 0), w.len_k) : w.len_k;
-        const int tile_lim = min(max(w.first_lim + w.step * t * tt, 0), w.len_k);  // the tile's first row's
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + t * 128 + lane_base, to = tmem + 256 + t * 128 + lane_base;
-        float m = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < my_tiles && ok; ++j) {
-            ok = mbar_wait(&s_full[t], j & 1);
-            if (!ok) break;
+        const uint32_t ts = tmem + t * 128 + lane_base, to = tmem + 256 + t * 128 + half * (D / 2) + lane_base;
+        // The two warps of a row meet: each gives a value and gets the other's.
+        uint32_t meetings = 0;
+        auto exchange = [&](float x) {
+            float* const ex = s_half + (meetings++ & 1) * 512 + t * 256;
+            ex[half * 128 + row] = x;
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + t * 4 + (warp & 3)) : "memory");
+            return ex[(half ^ 1) * 128 + row];
+        };
+        uint32_t tiles = 0, outs = 0;  // over all pieces of work
+        Work w;
+        uint32_t it = 0;
+        while (true) {
+            // Both warps of a row stop together, or one would wait for the other for good.
+            next_work(w, it);
+            if (exchange(ok ? 0.0f : 1.0f) != 0.0f) ok = false;
+            if (!ok || w.stop) break;
+            const Tiles x = tiles_of(w, tt, p.splits);
+            const int my_tiles = t ? x.nt1 : x.nt0, j0 = x.j0, per = x.per;
+            const bool valid = row_tok < (t ? x.tok1 : x.tok0);
+            const int lim = valid ? min(max(w.first_lim + w.step * (t * tt + row_tok), 0), w.len_k) : w.len_k;
+            const int tile_lim = min(max(w.first_lim + w.step * t * tt, 0), w.len_k);  // the tile's first row's
+            float m = -INFINITY, l = 0.0f;
+        for (int j = 0; j < my_tiles; ++j) {
+            // after a wait that ran out the row's warps only keep meeting
+            wait(&s_full[t], tiles++ & 1);
             tc::fence_after_sync();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::tmem_ld32(ts + c * 32, s[c]);
+            uint32_t s[2][32];
+            tc::tmem_ld32(ts + half * 64, s[0]);
+            tc::tmem_ld32(ts + half * 64 + 32, s[1]);
             tc::tmem_ld_wait();
-            const int key = (j0 + j) * kKeys;
-            if (key + kKeys > tile_lim) {
+            const int key = (j0 + j) * kKeys + half * 64;
+            if (key + 64 > tile_lim) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (key + c * 32 + i >= lim) s[c][i] = 0xff800000u;  // -inf
@@ -468,17 +607,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             float mx[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                auto f = [&](int i) { return __uint_as_float(s[c][i]); };
+                auto f = [&](int i) { return __uint_as_float(s[c >> 1][(c & 1) * 16 + i]); };
                 mx[c] = max3(f(0), f(1), f(2));
 #pragma unroll
-                for (int i = 3; i < 31; i += 2) mx[c] = max3(mx[c], f(i), f(i + 1));
-                mx[c] = max3(mx[c], mx[c], f(31));
+                for (int i = 3; i < 15; i += 2) mx[c] = max3(mx[c], f(i), f(i + 1));
+                mx[c] = max3(mx[c], f(15), f(15));
             }
-            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
+            float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            // also: both halves of S are in registers after this, and P may take their place
+            top = fmaxf(top, exchange(top)) * p.scale_log2;
             if (j == 0) {
                 m = top == INFINITY ? __int_as_float(0x7fc00000) : top;
             } else if (__any_sync(0xffffffffu, !(top - m <= kGrow))) {
-                // Grown too far, or NaN (a score is NaN or infinite, or the row has seen no key)
+                // Grown too far, or NaN (a score is NaN or infinite, or the row has seen no key).
+                // Each of the two warps sees the same values, and rescales half of O.
                 float up = !(top - m <= kGrow) ? top : m;
                 if (up == INFINITY) up = __int_as_float(0x7fc00000);
                 const float f = m == up ? 1.0f : ex2(m - up);
@@ -486,72 +628,78 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 l *= f;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(to + c * 32, o);
+                    uint32_t o[16];
+                    tmem_ld16(to + c * 16, o);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tc::tmem_st32(to + c * 32, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st16(to + c * 16, o);
                 }
             }
             const float ref = m == -INFINITY ? 0.0f : m;
             const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
             uint64_t ref2 = pair(-ref, -ref);
-            uint64_t sum[4] = {0, 0, 0, 0};
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {  // halves of 64 keys
-                uint32_t pk[32];
+            for (int c = 0; c < 2; ++c) {
+                uint32_t pk[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint32_t* e = &s[c + i / 16][(2 * i) & 31];
-                    const float2 x = halves(fma2(pair(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, ref2));
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x =
+                        halves(fma2(pair(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, ref2));
                     const float a = ex2(x.x), b = ex2(x.y);
-                    sum[i & 3] = add2(sum[i & 3], pair(a, b));
+                    sum[i & 1] = add2(sum[i & 1], pair(a, b));
                     pk[i] = H::pack(a, b);
                 }
-                tc::tmem_st32(ts + c * 16, pk);
+                tmem_st16(ts + half * 32 + c * 16, pk);
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
-                tc::mbar_arrive(&p_full[2 * t + c / 2]);
-                // the second half's exponentials stay behind this arrival
+                tc::mbar_arrive(&p_full[2 * t + c]);
+                // the second part's exponentials stay behind this arrival
                 asm volatile("" : "+l"(ref2));
             }
-            const float2 s01 = halves(add2(sum[0], sum[1])), s23 = halves(add2(sum[2], sum[3]));
-            l += (s01.x + s01.y) + (s23.x + s23.y);
+            const float2 both = halves(add2(sum[0], sum[1]));
+            l += both.x + both.y;
         }
-        if (ok && my_tiles > 0) ok = mbar_wait(&o_full[t], 0);
+        if (my_tiles > 0) {
+            wait(&o_full[t], outs++ & 1);
+            const float other = exchange(ok ? l : __int_as_float(0x7fc00000));
+            // one order of the two, so that both warps hold the same sum
+            l = half ? other + l : l + other;
+            if (!ok) l = __int_as_float(0x7fc00000);
+        }
         tc::fence_after_sync();
         // ---- results
-        const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + kh * p.group + row_head);
-        const bool leak = !PAGED && my_tiles > 0 && *reinterpret_cast<volatile int*>(s_leak) != 0;
+        const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + w.kh * p.group + row_head);
+        const bool leak = !PAGED && my_tiles > 0 && ok && *reinterpret_cast<volatile int*>(&s_leak[it % kAhead]) != 0;
         const bool part = p.part;
         const long long rows = (long long)p.n_q * p.heads;
-        float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        if (!ok) inv = __int_as_float(0x7fc00000);
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
         using T = typename H::type;
         if (!leak) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
+                uint32_t o[16];
                 if (my_tiles > 0) {
-                    tc::tmem_ld32(to + c * 32, o);
+                    tmem_ld16(to + c * 16, o);
                     tc::tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                    for (int i = 0; i < 16; ++i) o[i] = 0;
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (!valid || c * 32 + i >= p.dim) continue;
+                for (int i = 0; i < 16; i += 8) {
+                    const int d = half * (D / 2) + c * 16 + i;
+                    if (!valid || d >= p.dim) continue;
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f && ok ? 0.0f : __uint_as_float(o[i + e]) * inv;
+                    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : __uint_as_float(o[i + e]) * inv;
                     if (part) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + (split * rows + at) * p.dim + c * 32 + i);
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + at) * p.dim + d);
                         dst[0] = make_float4(x[0], x[1], x[2], x[3]);
                         dst[1] = make_float4(x[4], x[5], x[6], x[7]);
                     } else {
-                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + c * 32 + i) = pack8<H>(x);
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + d) = pack8<H>(x);
                     }
                 }
                 __syncwarp();
@@ -559,13 +707,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         } else if (valid) {
             // One key at a time, eight output values a pass, with the maximum and sum that the
             // scores gave: only where an unseen value row is not finite.
-            const T* q = static_cast<const T*>(p.q.p) + (w.q0 + t * tt + row_tok) * p.q.tok + (kh * p.group + row_head) * p.q.head;
-            const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + kh * p.k.head;
-            const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + kh * p.v.head;
+            const T* q = static_cast<const T*>(p.q.p) + (w.q0 + t * tt + row_tok) * p.q.tok + (w.kh * p.group + row_head) * p.q.head;
+            const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + w.kh * p.k.head;
+            const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + w.kh * p.v.head;
             const int from = j0 * kKeys, to_key = min(lim, (j0 + per) * kKeys);
             const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
-            for (int c = 0; c < p.dim; c += 8) {
+            for (int c = half * 8; c < p.dim; c += 16) {
                 float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
                 for (int key = from; key < to_key; ++key) {
@@ -587,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[i] *= inv;
                 if (part) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + (split * rows + at) * p.dim + c);
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + at) * p.dim + c);
                     dst[0] = make_float4(o[0], o[1], o[2], o[3]);
                     dst[1] = make_float4(o[4], o[5], o[6], o[7]);
                 } else {
@@ -595,15 +743,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
             }
         }
-        if (valid) {
-            const float lse2 = ok ? m + log2f(l) : __int_as_float(0x7fc00000);
-            if (part) p.part_lse[split * rows + at] = lse2;
+        if (valid && half == 0) {
+            const float lse2 = m + log2f(l);
+            if (part) p.part_lse[w.split * rows + at] = lse2;
             else if (p.lse) p.lse[at] = lse2 * 0.6931471805599453f;
         }
+        // the next piece's first P, and with it the first product into O, comes after these reads
         tc::fence_before_sync();
+        work_done(it++);
+        }
+        // A wait ran out: this block's other rows are NaN too.
+        if (!ok) {
+            for (int item = blockIdx.x; item < p.items && half == 0; item += gridDim.x) {
+                if (p.counter) break;
+                const Work v = item_work<PAGED>(p, item, lane);
+                if (row_tok >= min(max(v.tokens - t * tt, 0), tt)) continue;
+                const long long at = (long long)(v.q0 + t * tt + row_tok) * p.heads + v.kh * p.group + row_head;
+                for (int d = 0; d < p.dim && !p.part; ++d) static_cast<uint16_t*>(p.out)[at * p.dim + d] = 0x7fff;
+                if (p.part) p.part_lse[v.split * (long long)p.n_q * p.heads + at] = __int_as_float(0x7fc00000);
+            }
+        }
     }
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc::fence_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }

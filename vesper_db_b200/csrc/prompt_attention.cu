@@ -81,7 +81,7 @@ void fill_queries(TileParams& p, bool f16, const HeadsView& q, int heads, int kv
 }
 
 template <class H, int D, bool PAGED>
-void launch_tiles_as(const TileParams& p, long long blocks, cudaStream_t st) {
+void launch_tiles_as(const TileParams& p, unsigned blocks, cudaStream_t st) {
     auto* kernel = attn::attn_tile_kernel<H, D, PAGED>;
     constexpr int smem = attn::smem_bytes<D>();
     static const bool ready = [&] {
@@ -89,19 +89,29 @@ void launch_tiles_as(const TileParams& p, long long blocks, cudaStream_t st) {
         cudaFuncAttributes fa;
         VGPU_CHECK(cudaFuncGetAttributes(&fa, kernel));
         // the softmax warps' registers come out of what the block is launched with
-        if (fa.numRegs * kThreads < 256 * (attn::kSoftmaxRegs + attn::kServiceRegs))
+        if (fa.numRegs * kThreads < attn::kSoftmaxWarps * 32 * attn::kSoftmaxRegs + 128 * attn::kServiceRegs)
             throw CudaError("attn_tile_kernel: launched with too few registers for its split");
         return true;
     }();
     (void)ready;
-    kernel<<<(unsigned)blocks, kThreads, smem, st>>>(p);
+    kernel<<<blocks, kThreads, smem, st>>>(p);
     VGPU_LAUNCH("attn_tile_kernel");
 }
 
+// Pieces of work are handed out by a counter when every block gets several: their lengths
+// differ, and are known on the device only.
+bool counted(long long items) { return items > 2 * kSms; }
+
 template <bool PAGED>
-void launch_tiles(const TileParams& p, bool f16, long long blocks, cudaStream_t st) {
-    if (blocks <= 0) return;
-    if (blocks > 0x7fffffffLL) throw CudaError("attention: too many tiles for one launch");
+void launch_tiles(TileParams p, bool f16, long long items, int* counter, cudaStream_t st) {
+    if (items <= 0) return;
+    if (items > 0x7fffffffLL - kSms) throw CudaError("attention: too many tiles for one launch");
+    p.items = (int)items;
+    if (counted(items)) {
+        p.counter = counter;
+        VGPU_CHECK(cudaMemsetAsync(counter, 0, sizeof(int), st));
+    }
+    const unsigned blocks = (unsigned)std::min<long long>(items, kSms);
     if (f16) {
         if (p.dim <= 64) launch_tiles_as<F16, 64, PAGED>(p, blocks, st);
         else launch_tiles_as<F16, 128, PAGED>(p, blocks, st);
@@ -592,6 +602,8 @@ int splits_for(long long blocks, long long key_tiles) {
     return (int)std::max<long long>(1, std::min<long long>({by_sms, by_keys, 64}));
 }
 
+constexpr size_t kCounterBytes = 16;
+
 struct PromptPlan {
     bool small;       // small blocks, see attn_short.cuh
     long long tiles;  // upper bound of block tiles: the requests' lengths are on the device
@@ -649,7 +661,7 @@ SharedPlan shared_plan(const SharedArgs& a) {
     p.tile_lse_at = p.slots_at + slot_rows * a.dim;
     p.slot_lse_at = p.tile_lse_at + (size_t)p.splits * rows;
     p.where_at = (p.slot_lse_at + slot_rows + 1) / 2 * 2;
-    p.bytes = (p.where_at + 2 * (size_t)jobs) * sizeof(float);
+    p.bytes = kCounterBytes + (p.where_at + 2 * (size_t)jobs) * sizeof(float);
     return p;
 }
 
@@ -658,7 +670,9 @@ SharedPlan shared_plan(const SharedArgs& a) {
 size_t prompt_attention_workspace(const PromptArgs& a) {
     if (a.n_q == 0) return 0;
     const PromptPlan pl = prompt_plan(a);
-    return pl.splits > 1 ? part_bytes(pl.splits, a.n_q * a.heads, a.dim) : 0;
+    // the counter of pieces comes first
+    return pl.splits > 1 ? kCounterBytes + part_bytes(pl.splits, a.n_q * a.heads, a.dim)
+                         : (!pl.small && counted(pl.tiles * a.kv_heads) ? kCounterBytes : 0);
 }
 
 void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
@@ -692,13 +706,13 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
     p.part = pl.splits > 1;
     p.out = a.out;
     p.lse = a.lse;
-    p.part_o = static_cast<float*>(a.workspace);
+    p.part_o = static_cast<float*>(a.workspace) + kCounterBytes / sizeof(float);
     p.part_lse = p.part_o + pl.splits * rows * a.dim;
     if (pl.small) {
         launch_short(p, a.f16, pl.tiles * a.kv_heads, st);
         return;
     }
-    launch_tiles<false>(p, a.f16, pl.tiles * a.kv_heads * pl.splits, st);
+    launch_tiles<false>(p, a.f16, pl.tiles * a.kv_heads * pl.splits, static_cast<int*>(a.workspace), st);
     if (!p.part) return;
     JoinArgs j{};
     j.rows = rows;
@@ -718,7 +732,7 @@ size_t shared_attention_workspace(const SharedArgs& a) { return a.n_requests == 
 void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
     SharedPlan sp = shared_plan(a);
     const long long rows = (long long)a.n_requests * a.heads;
-    float* const base = static_cast<float*>(a.workspace);
+    float* const base = static_cast<float*>(a.workspace) + kCounterBytes / sizeof(float);
     JoinArgs j{};
     j.rows = rows;
     j.heads = a.heads;
@@ -742,7 +756,8 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
         p.part = true;
         p.part_o = base;
         p.part_lse = base + sp.tile_lse_at;
-        launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * p.splits, st);
+        launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * p.splits,
+                           static_cast<int*>(a.workspace), st);
     }
     sp.pages.o = base + sp.slots_at;
     sp.pages.lse = base + sp.slot_lse_at;
