@@ -11,25 +11,39 @@ paged cache [pages, page_size, kv_heads, head_dim]:
 All take torch tensors on one CUDA device, queue their work on that device's current stream through the vesper_*_device
 entry points of libvesper_c.so, synchronise nothing and can be captured in a CUDA graph.  Outputs and workspaces come
 from torch's allocator in that stream's order.  Arguments that do not fit raise VesperError before any work is queued.
+The checks and the calls are native (csrc/attention_torch.cpp, built to _attention.so beside the library).
 """
 from __future__ import annotations
 
-import functools
 import struct
 from typing import NamedTuple
 
 import torch
 
 from . import _native as N
-from .index import VesperError, _check
+from .index import _check
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+try:
+    from . import _attention as _ops
+except ImportError as e:
+    raise RuntimeError("vesper_db_b200/_attention.so is missing or does not load: build it with "
+                       f"`python -m vesper_db_b200.build` ({e})") from e
 
-# The params structs of include/vesper_b200.h as one packed call: every field is 8 bytes wide.
+# The params structs of include/vesper_b200.h: every field is 8 bytes wide.
 _TABLES = struct.Struct("@17q")
 _ROTATE = struct.Struct("@8qd" + "q" * 27)
 _PROMPT = struct.Struct("@9qd" + "q" * 15)
 _SHARED = struct.Struct("@6qd" + "q" * 23)
+_STRUCTS = {"page_tables": _TABLES, "norm_rotate": _ROTATE, "prompt_attention": _PROMPT,
+            "shared_prefix_attention": _SHARED}
+
+
+def call_device(name: str, fields, cuda_stream: int = 0) -> None:
+    """vesper_<name>_device itself, for callers that hold device addresses (e.g. torch data_ptr()) instead of tensors:
+    the params struct's members after struct_size, in the header's order."""
+    packed = _STRUCTS[name]
+    lib = N.load()
+    _check(lib, getattr(lib, f"vesper_{name}_device")(packed.pack(packed.size, *fields), cuda_stream))
 
 
 class PageTables(NamedTuple):
@@ -41,124 +55,6 @@ class PageTables(NamedTuple):
     used: torch.Tensor       # [1] int32: pages that the batch takes from the free list
 
 
-# Entry points of the library, resolved on the first call.
-_lib = None
-
-
-def _entries():
-    global _lib
-    _lib = N.load()
-    return _lib
-
-
-def _refuse(why: str):
-    raise VesperError(N.VESPER_ERROR_INVALID_PARAM, why)
-
-
-def _wrong(t: torch.Tensor, device: torch.device, dtype: torch.dtype, name: str):
-    if t.device != device:
-        _refuse(f"{name} is on {t.device}, not on {device}")
-    _refuse(f"{name} is {t.dtype}, {dtype} expected")
-
-
-def _ints(t: torch.Tensor, device: torch.device, name: str, n: int | None = None, dtype=torch.int32) -> int:
-    """Address of a contiguous vector, of whole numbers unless dtype says otherwise."""
-    if t.dtype is not dtype or t.device != device:
-        _wrong(t, device, dtype, name)
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
-        _refuse(f"{name} must be a contiguous vector" + ("" if n is None else f" of {n}"))
-    return t.data_ptr()
-
-
-def _cuda(t: torch.Tensor, name: str) -> torch.device:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _refuse(f"{name} must be a CUDA tensor")
-    return t.device
-
-
-def _odd_strides(t: torch.Tensor, name: str) -> tuple[int, ...]:
-    """All strides but the last, which must be 1; those of single-element dims do not matter."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        _refuse(f"{name}: the last dimension must be contiguous")
-    return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:-1], t.stride()))
-
-
-def _heads(t: torch.Tensor, device, dtype, name: str, tokens: int | None, heads: int | None, dim: int):
-    """(address, token stride, head stride) of a [tokens, heads, dim] tensor."""
-    if t.dtype is not dtype or t.device != device:
-        _wrong(t, device, dtype, name)
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or \
-            (heads is not None and shape[1] != heads):
-        _refuse(f"{name} has shape {tuple(shape)}: [tokens, heads, head_dim] in line with q expected")
-    a, b, c = t.stride()
-    if c != 1 or a % 8 or b % 8:
-        a, b = _odd_strides(t, name)
-    return t.data_ptr(), a, b
-
-
-def _queries(q: torch.Tensor):
-    """Device, dtype code, shape and fields of q."""
-    dev, dt = _cuda(q, "q"), _DTYPES.get(q.dtype)
-    if dt is None or q.dim() != 3:
-        _refuse("q must be bf16 or f16, [tokens, heads, head_dim]")
-    t, heads, dim = q.shape
-    a, b, c = q.stride()
-    if c != 1 or a % 8 or b % 8:
-        a, b = _odd_strides(q, "q")
-    return dev, dt, t, heads, dim, (q.data_ptr(), a, b)
-
-
-def _caches(k_cache, v_cache, device, dtype, kv_heads: int | None, dim: int):
-    """Fields of both caches, then pages and page size."""
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype is not dtype or t.device != device:
-            _wrong(t, device, dtype, name)
-    shape = k_cache.shape
-    if len(shape) != 4 or shape != v_cache.shape or shape[3] != dim or (kv_heads is not None and shape[2] != kv_heads):
-        _refuse(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)}: "
-                "[pages, page_size, kv_heads, head_dim] in line with q expected")
-    a, b, c, d = k_cache.stride()
-    e, f, g, h = v_cache.stride()
-    if d != 1 or h != 1 or (a | b | c | e | f | g) % 8:
-        a, b, c = _odd_strides(k_cache, "k_cache")
-        e, f, g = _odd_strides(v_cache, "v_cache")
-    return k_cache.data_ptr(), a, b, c, v_cache.data_ptr(), e, f, g, shape[0], shape[1]
-
-
-def _table(table: torch.Tensor, device, n: int):
-    """Address, width and row stride of a [n, width] table."""
-    if table.dtype is not torch.int32 or table.device != device:
-        _wrong(table, device, torch.int32, "table")
-    if table.dim() != 2 or table.shape[0] != n or (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse("table must be [requests, width] with contiguous rows")
-    width = table.shape[1]
-    return table.data_ptr(), width, table.stride(0) if n > 1 else width
-
-
-def _call(fn, params: bytes, device: torch.device) -> None:
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)  # the address of torch.cuda.current_stream(device)
-    if index == torch.cuda.current_device():
-        status = fn(params, stream)
-    else:  # the library launches on the calling thread's device
-        with torch.cuda.device(device):
-            status = fn(params, stream)
-    if status != N.VESPER_OK:
-        _check(_lib, status)
-
-
-@functools.lru_cache(maxsize=4096)
-def _prompt_workspace(*sizes) -> int:
-    return _lib.vesper_prompt_attention_workspace(_PROMPT.pack(*sizes, *(0,) * 15))
-
-
-@functools.lru_cache(maxsize=4096)
-def _shared_workspace(head: tuple, n_pages: int, page_size: int, prefix_len: int, width: int) -> int:
-    return _lib.vesper_shared_prefix_attention_workspace(
-        _SHARED.pack(*head, *(0,) * 11, n_pages, page_size, 0, prefix_len, 0, width, *(0,) * 6))
-
-
 def page_tables(cached: torch.Tensor, fresh: torch.Tensor, free: torch.Tensor, table: torch.Tensor, page_size: int,
                 total: int, base: int = 0) -> PageTables:
     """Pages, cache slots and positions of a batch's new tokens (vesper_page_tables_device).
@@ -168,19 +64,7 @@ def page_tables(cached: torch.Tensor, fresh: torch.Tensor, free: torch.Tensor, t
     fresh; rows past it get slot -1 and position 0); base: position of a request's first token, the length of the
     prefix that it follows.  Where free does not suffice (used > len(free)), entries and slots are -1.
     """
-    dev = _cuda(cached, "cached")
-    n = cached.shape[0] if cached.dim() == 1 else _refuse("cached must be a vector")
-    c, f, fr = _ints(cached, dev, "cached", n), _ints(fresh, dev, "fresh", n), _ints(free, dev, "free")
-    if total < 0 or page_size < 0:
-        _refuse("total and page_size must not be negative")
-    ints = cached.new_empty(2 * n + 2 + total)
-    slots = cached.new_empty(total, dtype=torch.int64)
-    p = ints.data_ptr()
-    _call((_lib or _entries()).vesper_page_tables_device, _TABLES.pack(
-        _TABLES.size, c, f, n, fr, free.shape[0], *_table(table, dev, n), page_size, total, base, p, p + 4 * n,
-        p + 8 * n + 4, slots.data_ptr(), p + 8 * n + 4 + 4 * total), dev)
-    lengths, starts, positions, used = ints.split((n, n + 1, total, 1))
-    return PageTables(table, lengths, starts, positions, slots, used)
+    return PageTables(table, *_ops.page_tables(cached, fresh, free, table, page_size, total, base))
 
 
 def norm_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor,
@@ -195,30 +79,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positi
     With slots (int64 [tokens], -1: skip), keys and values go to the caches.  Returns (q, k) as new contiguous tensors,
     k None without keep_k.
     """
-    dev, dt, t, heads, dim, fq = _queries(q)
-    fk = _heads(k, dev, q.dtype, "k", t, None, dim)
-    kv = k.shape[1]
-    if turns.dtype is not torch.float32 or turns.device != dev:
-        _wrong(turns, dev, torch.float32, "turns")
-    if turns.dim() != 2 or not turns.is_contiguous():
-        _refuse("turns must be [positions, turned], contiguous")
-    wq = 0 if q_weight is None else _ints(q_weight, dev, "q_weight", dim, q.dtype)
-    wk = 0 if k_weight is None else _ints(k_weight, dev, "k_weight", dim, q.dtype)
-    if slots is not None:
-        if v is None or k_cache is None or v_cache is None:
-            _refuse("slots need v, k_cache and v_cache")
-        fs = _ints(slots, dev, "slots", t, torch.int64)
-        fv = _heads(v, dev, q.dtype, "v", t, kv, dim)
-        fc = _caches(k_cache, v_cache, dev, q.dtype, kv, dim)
-    else:
-        fs, fv, fc = 0, (0, 0, 0), (0,) * 10
-    out_q = q.new_empty((t, heads, dim))
-    out_k = q.new_empty((t, kv, dim)) if keep_k else None
-    _call((_lib or _entries()).vesper_norm_rotate_device, _ROTATE.pack(
-        _ROTATE.size, dt, t, heads, kv, dim, turns.shape[1], 1 if pairs else 0, eps, *fq, *fk, *fv,
-        _ints(positions, dev, "positions", t), turns.data_ptr(), turns.shape[0], wq, wk, fs, *fc, out_q.data_ptr(),
-        out_k.data_ptr() if keep_k else 0), dev)
-    return out_q, out_k
+    return _ops.norm_rotate(q, k, v, positions, turns, q_weight, k_weight, eps, pairs, slots, k_cache, v_cache, keep_k)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
@@ -232,25 +93,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     [tokens, heads, head_dim], with stats (out, lse): the float32 [tokens, heads] log-sum-exp.  Rows that see no key
     are zero, their lse -inf.
     """
-    dev, dt, t, heads, dim, fq = _queries(q)
-    fk = _heads(k, dev, q.dtype, "k", None, None, dim)
-    n_k, kv = k.shape[0], k.shape[1]
-    fv = _heads(v, dev, q.dtype, "v", n_k, kv, dim)
-    s = _ints(starts, dev, "starts")
-    n = starts.shape[0] - 1
-    if n < 0:
-        _refuse("starts must hold at least one entry")
-    sk = 0 if starts_k is None else _ints(starts_k, dev, "starts_k", n + 1)
-    out = q.new_empty((t, heads, dim))
-    lse = q.new_empty((t, heads), dtype=torch.float32) if stats else None
-    lib = _lib or _entries()
-    sizes = (_PROMPT.size, dt, n, t, n_k, heads, kv, dim, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
-    need = _prompt_workspace(*sizes)
-    space = q.new_empty(need, dtype=torch.uint8) if need else None
-    _call(lib.vesper_prompt_attention_device, _PROMPT.pack(
-        *sizes, *fq, *fk, *fv, s, sk, out.data_ptr(), lse.data_ptr() if stats else 0, space.data_ptr() if need else 0,
-        need), dev)
-    return (out, lse) if stats else out
+    return _ops.prompt_attention(q, k, v, starts, starts_k, causal, scale, stats)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pages: torch.Tensor,
@@ -262,19 +105,4 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     hold the prefix_len tokens all requests begin with; table int32 [requests, width] and lengths int32 [requests]: the
     pages and the count of each request's own tokens.  Returns out [requests, heads, head_dim], with stats (out, lse).
     """
-    dev, dt, b, heads, dim, fq = _queries(q)
-    fc = _caches(k_cache, v_cache, dev, q.dtype, None, dim)
-    pages = _ints(prefix_pages, dev, "prefix_pages")
-    if prefix_len < 0 or prefix_pages.shape[0] * fc[9] < prefix_len:
-        _refuse("prefix_pages do not hold prefix_len tokens")
-    ft = _table(table, dev, b)
-    out = q.new_empty((b, heads, dim))
-    lse = q.new_empty((b, heads), dtype=torch.float32) if stats else None
-    lib = _lib or _entries()
-    head = (_SHARED.size, dt, b, heads, k_cache.shape[2], dim, dim ** -0.5 if scale is None else scale)
-    need = _shared_workspace(head, fc[8], fc[9], prefix_len, ft[1])
-    space = q.new_empty(need, dtype=torch.uint8) if need else None
-    _call(lib.vesper_shared_prefix_attention_device, _SHARED.pack(
-        *head, *fq, *fc, pages, prefix_len, *ft, _ints(lengths, dev, "lengths", b), out.data_ptr(),
-        lse.data_ptr() if stats else 0, space.data_ptr() if need else 0, need), dev)
-    return (out, lse) if stats else out
+    return _ops.shared_prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengths, scale, stats)

@@ -1,4 +1,5 @@
-"""Build libvesper_c.so (the B200 IVF-PQ engine and its C ABI) in-tree.
+"""Build libvesper_c.so (the B200 IVF-PQ engine and its C ABI) and _attention.so (the attention
+operators on torch tensors, over that ABI) in-tree.
 
 CUDA sources are compiled for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``);
 host sources with g++ -std=c++23.  Objects go to vesper_db_b200/_build/ and are rebuilt
@@ -19,6 +20,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libvesper_c.so")
+EXT_SRC = os.path.join(CSRC, "attention_torch.cpp")
+EXT = os.path.join(PKG, "_attention.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA, "bin", "nvcc")
 CXX = "g++"
@@ -61,6 +64,8 @@ def build(verbose: bool = False) -> str:
             jobs.append(("nvcc", [NVCC, *NVCC_FLAGS, "-c", src, "-o", obj]))
         objs.append(obj)
     for src in sorted(glob.glob(os.path.join(CSRC, "*.cpp"))):
+        if src == EXT_SRC:
+            continue
         obj = os.path.join(BUILD, os.path.basename(src) + ".o")
         if _stale(obj, src, deps):
             jobs.append(("g++ ", [CXX, *CXX_FLAGS, "-c", src, "-o", obj]))
@@ -79,7 +84,25 @@ def build(verbose: bool = False) -> str:
     if jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         _run([NVCC, "-shared", "-Xlinker", "--no-undefined", "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static",
               "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"])
+    if _stale(EXT, EXT_SRC, [os.path.join(ROOT, "include", "vesper_b200.h"), os.path.join(ROOT, "include", "vesper.h")]):
+        _build_extension(verbose)
     return LIB
+
+
+def _build_extension(verbose: bool) -> None:
+    """The extension module: torch's and Python's headers, linked to the library beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    if verbose:
+        print("g++ ", os.path.basename(EXT_SRC), flush=True)
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          *[f"-isystem{p}" for p in include_paths()], f"-isystem{sysconfig.get_paths()['include']}",
+          f"-isystem{CUDA}/include", f"-I{ROOT}/include", EXT_SRC, f"-L{PKG}", "-l:libvesper_c.so", f"-L{lib}", "-lc10",
+          "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-o", EXT])
 
 
 if __name__ == "__main__":

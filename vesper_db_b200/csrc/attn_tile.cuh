@@ -178,6 +178,10 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
         : "memory");
 }
 
+// Lane 0's value, known to the compiler as one for the warp: descriptors made from it stay in
+// uniform registers, which a product's issue needs them in.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // What a block works on.
 struct Work {
     int q0;        // first row of q of the block's first tile
@@ -344,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
     const int tt = p.tile_tokens;
 
     bool ok = true;  // sticky: after a wait that ran out a warp waits no more
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t id_s = common | ((uint32_t)(kKeys >> 3) << 17);
             constexpr uint32_t id_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-            const int t = warp - 17;
+            const int t = uniform(warp - 17);
             const uint32_t t_s = tmem + t * 128, t_o = tmem + 256 + t * 128;
             const uint64_t q_desc = tc::sw128_kmajor_desc(s_q + t * kTileBytes);
             auto scores = [&](int slot) {
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 work_done(it);
                 if (w.stop) break;
                 const Tiles x = tiles_of(w, tt, p.splits);
-                const int n = x.n, mine = t ? x.nt1 : x.nt0;
+                const int n = uniform(x.n), mine = uniform(t ? x.nt1 : x.nt0);
                 if (n == 0) continue;
                 auto slot_of = [&](int i) { return (int)((kv + i) % kSlots); };
                 auto arrived = [&](int i) { return wait(&kv_full[slot_of(i)], ((kv + i) / kSlots) & 1); };
