@@ -38,6 +38,7 @@ struct PageTablesArgs {
     int32_t* positions;
     int64_t* slots;
     int32_t* used;
+    bool wide;  // positions and slots are 16-byte aligned
 };
 
 struct NormRotateArgs {

@@ -162,6 +162,7 @@ VESPER_C_API vesper_status_t vesper_page_tables_device(const vesper_page_tables_
         a.positions = p.d_positions;
         a.slots = p.d_slots;
         a.used = p.d_used;
+        a.wide = aligned16(p.d_positions) && aligned16(p.d_slots);
         vgpu::launch_page_tables(a, static_cast<cudaStream_t>(cuda_stream));
     });
 }

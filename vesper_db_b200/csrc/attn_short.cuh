@@ -71,18 +71,26 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
     const int n = (max(last, 0) + kShortKeys - 1) / kShortKeys;
     const int min_lim = min(max(w.first_lim, 0), w.len_k);  // keys that every row sees
 
+    // A thread copies the same 16-byte chunk of every kRowStep-th row; rows past the last key
+    // are filled with zeros (nothing is read for them).
     const uint32_t s_kv = tc::smem_u32(smem);
+    constexpr int kRowStep = kShortThreads / kChunks;
+    const int row0 = tid / kChunks, chunk = tid % kChunks;
+    const uint32_t at0 = row0 * kRowBytes + ((chunk ^ (row0 & 7)) << 4);  // kRowStep is a multiple of 8
+    const bool here = chunk * 8 < p.dim;
+    const T* k_at = static_cast<const T*>(p.k.p) + (w.k0 + row0) * p.k.tok + kh * p.k.head + (here ? chunk * 8 : 0);
+    const T* v_at = static_cast<const T*>(p.v.p) + (w.k0 + row0) * p.v.tok + kh * p.v.head + (here ? chunk * 8 : 0);
+    const long long k_step = kRowStep * p.k.tok, v_step = kRowStep * p.v.tok;
     auto request = [&](int j) {
-        const uint32_t dst = s_kv + (j & 1) * 2 * kTileBytes;
+        const uint32_t dst = s_kv + (j & 1) * 2 * kTileBytes + at0;
+        const int left = here ? w.len_k - j * kShortKeys - row0 : 0;
 #pragma unroll
-        for (int i = 0; i < kShortKeys * kChunks / kShortThreads; ++i) {
-            const int e = i * kShortThreads + tid, row = e / kChunks, c = e % kChunks;
-            const long long key = w.k0 + min(j * kShortKeys + row, w.len_k - 1);
-            const bool some = j * kShortKeys + row < w.len_k && c * 8 < p.dim;
-            const uint32_t at = row * kRowBytes + ((c ^ (row & 7)) << 4);
-            const int d = c * 8 < p.dim ? c * 8 : 0;
-            copy16(dst + at, static_cast<const T*>(p.k.p) + key * p.k.tok + kh * p.k.head + d, some);
-            copy16(dst + kTileBytes + at, static_cast<const T*>(p.v.p) + key * p.v.tok + kh * p.v.head + d, some);
+        for (int i = 0; i < kShortKeys / kRowStep; ++i) {
+            const bool some = i * kRowStep < left;
+            copy16(dst + i * kRowStep * kRowBytes, some ? k_at : p.k.p, some);
+            copy16(dst + kTileBytes + i * kRowStep * kRowBytes, some ? v_at : p.v.p, some);
+            k_at += k_step;
+            v_at += v_step;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };

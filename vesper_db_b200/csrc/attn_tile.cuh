@@ -315,6 +315,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     // The own pages' kernel may be queued behind this one and does not depend on it.
     if (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+    if (warp == 16 && lane < 3 && p.n_k > 0) {
+        const CUtensorMap* map = lane == 0 ? &p.mq : (lane == 1 ? &p.mk : &p.mv);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
     if (warp == 17) {
         if (lane == 0) {
             for (int i = 0; i < 2; ++i) {

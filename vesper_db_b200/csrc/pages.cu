@@ -16,10 +16,12 @@ namespace {
 //   table[b, had_b + i] = free[first_b + i],
 //   starts_b = sum_{a < b} fresh_a; token t of request b has n = cached_b + t - starts_b,
 //   slot table[b, n / P] * P + n % P, position base + n.
-// One launch: every block scans all requests itself (two int32 loads each, from L2), so
-// no block waits for another; then each block fills its share of tokens and table rows.
-// A token's new page is taken from the free list directly, never from a table entry that
-// another block may still be writing.
+// One launch: every block scans all requests itself (two int32 loads each, from L2; a
+// thread takes a run of neighbouring ones), so no block waits for another; then each block
+// fills its share of tokens and table rows.  What the tokens need of a request is in shared
+// memory by then, and a token's new page is taken from the free list directly, never from a
+// table entry that another block may still be writing.  Bound by the latency of its chain of
+// loads: lengths, then pages, then the stores.
 // ---------------------------------------------------------------------------------
 constexpr int kScanThreads = 512;
 
@@ -29,55 +31,60 @@ __device__ __forceinline__ int clamp_int(long long v) {
 
 __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_constant__ PageTablesArgs a) {
     extern __shared__ int smem[];
-    int* s_start = smem;                        // [n + 1] first token of each request
-    int* s_first = smem + a.n_requests + 1;     // [n + 1] first free-list entry of each request
+    const int n = a.n_requests;
+    int* s_start = smem;              // [n + 1] first token of each request
+    int* s_first = smem + n + 1;      // [n + 1] first free-list entry of each request
+    int* s_old = smem + 2 * (n + 1);  // [n] tokens held
     __shared__ long long s_warp[2][kScanThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_requests;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int page = 1 << a.page_shift;
 
-    // Exclusive scans, kScanThreads requests at a time; sums in 64 bits.
-    long long run_t = 0, run_p = 0;
-    for (int r0 = 0; r0 < n; r0 += kScanThreads) {
-        const int r = r0 + tid;
-        long long fresh = 0, pages = 0;
-        if (r < n) {
-            const long long old = max(a.cached[r], 0);
-            fresh = max(a.fresh[r], 0);
-            pages = ((old + fresh + page - 1) >> a.page_shift) - ((old + page - 1) >> a.page_shift);
-            if (blockIdx.x == 0) a.lengths[r] = clamp_int(old + fresh);
-        }
-        long long it = fresh, ip = pages;
+    // Exclusive scans of the new tokens and new pages; sums in 64 bits.
+    const int per = (n + kScanThreads - 1) / kScanThreads, r0 = min(tid * per, n), r1 = min(r0 + per, n);
+    long long sum_t = 0, sum_p = 0;
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) {
+        const long long old = max(__ldg(a.cached + r), 0), fresh = max(__ldg(a.fresh + r), 0);
+        s_old[r] = (int)old;
+        s_start[r] = clamp_int(sum_t);  // within the run, for now
+        s_first[r] = clamp_int(sum_p);
+        sum_t += fresh;
+        sum_p += ((old + fresh + page - 1) >> a.page_shift) - ((old + page - 1) >> a.page_shift);
+        if (blockIdx.x == 0) a.lengths[r] = clamp_int(old + fresh);
+    }
+    long long it = sum_t, ip = sum_p;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long ut = __shfl_up_sync(0xffffffffu, it, o), up = __shfl_up_sync(0xffffffffu, ip, o);
-            if (lane >= o) { it += ut; ip += up; }
-        }
-        if (lane == 31) { s_warp[0][warp] = it; s_warp[1][warp] = ip; }
-        __syncthreads();
-        long long bt = run_t, bp = run_p;
-        for (int w = 0; w < kScanThreads / 32; ++w) {
-            if (w < warp) { bt += s_warp[0][w]; bp += s_warp[1][w]; }
-            run_t += s_warp[0][w];
-            run_p += s_warp[1][w];
-        }
-        if (r < n) {
-            s_start[r] = clamp_int(bt + it - fresh);
-            s_first[r] = clamp_int(bp + ip - pages);
-        }
-        __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long ut = __shfl_up_sync(0xffffffffu, it, o), up = __shfl_up_sync(0xffffffffu, ip, o);
+        if (lane >= o) { it += ut; ip += up; }
+    }
+    if (lane == 31) { s_warp[0][warp] = it; s_warp[1][warp] = ip; }
+    __syncthreads();
+    long long bt = it - sum_t, bp = ip - sum_p, all_t = 0, all_p = 0;
+#pragma unroll
+    for (int w = 0; w < kScanThreads / 32; ++w) {
+        if (w < warp) { bt += s_warp[0][w]; bp += s_warp[1][w]; }
+        all_t += s_warp[0][w];
+        all_p += s_warp[1][w];
+    }
+    for (int r = r0; r < r1; ++r) {
+        s_start[r] = clamp_int(bt + s_start[r]);
+        s_first[r] = clamp_int(bp + s_first[r]);
+        if (blockIdx.x == 0) a.starts[r] = s_start[r];
     }
     if (tid == 0) {
-        s_start[n] = clamp_int(run_t);
-        s_first[n] = clamp_int(run_p);
-        if (blockIdx.x == 0) a.used[0] = clamp_int(run_p);
+        s_start[n] = clamp_int(all_t);
+        s_first[n] = clamp_int(all_p);
+        if (blockIdx.x == 0) {
+            a.starts[n] = s_start[n];
+            a.used[0] = s_first[n];
+        }
     }
     __syncthreads();
-    if (blockIdx.x == 0)
-        for (int r = tid; r <= n; r += kScanThreads) a.starts[r] = s_start[r];
 
     // New table entries: one warp a request.
     for (int r = blockIdx.x * (kScanThreads / 32) + warp; r < n; r += gridDim.x * (kScanThreads / 32)) {
-        const long long had = ((long long)max(a.cached[r], 0) + page - 1) >> a.page_shift;
+        const long long had = ((long long)s_old[r] + page - 1) >> a.page_shift;
         const int first = s_first[r], more = s_first[r + 1] - first;
         for (int i = lane; i < more; i += 32) {
             if (had + i >= a.table_width) break;
@@ -95,31 +102,44 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
             const int mid = (lo + hi) >> 1;
             if (s_start[mid] <= t0) lo = mid; else hi = mid;
         }
-        int r = lo;
+        int r = lo, pos[kRun];
+        long long from[kRun];  // where the page's number stands: an index of the table, or -2 - one of the free list
+        int off[kRun];
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
             const long long t = t0 + i;
-            if (t >= a.n_tokens) break;
             while (r < n && s_start[r + 1] <= t) ++r;
-            int pos = 0;
-            int64_t slot = -1;
+            pos[i] = 0;
+            from[i] = -1;
+            off[i] = 0;
             if (r < n) {
-                const long long old = max(a.cached[r], 0), at = old + t - s_start[r];
+                const long long old = s_old[r], at = old + t - s_start[r];
                 const long long col = at >> a.page_shift, had = (old + page - 1) >> a.page_shift;
-                int32_t pg = -1;
+                const long long f = s_first[r] + col - had;
                 if (col < a.table_width) {
-                    if (col < had) {
-                        pg = a.table[(long long)r * a.table_stride + col];
-                    } else {
-                        const long long f = s_first[r] + col - had;
-                        if (f < a.n_free) pg = a.free_pages[f];
-                    }
+                    if (col < had) from[i] = (long long)r * a.table_stride + col;
+                    else if (f < a.n_free) from[i] = -2 - f;
                 }
-                if (pg >= 0) slot = ((int64_t)pg << a.page_shift) + (at & (page - 1));
-                pos = clamp_int(at + a.base);
+                off[i] = (int)(at & (page - 1));
+                pos[i] = clamp_int(at + a.base);
             }
-            a.positions[t] = pos;
-            a.slots[t] = slot;
+        }
+        int32_t pg[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+            pg[i] = from[i] >= 0 ? a.table[from[i]] : (from[i] < -1 ? __ldg(a.free_pages - 2 - from[i]) : -1);
+        int64_t slot[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) slot[i] = pg[i] >= 0 ? ((int64_t)pg[i] << a.page_shift) + off[i] : -1;
+        if (t0 + kRun <= a.n_tokens && a.wide) {
+            *reinterpret_cast<int4*>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<longlong2*>(a.slots + t0) = make_longlong2(slot[0], slot[1]);
+            *reinterpret_cast<longlong2*>(a.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+        } else {
+            for (int i = 0; i < kRun && t0 + i < a.n_tokens; ++i) {
+                a.positions[t0 + i] = pos[i];
+                a.slots[t0 + i] = slot[i];
+            }
         }
     }
 }
@@ -312,12 +332,12 @@ void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
 }  // namespace
 
 void launch_page_tables(const PageTablesArgs& a, cudaStream_t st) {
-    const size_t smem = 2 * ((size_t)a.n_requests + 1) * sizeof(int);
+    const size_t smem = 3 * ((size_t)a.n_requests + 1) * sizeof(int);
     if (smem > 48 * 1024)
         VGPU_CHECK(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const long long per_block = kScanThreads * 4;
     const long long want = std::max<long long>((a.n_tokens + per_block - 1) / per_block, (a.n_requests + 63) / 64);
-    const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 2);
+    const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 3);
     page_tables_kernel<<<blocks, kScanThreads, smem, st>>>(a);
     VGPU_LAUNCH("page_tables_kernel");
 }
