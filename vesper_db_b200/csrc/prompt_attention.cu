@@ -19,11 +19,12 @@ using attn::TileParams;
 
 constexpr int kSms = 148;
 // Prompts go to the small blocks when their mean is at most this many query rows (tokens
-// times group: a tensor-memory block's 256) and keys.  30,000 tokens of one length, us in
-// small blocks / tiles: 32 + 8 heads of 128, 64 tokens (256 rows) 283 / 333, 128 tokens
-// 324 / 292; 12 heads of 64, 200 tokens 113 / 147, 300 tokens 112 / 159, 600 tokens 167 / 154.
-constexpr int kShortMeanRows = 256, kShortMeanKeys = 512;
-
+// times group) and keys: twice as many rows, and more, while the tiles would not give every
+// SM a block, as it is the latency of one that counts then.  30,000 tokens of one length, us
+// in small blocks / tiles: 32 + 8 heads of 128, 16 tokens (64 rows) 334 / 465, 32 tokens
+// 302 / 284; 12 heads of 64, 100 tokens 89 / 111, 200 tokens 107 / 113 (causal), 136 / 93
+// (full).  1,500 tokens: 32 + 8 heads, 64 tokens 20 / 26, 150 tokens 25 / 25.
+constexpr int kShortMeanRows = 128, kShortMeanRowsFew = 384, kShortMeanKeys = 512;
 // Prefix rows in tiles of 8 or 16: up to this many of them, re-reading the prefix for each
 // from L2 is quicker than a tensor-core tile.
 constexpr int kFewRowTiles = 4;
@@ -612,7 +613,9 @@ struct PromptPlan {
 PromptPlan prompt_plan(const PromptArgs& a) {
     const int group = a.heads / a.kv_heads;
     PromptPlan pl;
-    pl.small = group <= attn::kShortRows && a.n_q * group <= (long long)kShortMeanRows * a.n_requests &&
+    const long long blocks = ((a.n_q + 2 * (kRows / group) - 1) / (2 * (kRows / group)) + a.n_requests) * a.kv_heads;
+    const int rows = blocks <= kSms ? kShortMeanRowsFew : kShortMeanRows;
+    pl.small = group <= attn::kShortRows && a.n_q * group <= (long long)rows * a.n_requests &&
                a.n_k <= (long long)kShortMeanKeys * a.n_requests;
     if (pl.small) {
         pl.tiles = a.n_q / (attn::kShortRows / group) + a.n_requests + 2;
