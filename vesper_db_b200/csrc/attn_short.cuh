@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kh = blockIdx.x % p.kv_heads;
     if (warp == 0) {
-        const Work w = find_work(p, blockIdx.x / p.kv_heads, lane, p.tile_tokens);
+        int near = -1;
+        const Work w = find_work(p, blockIdx.x / p.kv_heads, lane, p.tile_tokens, near);
         if (lane == 0) {
             s_work = w;
             s_leak = 0;

@@ -224,30 +224,62 @@ __device__ __forceinline__ Tiles tiles_of(const Work& w, int tt, int splits) {
 // adding up lengths: 32 candidates a step.  Rows before the first and after the last request
 // are requests without keys.  Last pieces come first: the rows of a causal prompt's end see
 // the most keys.
-__device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane, int span) {
+//
+// `near` is the request of the last piece that the warp looked for, or -1: the pieces that a
+// block takes come in order, so the next one's request is mostly among the 32 up to there,
+// and one step of loads finds it with its keys (the search from scratch takes three or four,
+// one after the other, 1.5 us).
+__device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane, int span, int& near) {
     const int n = p.n_requests + 2;
     auto bound = [&](int b) {  // first row of request b
-        if (b == 0) return 0;
+        if (b <= 0) return 0;
         if (b >= n) return p.n_q;
-        return min(max(p.starts[b - 1], 0), p.n_q);
+        return min(max(__ldg(p.starts + b - 1), 0), p.n_q);
+    };
+    auto key_bound = [&](int b) {  // first key row of request b, 1 .. n_requests + 1
+        return min(max(__ldg(p.starts_k + b - 1), 0), p.n_k);
     };
     const int want = p.n_q / span + n - 1 - idx;
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, c = lo + (lane + 1) * step;
-        const bool before = c < hi && bound(c) / span + c <= want;
-        lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
-        hi = min(hi, lo + step);
+    int lo = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+    bool found = false;
+    if (near >= 0) {
+        const int b = near - lane;
+        int kb = 0, ke = 0;
+        const int qb = bound(b), qe = bound(b + 1);
+        if (b > 0 && b <= p.n_requests) {
+            kb = key_bound(b);
+            ke = max(key_bound(b + 1), kb);
+        }
+        const unsigned at = __ballot_sync(0xffffffffu, b >= 0 && qb / span + b <= want);
+        found = at != 0;
+        const int src = found ? __ffs(at) - 1 : 0;
+        lo = near - src;
+        q0 = __shfl_sync(0xffffffffu, qb, src);
+        q1 = __shfl_sync(0xffffffffu, qe, src);
+        k0 = __shfl_sync(0xffffffffu, kb, src);
+        k1 = __shfl_sync(0xffffffffu, ke, src);
     }
+    if (!found) {
+        int hi = n;
+        lo = 0;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, c = lo + (lane + 1) * step;
+            const bool before = c < hi && bound(c) / span + c <= want;
+            lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+            hi = min(hi, lo + step);
+        }
+        q0 = bound(lo);
+        q1 = bound(lo + 1);
+        if (lo > 0 && lo <= p.n_requests) {
+            k0 = key_bound(lo);
+            k1 = max(key_bound(lo + 1), k0);
+        }
+    }
+    near = lo;
     Work w{};
-    const int q0 = bound(lo), len_q = bound(lo + 1) - q0, tok = (want - q0 / span - lo) * span;
+    const int len_q = q1 - q0, tok = (want - q0 / span - lo) * span;
     w.q0 = q0 + tok;
     w.tokens = tok >= 0 ? len_q - tok : 0;
-    int k0 = 0, k1 = 0;
-    if (lo > 0 && lo <= p.n_requests) {
-        k0 = min(max(p.starts_k[lo - 1], 0), p.n_k);
-        k1 = min(max(p.starts_k[lo], k0), p.n_k);
-    }
     w.k0 = k0;
     w.len_k = k1 - k0;
     w.step = p.causal ? 1 : 0;
@@ -267,7 +299,7 @@ __device__ __forceinline__ bool not_finite(uint4 u) {
 
 // Piece of work number `item`: key heads fastest, then splits.  Run by one whole warp.
 template <bool PAGED>
-__device__ __forceinline__ Work item_work(const TileParams& p, int item, int lane) {
+__device__ __forceinline__ Work item_work(const TileParams& p, int item, int lane, int& near) {
     Work w{};
     const int kh = item % p.kv_heads, rest = item / p.kv_heads, split = rest % p.splits, block = rest / p.splits;
     if (PAGED) {  // every row sees the whole prefix
@@ -275,7 +307,7 @@ __device__ __forceinline__ Work item_work(const TileParams& p, int item, int lan
         w.tokens = p.n_q - w.q0;
         w.len_k = w.first_lim = p.n_k;
     } else {
-        w = find_work(p, block, lane, 2 * p.tile_tokens);
+        w = find_work(p, block, lane, 2 * p.tile_tokens, near);
     }
     w.kh = kh;
     w.split = split;
@@ -386,13 +418,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         tma4(s_q + t * kTileBytes + h * kHalfBytes, &p.mq, h * 64, 0, w.kh, w.q0 + t * tt, &q_full[t]);
                 }
             };
-            int item = blockIdx.x;
+            int item = blockIdx.x, near = -1;
             while (ok) {
                 Work w{};
                 w.stop = 1;
                 // pieces that turn out to be empty are passed over
                 while (item < p.items) {
-                    w = item_work<PAGED>(p, item, lane);
+                    w = item_work<PAGED>(p, item, lane, near);
                     if (w.tokens > 0) break;
                     w.stop = 1;
                     if (p.counter) {
@@ -680,6 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         // ---- results
         const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + w.kh * p.group + row_head);
         const bool leak = !PAGED && my_tiles > 0 && ok && *reinterpret_cast<volatile int*>(&s_leak[it % kAhead]) != 0;
+        // The piece's place is handed back before the stores: the arrival would wait for them.
+        work_done(it++);
         const bool part = p.part;
         const long long rows = (long long)p.n_q * p.heads;
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
@@ -758,13 +792,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         }
         // the next piece's first P, and with it the first product into O, comes after these reads
         tc::fence_before_sync();
-        work_done(it++);
         }
         // A wait ran out: this block's other rows are NaN too.
         if (!ok) {
             for (int item = blockIdx.x; item < p.items && half == 0; item += gridDim.x) {
                 if (p.counter) break;
-                const Work v = item_work<PAGED>(p, item, lane);
+                int near = -1;
+                const Work v = item_work<PAGED>(p, item, lane, near);
                 if (row_tok >= min(max(v.tokens - t * tt, 0), tt)) continue;
                 const long long at = (long long)(v.q0 + t * tt + row_tok) * p.heads + v.kh * p.group + row_head;
                 for (int d = 0; d < p.dim && !p.part; ++d) static_cast<uint16_t*>(p.out)[at * p.dim + d] = 0x7fff;
