@@ -585,3 +585,65 @@ def test_prompt_many_requests(V):
     check_prompt(V, lens, None, 2, 1, 64, torch.bfloat16, True, seed=3)
     lens = [1] * 40 + [0] * 40 + [9000]
     check_prompt(V, lens, None, 2, 1, 64, torch.bfloat16, False, seed=4)
+
+
+# ------------------------------------------------------------------------------------------ refusals on tensors
+def refused(says, call):
+    from vesper_db_b200 import VesperError
+    with pytest.raises(VesperError, match=says):
+        call()
+
+
+def test_refusals_of_tensors(V):
+    q, k = rand(5, 8, 64), rand(5, 2, 64)
+    st, pos, slots = ints([0, 5]), ints([0] * 5), ints([0] * 5, torch.int64)
+    turns = torch.zeros(9, 64, device="cuda")
+    kc = rand(4, 16, 2, 64)
+    table, lens, pages = ints([[0, 1]] * 5), ints([3] * 5), ints([2])
+    P, R, S, T = V.prompt_attention, V.norm_rotate, V.shared_prefix_attention, V.page_tables
+    refused("bf16 or f16", lambda: P(q.float(), k.float(), k.float(), st))
+    refused("k is Half", lambda: P(q, k.half(), k, st))
+    refused("CUDA", lambda: P(q.cpu(), k, k, st))
+    refused("k is on cpu", lambda: P(q, k.cpu(), k, st))
+    refused("k has shape", lambda: P(q, k[..., :32], k, st))
+    refused("v has shape", lambda: P(q, k, k[:4], st))
+    refused("multiple of kv_heads", lambda: P(q[:, :7], k, k, st))
+    refused("starts is Long", lambda: P(q, k, k, st.long()))
+    refused("starts_k must be", lambda: P(q, k, k, st, ints([0, 1, 5])))
+    refused("d_starts_k", lambda: P(q, rand(9, 2, 64), rand(9, 2, 64), st))
+    refused("scale", lambda: P(q, k, k, st, scale=0.0))
+    refused("scale must be a number", lambda: P(q, k, k, st, scale="x"))
+    refused("last dimension", lambda: P(rand(5, 64, 8).transpose(1, 2), k, k, st))
+    refused("head_dim", lambda: P(rand(5, 8, 136), rand(5, 2, 136), rand(5, 2, 136), st))
+    refused("strides", lambda: P(rand(5, 8, 68)[..., :64], k, k, st))
+    refused("aligned", lambda: P(rand(5 * 8 * 64 + 4)[4:].view(5, 8, 64), k, k, st))
+    refused("turned", lambda: R(q, k, None, pos, turns[:, :24].contiguous()))
+    refused("turns is", lambda: R(q, k, None, pos, turns.half()))
+    refused("slots need", lambda: R(q, k, None, pos, turns, slots=slots))
+    refused("slots is Int", lambda: R(q, k, k, pos, turns, slots=pos, k_cache=kc, v_cache=kc))
+    refused("k_cache", lambda: R(q, k, k, pos, turns, slots=slots, k_cache=kc[:, :, :1], v_cache=kc))
+    refused("q_weight", lambda: R(q, k, None, pos, turns, q_weight=q[0, 0, :32]))
+    refused("eps", lambda: R(q, k, None, pos, turns, eps=-1.0))
+    refused("positions", lambda: R(q, k, None, pos[:4], turns))
+    refused("prefix_pages do not hold", lambda: S(q, kc, kc, pages, 17, table, lens))
+    refused("prefix_len", lambda: S(q, kc, kc, pages, -1, table, lens))
+    refused("table must be", lambda: S(q, kc, kc, pages, 9, table[:4], lens))
+    refused("lengths must be", lambda: S(q, kc, kc, pages, 9, table, lens[:4]))
+    refused("page_size", lambda: S(q, kc[:, :8], kc[:, :8], pages, 4, table, lens))
+    refused("fresh must be", lambda: T(lens, lens[:2], pages, table, 16, 9))
+    refused("page_size", lambda: T(lens, lens, pages, table, 17, 9))
+    refused("total must not be negative", lambda: T(lens, lens, pages, table, 16, -1))
+    refused("base", lambda: T(lens, lens, pages, table, 16, 9, base=-1))
+    refused("contiguous rows", lambda: T(lens[:2], lens[:2], pages, table.T, 16, 9))
+
+
+def test_calls_with_addresses(V):
+    """The C entry points with device addresses give what the tensors' calls give."""
+    from vesper_db_b200 import attention as A
+    q, k, v = rand(70, 4, 64, seed=1), rand(70, 2, 64, seed=2), rand(70, 2, 64, seed=3)
+    st, out = ints([0, 30, 70]), torch.empty(70, 4, 64, dtype=torch.bfloat16, device="cuda")
+    A.call_device("prompt_attention", [0, 2, 70, 70, 4, 2, 64, 1, 0.125, q.data_ptr(), 256, 64, k.data_ptr(), 128, 64,
+                                       v.data_ptr(), 128, 64, st.data_ptr(), 0, out.data_ptr(), 0, 0, 0],
+                  torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(out, V.prompt_attention(q, k, v, st))
+    refused("scale", lambda: A.call_device("prompt_attention", [0, 2, 70, 70, 4, 2, 64, 1, -1.0] + [0] * 15))
