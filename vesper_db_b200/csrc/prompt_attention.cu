@@ -279,29 +279,50 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
     const int mask = (1 << a.page_shift) - 1;
     uint4 kf[2][KC], vf[4][VC];
     // 16 keys lie in one page.  Rows past the job's keys are not read: they may hold anything.
+    // Whole blocks of whole rows take the short way: no test a load, no zeros beforehand.
+    const bool whole = a.dim == D;
+    const T* const k_lane = static_cast<const T*>(a.k_cache.p) + kh * a.k_cache.head + g * a.k_cache.tok + t * 8;
+    const T* const v_lane = static_cast<const T*>(a.v_cache.p) + kh * a.v_cache.head + 2 * t * a.v_cache.tok + g * 8;
+    const long long k_rows = 8 * a.k_cache.tok, v_row = a.v_cache.tok, v_rows = 8 * a.v_cache.tok;
+    auto left_of = [&](const Cursor& c, int pg) {  // keys of the block that are there
+        return pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - c.block * kBlockKeys : 0;
+    };
     auto load_k = [&](const Cursor& c, int pg) {
-        const int key = c.block * kBlockKeys, left = pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - key : 0;
-        const T* p = static_cast<const T*>(a.k_cache.p) + pg * a.k_cache.page + (key & mask) * a.k_cache.tok + kh * a.k_cache.head;
+        const int left = left_of(c, pg);
+        const T* p = k_lane + pg * a.k_cache.page + ((c.block * kBlockKeys) & mask) * a.k_cache.tok;
+        if (whole && left >= kBlockKeys) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r, p += k_rows)
+#pragma unroll
+                for (int i = 0; i < KC; ++i) kf[r][i] = __ldcs(reinterpret_cast<const uint4*>(p + i * 32));
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r, p += k_rows)
 #pragma unroll
             for (int i = 0; i < KC; ++i) {
-                const int ch = (i * 4 + t) * 8;
                 kf[r][i] = make_uint4(0, 0, 0, 0);
-                if (ch < a.dim && r * 8 + g < left)
-                    kf[r][i] = *reinterpret_cast<const uint4*>(p + (r * 8 + g) * a.k_cache.tok + ch);
+                if ((i * 4 + t) * 8 < a.dim && r * 8 + g < left) kf[r][i] = *reinterpret_cast<const uint4*>(p + i * 32);
             }
     };
     auto load_v = [&](const Cursor& c, int pg) {
-        const int key = c.block * kBlockKeys, left = pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - key : 0;
-        const T* p = static_cast<const T*>(a.v_cache.p) + pg * a.v_cache.page + (key & mask) * a.v_cache.tok + kh * a.v_cache.head;
+        const int left = left_of(c, pg);
+        const T* p = v_lane + pg * a.v_cache.page + ((c.block * kBlockKeys) & mask) * a.v_cache.tok;
+        if (whole && left >= kBlockKeys) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < VC; ++i)
+                    vf[r][i] = __ldcs(reinterpret_cast<const uint4*>(p + (r & 1) * v_row + (r >> 1) * v_rows + i * 64));
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
-                const int ch = (i * 8 + g) * 8, k = 2 * t + (r & 1) + (r >> 1) * 8;
                 vf[r][i] = make_uint4(0, 0, 0, 0);
-                if (ch < a.dim && k < left) vf[r][i] = *reinterpret_cast<const uint4*>(p + k * a.v_cache.tok + ch);
+                if ((i * 8 + g) * 8 < a.dim && 2 * t + (r & 1) + (r >> 1) * 8 < left)
+                    vf[r][i] = *reinterpret_cast<const uint4*>(p + (r & 1) * v_row + (r >> 1) * v_rows + i * 64);
             }
     };
     // Rows of a job: row r is query head kh * group + (m0 + r) % group of request
