@@ -23,7 +23,7 @@ namespace {
 // table entry that another block may still be writing.  Bound by the latency of its chain of
 // loads: lengths, then pages, then the stores.
 // ---------------------------------------------------------------------------------
-constexpr int kScanThreads = 512;
+constexpr int kScanThreads = 512, kRun = 4;  // tokens a thread takes at once
 
 __device__ __forceinline__ int clamp_int(long long v) {
     return (int)(v < 0 ? 0 : (v > 0x7fffffffLL ? 0x7fffffffLL : v));
@@ -94,7 +94,6 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
     }
 
     // Tokens: a run of kRun consecutive ones a thread, one search for the first of them.
-    constexpr int kRun = 4;
     for (long long t0 = ((long long)blockIdx.x * kScanThreads + tid) * kRun; t0 < a.n_tokens;
          t0 += (long long)gridDim.x * kScanThreads * kRun) {
         int lo = 0, hi = n;  // the last request whose start is <= t0
@@ -132,9 +131,12 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < kRun; ++i) slot[i] = pg[i] >= 0 ? ((int64_t)pg[i] << a.page_shift) + off[i] : -1;
         if (t0 + kRun <= a.n_tokens && a.wide) {
-            *reinterpret_cast<int4*>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-            *reinterpret_cast<longlong2*>(a.slots + t0) = make_longlong2(slot[0], slot[1]);
-            *reinterpret_cast<longlong2*>(a.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+#pragma unroll
+            for (int i = 0; i < kRun; i += 4)
+                *reinterpret_cast<int4*>(a.positions + t0 + i) = make_int4(pos[i], pos[i + 1], pos[i + 2], pos[i + 3]);
+#pragma unroll
+            for (int i = 0; i < kRun; i += 2)
+                *reinterpret_cast<longlong2*>(a.slots + t0 + i) = make_longlong2(slot[i], slot[i + 1]);
         } else {
             for (int i = 0; i < kRun && t0 + i < a.n_tokens; ++i) {
                 a.positions[t0 + i] = pos[i];
@@ -335,9 +337,9 @@ void launch_page_tables(const PageTablesArgs& a, cudaStream_t st) {
     const size_t smem = 3 * ((size_t)a.n_requests + 1) * sizeof(int);
     if (smem > 48 * 1024)
         VGPU_CHECK(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const long long per_block = kScanThreads * 4;
+    const long long per_block = kScanThreads * kRun;
     const long long want = std::max<long long>((a.n_tokens + per_block - 1) / per_block, (a.n_requests + 63) / 64);
-    const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 3);
+    const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 2);
     page_tables_kernel<<<blocks, kScanThreads, smem, st>>>(a);
     VGPU_LAUNCH("page_tables_kernel");
 }

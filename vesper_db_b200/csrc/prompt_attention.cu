@@ -145,6 +145,21 @@ void launch_short(const TileParams& p, bool f16, long long blocks, cudaStream_t 
     }
 }
 
+// A launch that may overlap the end of the stream's last kernel, if that one allows it.
+template <class K, class... Args>
+void launch_ahead(K* kernel, unsigned blocks, unsigned threads, bool ahead, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = ahead ? 1 : 0;
+    VGPU_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 // ---------------------------------------------------------------------------------
 // Pages of a cache with few query rows: each request's own pages, and the prefix when the
 // whole batch has few rows.  Bound by reading keys and values once.
@@ -189,6 +204,7 @@ struct PagesPlan {
     int own_jobs, tiles;  // jobs of own pages: `tiles` of them a request
     int prefix_jobs;      // 0: the prefix is not taken here
     int warps;            // of each key head
+    bool alone;           // the only kernel of the call before the join
     // Results: [slots][kv_heads][8 * NT][dim], their log2-sum-exp, and of each job its first
     // warp and how many warps it has.
     float* o;
@@ -213,6 +229,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
     constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key, of a value row
     constexpr int kThreadsHere = kOwnWarps * 32;
     __shared__ int s_sum[kThreadsHere + 1];
+    if (pl.alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int group = a.heads / a.kv_heads, jobs = pl.own_jobs + pl.prefix_jobs;
     const int warp_all = blockIdx.x * kOwnWarps + (tid >> 5);
@@ -222,7 +239,11 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
     // Blocks before each thread's share of the jobs.
     const int per = (jobs + kThreadsHere - 1) / kThreadsHere;
     int mine = 0;
-    for (int j = tid * per; j < min(jobs, (tid + 1) * per); ++j) mine += blocks_of(j);
+    for (int j = tid * per; j < min(jobs, (tid + 1) * per); ++j) {
+        const int n = blocks_of(j);
+        mine += n;
+        if (n == 0 && blockIdx.x == 0) pl.where[j] = make_int2(0, 0);  // the others' is written with their first block
+    }
     s_sum[tid + 1] = mine;
     if (tid == 0) s_sum[0] = 0;
     __syncthreads();
@@ -488,18 +509,7 @@ void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, bool after_t
     const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
     // After the prefix's tiles: nothing here depends on them, and they leave SMs idle, so
     // the blocks may start as soon as all of the tiles' blocks have.
-    auto launch = [&](auto* kernel) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(blocks);
-        cfg.blockDim = dim3(kOwnWarps * 32);
-        cfg.stream = st;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = after_tiles ? 1 : 0;
-        VGPU_CHECK(cudaLaunchKernelEx(&cfg, kernel, a, pl));
-    };
+    auto launch = [&](auto* kernel) { launch_ahead(kernel, blocks, kOwnWarps * 32, after_tiles, st, a, pl); };
     if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
     else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
     VGPU_LAUNCH("pages_kernel");
@@ -520,7 +530,6 @@ struct JoinArgs {
     bool paged;
     int nt;
     PagesPlan pages;
-    const int32_t* lengths;
     bool own;  // there are own pages
     void* out;
     float* lse;
@@ -530,6 +539,7 @@ template <class H>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs a) {
     const int lane = threadIdx.x & 31;
     const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // no wait unless launched ahead
     if (row >= a.rows) return;
     const bool live = lane * 4 < a.dim;
     // Slots of the row's own job, then of its prefix job.
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
     long long own_at = 0, shared_at = 0;  // rows of slots
     if (a.paged) {
         const int tall = 8 * a.nt;
-        if (a.own && a.lengths[b] > 0) {
+        if (a.own) {
             const int job = b * a.pages.tiles + g / tall;
             const int2 w = a.pages.where[job];
             own = w.y;
@@ -608,10 +618,10 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
     if (a.lse && lane == 0) a.lse[row] = nan ? __int_as_float(0x7fc00000) : (m + log2f(total)) / kLog2e;
 }
 
-void launch_join(bool f16, const JoinArgs& a, cudaStream_t st) {
-    const int blocks = ceil_div(a.rows, 4);
-    if (f16) join_kernel<F16><<<blocks, 128, 0, st>>>(a);
-    else join_kernel<Bf16><<<blocks, 128, 0, st>>>(a);
+// `ahead`: the one kernel whose results are joined is the last one queued, and lets this one
+// be set up while it runs.
+void launch_join(bool f16, const JoinArgs& a, bool ahead, cudaStream_t st) {
+    launch_ahead(f16 ? join_kernel<F16> : join_kernel<Bf16>, (unsigned)ceil_div(a.rows, 4), 128, ahead, st, a);
     VGPU_LAUNCH("join_kernel");
 }
 
@@ -748,7 +758,7 @@ void launch_prompt_attention(const PromptArgs& a, cudaStream_t st) {
     j.tile_lse = p.part_lse;
     j.out = a.out;
     j.lse = a.lse;
-    launch_join(a.f16, j, st);
+    launch_join(a.f16, j, false, st);
 }
 
 size_t shared_attention_workspace(const SharedArgs& a) { return a.n_requests == 0 ? 0 : shared_plan(a).bytes; }
@@ -783,6 +793,7 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
         launch_tiles<true>(p, a.f16, (long long)ceil_div(a.n_requests, 2 * p.tile_tokens) * a.kv_heads * p.splits,
                            static_cast<int*>(a.workspace), st);
     }
+    sp.pages.alone = sp.splits == 0 && sp.pages.own_jobs + sp.pages.prefix_jobs > 0;
     sp.pages.o = base + sp.slots_at;
     sp.pages.lse = base + sp.slot_lse_at;
     sp.pages.where = reinterpret_cast<int2*>(base + sp.where_at);
@@ -791,11 +802,10 @@ void launch_shared_attention(const SharedArgs& a, cudaStream_t st) {
     j.paged = true;
     j.nt = sp.nt;
     j.pages = sp.pages;
-    j.lengths = a.lengths;
     j.own = sp.pages.own_jobs > 0;
     j.out = a.out;
     j.lse = a.lse;
-    launch_join(a.f16, j, st);
+    launch_join(a.f16, j, sp.pages.alone, st);
 }
 
 }  // namespace vgpu
