@@ -147,10 +147,11 @@ void launch_short(const TileParams& p, bool f16, long long blocks, cudaStream_t 
 
 // A launch that may overlap the end of the stream's last kernel, if that one allows it.
 template <class K, class... Args>
-void launch_ahead(K* kernel, unsigned blocks, unsigned threads, bool ahead, cudaStream_t st, const Args&... args) {
+void launch_ahead(K* kernel, unsigned blocks, unsigned threads, int smem, bool ahead, cudaStream_t st, const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -175,17 +176,18 @@ void launch_ahead(K* kernel, unsigned blocks, unsigned threads, bool ahead, cuda
 //
 // The products are m16n8k16 steps of one warp, S^T = K Q^T (16 keys by 8 rows) and
 // O^T = V^T P^T (16 values by 8 rows): with the rows on the short side few of them waste
-// little.  Operands go from global memory to registers in 16-byte loads, without a stop in
-// shared memory:
+// little.  Each warp copies its blocks into shared-memory stages of its own, two blocks ahead
+// (asynchronous copies: what is in flight costs no registers; with the next block in registers
+// instead, 175 MB took 40 us), and reads operands from there in 16-byte pieces:
 //   * keys: the order of the contraction index is free, so lane (g, t) = (lane / 4,
-//     lane % 4) holds chunks t, t + 4, ... (eight values each) of keys g and g + 8, and the
+//     lane % 4) takes chunks t, t + 4, ... (eight values each) of keys g and g + 8, and the
 //     queries are laid out the same way;
-//   * values: the order of the output rows is free, so lane (g, t) holds chunks g and g + 8
+//   * values: the order of the output rows is free, so lane (g, t) takes chunks g and g + 8
 //     of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and rows g and g + 8 of step (i, e) are values e
 //     and e + 4 of chunk 8 i + g: one byte permutation makes each operand register;
 //   * probabilities: one 8 x 8 transposition between registers turns S^T into P^T.
-// The next keys are loaded while the scores become probabilities, the next values while
-// the next scores are made, the page number after that one block earlier still.
+// Chunk c of row r stands at c ^ (r & 6) ^ 4 (r & 1): both ways of reading then take eight
+// different bank groups at a time.
 // ---------------------------------------------------------------------------------
 constexpr int kOwnWarps = 4;
 
@@ -199,6 +201,7 @@ __device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 
 
 constexpr int kBlockKeys = 16;
 constexpr int kMinRange = 2;  // blocks a warp takes at least
+constexpr int kStages = 3;
 
 struct PagesPlan {
     int own_jobs, tiles;  // jobs of own pages: `tiles` of them a request
@@ -223,7 +226,7 @@ __device__ __forceinline__ int job_keys(const SharedArgs& a, const PagesPlan& pl
 }
 
 template <class H, int D, int NT>
-__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 && D == 64 ? 4 : 2)
     pages_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ PagesPlan pl) {
     using T = typename H::type;
     constexpr int KC = D / 32, VC = D / 64;  // chunks a lane holds of a key, of a value row
@@ -298,53 +301,39 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
         return c.job >= pl.own_jobs ? a.prefix_pages[i] : a.table[(long long)(c.job / pl.tiles) * a.table_stride + i];
     };
     const int mask = (1 << a.page_shift) - 1;
-    uint4 kf[2][KC], vf[4][VC];
-    // 16 keys lie in one page.  Rows past the job's keys are not read: they may hold anything.
-    // Whole blocks of whole rows take the short way: no test a load, no zeros beforehand.
-    const bool whole = a.dim == D;
-    const T* const k_lane = static_cast<const T*>(a.k_cache.p) + kh * a.k_cache.head + g * a.k_cache.tok + t * 8;
-    const T* const v_lane = static_cast<const T*>(a.v_cache.p) + kh * a.v_cache.head + 2 * t * a.v_cache.tok + g * 8;
-    const long long k_rows = 8 * a.k_cache.tok, v_row = a.v_cache.tok, v_rows = 8 * a.v_cache.tok;
-    auto left_of = [&](const Cursor& c, int pg) {  // keys of the block that are there
-        return pg >= 0 && pg < a.n_pages && c.at < end ? c.keys - c.block * kBlockKeys : 0;
-    };
-    auto load_k = [&](const Cursor& c, int pg) {
-        const int left = left_of(c, pg);
-        const T* p = k_lane + pg * a.k_cache.page + ((c.block * kBlockKeys) & mask) * a.k_cache.tok;
-        if (whole && left >= kBlockKeys) {
+    // Stages of this warp: 16 rows of keys, 16 of values.  16 keys lie in one page; rows past
+    // the job's keys are filled with zeros, nothing is read for them.
+    extern __shared__ __align__(128) uint8_t stages[];
+    constexpr int kChunks = D / 8, kRowBytes = D * 2, kHalf = kBlockKeys * kRowBytes;
+    constexpr int kRowStep = 32 / kChunks;  // rows a pass of the warp copies
+    const uint32_t stage0 = tc::smem_u32(stages) + (tid >> 5) * kStages * 2 * kHalf;
+    auto place = [](int row, int chunk) { return row * kRowBytes + ((chunk ^ (row & 6) ^ ((row & 1) << 2)) << 4); };
+    const int chunk = lane % kChunks, row0 = lane / kChunks;
+    const bool here = chunk * 8 < a.dim;
+    const T* const k_lane = static_cast<const T*>(a.k_cache.p) + kh * a.k_cache.head + row0 * a.k_cache.tok + (here ? chunk * 8 : 0);
+    const T* const v_lane = static_cast<const T*>(a.v_cache.p) + kh * a.v_cache.head + row0 * a.v_cache.tok + (here ? chunk * 8 : 0);
+    const long long k_step = kRowStep * a.k_cache.tok, v_step = kRowStep * a.v_cache.tok;
+    auto request = [&](const Cursor& c, int pg, int stage) {
+        const int first = c.block * kBlockKeys;
+        const int left = pg >= 0 && pg < a.n_pages && c.at < end && here ? c.keys - first - row0 : 0;
+        const T* kp = k_lane + pg * a.k_cache.page + (first & mask) * a.k_cache.tok;
+        const T* vp = v_lane + pg * a.v_cache.page + (first & mask) * a.v_cache.tok;
+        const uint32_t dst = stage0 + stage * 2 * kHalf;
 #pragma unroll
-            for (int r = 0; r < 2; ++r, p += k_rows)
-#pragma unroll
-                for (int i = 0; i < KC; ++i) kf[r][i] = __ldcs(reinterpret_cast<const uint4*>(p + i * 32));
-            return;
+        for (int i = 0; i < kBlockKeys / kRowStep; ++i) {
+            const bool some = i * kRowStep < left;
+            const uint32_t at = dst + place(row0 + i * kRowStep, chunk);
+            attn::copy16(at, some ? static_cast<const void*>(kp) : a.k_cache.p, some);
+            attn::copy16(at + kHalf, some ? static_cast<const void*>(vp) : a.v_cache.p, some);
+            kp += k_step;
+            vp += v_step;
         }
-#pragma unroll
-        for (int r = 0; r < 2; ++r, p += k_rows)
-#pragma unroll
-            for (int i = 0; i < KC; ++i) {
-                kf[r][i] = make_uint4(0, 0, 0, 0);
-                if ((i * 4 + t) * 8 < a.dim && r * 8 + g < left) kf[r][i] = *reinterpret_cast<const uint4*>(p + i * 32);
-            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto load_v = [&](const Cursor& c, int pg) {
-        const int left = left_of(c, pg);
-        const T* p = v_lane + pg * a.v_cache.page + ((c.block * kBlockKeys) & mask) * a.v_cache.tok;
-        if (whole && left >= kBlockKeys) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int i = 0; i < VC; ++i)
-                    vf[r][i] = __ldcs(reinterpret_cast<const uint4*>(p + (r & 1) * v_row + (r >> 1) * v_rows + i * 64));
-            return;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < VC; ++i) {
-                vf[r][i] = make_uint4(0, 0, 0, 0);
-                if ((i * 8 + g) * 8 < a.dim && 2 * t + (r & 1) + (r >> 1) * 8 < left)
-                    vf[r][i] = *reinterpret_cast<const uint4*>(p + (r & 1) * v_row + (r >> 1) * v_rows + i * 64);
-            }
+    auto piece = [&](uint32_t base, int row, int ch) {
+        uint4 u;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(base + place(row, ch)));
+        return u;
     };
     // Rows of a job: row r is query head kh * group + (m0 + r) % group of request
     // b + (m0 + r) / group.
@@ -418,11 +407,14 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
         clear();
     };
 
-    Cursor next = after(cur);
-    int pg = page_of(cur), pg_next = page_of(next);
+    Cursor next = after(cur), then = after(next);
+    {
+        const int pg0 = page_of(cur), pg1 = page_of(next);
+        request(cur, pg0, 0);
+        request(next, pg1, 1);
+    }
+    int pg = page_of(then), stage = 0;
     load_q(cur.job);
-    load_k(cur, pg);
-    load_v(cur, pg);
     clear();
     const float scale = a.scale * kLog2e;
     while (true) {
@@ -430,21 +422,27 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
             const int last = cur.at + (cur.keys + kBlockKeys - 1) / kBlockKeys - 1;
             pl.where[cur.job] = make_int2(warp, last / range - warp + 1);
         }
+        __syncwarp();  // every lane is done with the stage that is filled next
+        request(then, pg, stage == 0 ? 2 : stage - 1);
+        const Cursor last = after(then);
+        pg = page_of(last);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();
+        const uint32_t sk = stage0 + stage * 2 * kHalf, sv = sk + kHalf;
         float s[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < KC; ++i) {
-                attn::mma16816<H>(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qb[nt][2 * i][0], qb[nt][2 * i][1]);
-                attn::mma16816<H>(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
+        for (int i = 0; i < KC; ++i) {
+            const uint4 lo = piece(sk, g, i * 4 + t), hi = piece(sk, g + 8, i * 4 + t);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                attn::mma16816<H>(s[nt], lo.x, hi.x, lo.y, hi.y, qb[nt][2 * i][0], qb[nt][2 * i][1]);
+                attn::mma16816<H>(s[nt], lo.z, hi.z, lo.w, hi.w, qb[nt][2 * i + 1][0], qb[nt][2 * i + 1][1]);
             }
         }
         const bool ends = next.at >= end || next.job != cur.job;
-        load_k(next, pg_next);
         if (next.at < end && next.job != cur.job) load_q(next.job);
-        const Cursor then = after(next);
-        const int pg_then = page_of(then);
         const int key = cur.block * kBlockKeys + g;
         uint32_t pb[NT][2];
 #pragma unroll
@@ -483,24 +481,29 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 3 : 2)
             }
         }
 #pragma unroll
-        for (int i = 0; i < VC; ++i)
+        for (int i = 0; i < VC; ++i) {
+            uint4 vf[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vf[r] = piece(sv, 2 * t + (r & 1) + (r >> 1) * 8, i * 8 + g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-                const uint32_t a0 = __byte_perm(word(vf[0][i], e / 2), word(vf[1][i], e / 2), sel);
-                const uint32_t a1 = __byte_perm(word(vf[0][i], e / 2 + 2), word(vf[1][i], e / 2 + 2), sel);
-                const uint32_t a2 = __byte_perm(word(vf[2][i], e / 2), word(vf[3][i], e / 2), sel);
-                const uint32_t a3 = __byte_perm(word(vf[2][i], e / 2 + 2), word(vf[3][i], e / 2 + 2), sel);
+                const uint32_t a0 = __byte_perm(word(vf[0], e / 2), word(vf[1], e / 2), sel);
+                const uint32_t a1 = __byte_perm(word(vf[0], e / 2 + 2), word(vf[1], e / 2 + 2), sel);
+                const uint32_t a2 = __byte_perm(word(vf[2], e / 2), word(vf[3], e / 2), sel);
+                const uint32_t a3 = __byte_perm(word(vf[2], e / 2 + 2), word(vf[3], e / 2 + 2), sel);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) attn::mma16816<H>(o[nt][i][e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
-        load_v(next, pg_next);
+        }
         if (ends) flush(cur.job);
         if (next.at >= end) break;
         cur = next;
         next = then;
-        pg_next = pg_then;
+        then = last;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <class H>
@@ -509,7 +512,11 @@ void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, bool after_t
     const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
     // After the prefix's tiles: nothing here depends on them, and they leave SMs idle, so
     // the blocks may start as soon as all of the tiles' blocks have.
-    auto launch = [&](auto* kernel) { launch_ahead(kernel, blocks, kOwnWarps * 32, after_tiles, st, a, pl); };
+    const int smem = kOwnWarps * kStages * 2 * kBlockKeys * (a.dim <= 64 ? 64 : 128) * 2;
+    auto launch = [&](auto* kernel) {
+        VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        launch_ahead(kernel, blocks, kOwnWarps * 32, smem, after_tiles, st, a, pl);
+    };
     if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
     else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
     VGPU_LAUNCH("pages_kernel");
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
 // `ahead`: the one kernel whose results are joined is the last one queued, and lets this one
 // be set up while it runs.
 void launch_join(bool f16, const JoinArgs& a, bool ahead, cudaStream_t st) {
-    launch_ahead(f16 ? join_kernel<F16> : join_kernel<Bf16>, (unsigned)ceil_div(a.rows, 4), 128, ahead, st, a);
+    launch_ahead(f16 ? join_kernel<F16> : join_kernel<Bf16>, (unsigned)ceil_div(a.rows, 4), 128, 0, ahead, st, a);
     VGPU_LAUNCH("join_kernel");
 }
 
@@ -687,8 +694,8 @@ SharedPlan shared_plan(const SharedArgs& a) {
     // as many warps as are resident at once, and no more than the keys can use
     const long long cap = (((long long)a.table_width << a.page_shift) + kBlockKeys - 1) / kBlockKeys;
     const long long most = p.pages.own_jobs * cap + p.pages.prefix_jobs * ((a.prefix_len + kBlockKeys - 1) / kBlockKeys);
-    // (four times that after the tiles: their SMs come free one by one)
-    const long long resident = (long long)kSms * (p.nt == 1 ? 3 : 2) * kOwnWarps * (p.splits ? 4 : 1) / a.kv_heads;
+    // (twice that after the tiles: their SMs come free one by one)
+    const long long resident = (long long)kSms * (p.nt == 1 && a.dim <= 64 ? 4 : 2) * kOwnWarps * (p.splits ? 2 : 1) / a.kv_heads;
     p.pages.warps = (int)std::max<long long>(1, std::min<long long>(resident, (most + kMinRange - 1) / kMinRange));
     const size_t slot_rows = jobs ? (size_t)(jobs + p.pages.warps) * a.kv_heads * tall : 0;
     p.slots_at = (size_t)p.splits * rows * a.dim;
