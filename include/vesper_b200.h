@@ -412,8 +412,8 @@ VESPER_C_API vesper_status_t vesper_flat_get_last_timings(vesper_flat_timings_t*
  * dtype VESPER_BF16 or VESPER_F16; arithmetic is in 32 bits with one rounding at the
  * output, but the attention probabilities are rounded to dtype before they meet the
  * values (the sums they are divided by are not).
- * Strides are in elements.  Data pointers are 16-byte aligned, strides multiples of 8
- * elements, and the last dimension is contiguous.  page_size is a power of two from 16
+ * Strides are in elements.  Data pointers are 16-byte aligned, strides positive multiples
+ * of 8 elements, and the last dimension is contiguous.  page_size is a power of two from 16
  * to 256.  heads is a multiple of kv_heads, at most 128 times of it; query head h reads
  * key head h / (heads / kv_heads).
  * Refusals return VESPER_ERROR_INVALID_PARAM with a message, before any work is queued.

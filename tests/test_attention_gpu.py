@@ -647,3 +647,11 @@ def test_calls_with_addresses(V):
                   torch.cuda.current_stream().cuda_stream)
     assert torch.equal(out, V.prompt_attention(q, k, v, st))
     refused("scale", lambda: A.call_device("prompt_attention", [0, 2, 70, 70, 4, 2, 64, 1, -1.0] + [0] * 15))
+
+
+def test_expanded_tensors_are_refused(V):
+    q, k = rand(5, 8, 64), rand(5, 1, 64).expand(5, 2, 64)
+    refused("strides", lambda: V.prompt_attention(q, k, k, ints([0, 5])))
+    refused("strides", lambda: V.norm_rotate(q, k, None, ints([0] * 5), torch.zeros(9, 64, device="cuda")))
+    one = rand(1, 8, 64).expand(1, 8, 64)  # a single element's stride does not matter
+    assert V.prompt_attention(one, one[:, :2], one[:, :2], ints([0, 1])).shape == (1, 8, 64)

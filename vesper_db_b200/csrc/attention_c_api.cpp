@@ -52,7 +52,7 @@ constexpr size_t kMaxInt = 0x7fffffff;
 constexpr size_t kMaxStride = (size_t)1 << 38;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool stride_ok(size_t s) { return s % 8 == 0 && s < kMaxStride; }
+bool stride_ok(size_t s) { return s > 0 && s % 8 == 0 && s < kMaxStride; }
 
 int page_shift_of(size_t page_size) {
     int s = 4;

@@ -1,6 +1,7 @@
 // Attention over packed prompts, and over a shared prefix joined with each request's own
 // pages: launchers, the kernel of the own pages, and the join of partial results.
 #include <algorithm>
+#include <atomic>
 
 #include "attention.cuh"
 #include "attn_short.cuh"
@@ -81,20 +82,30 @@ void fill_queries(TileParams& p, bool f16, const HeadsView& q, int heads, int kv
                     {64, p.group, 1, p.tile_tokens});
 }
 
+// Opts a kernel in to its dynamic shared memory, once a device; `more` runs with it.
+template <class K, class F>
+void opt_in(std::atomic<uint64_t>& devices, K* kernel, int smem, F&& more) {
+    int dev = 0;
+    VGPU_CHECK(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (devices.load(std::memory_order_relaxed) & bit) return;
+    VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    more();
+    devices.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <class H, int D, bool PAGED>
 void launch_tiles_as(const TileParams& p, unsigned blocks, cudaStream_t st) {
     auto* kernel = attn::attn_tile_kernel<H, D, PAGED>;
     constexpr int smem = attn::smem_bytes<D>();
-    static const bool ready = [&] {
-        VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> devices{0};
+    opt_in(devices, kernel, smem, [&] {
         cudaFuncAttributes fa;
         VGPU_CHECK(cudaFuncGetAttributes(&fa, kernel));
         // the softmax warps' registers come out of what the block is launched with
         if (fa.numRegs * kThreads < attn::kSoftmaxWarps * 32 * attn::kSoftmaxRegs + 128 * attn::kServiceRegs)
             throw CudaError("attn_tile_kernel: launched with too few registers for its split");
-        return true;
-    }();
-    (void)ready;
+    });
     kernel<<<blocks, kThreads, smem, st>>>(p);
     VGPU_LAUNCH("attn_tile_kernel");
 }
@@ -125,11 +136,8 @@ void launch_tiles(TileParams p, bool f16, long long items, int* counter, cudaStr
 template <class H, int D>
 void launch_short_as(const TileParams& p, long long blocks, cudaStream_t st) {
     constexpr int smem = attn::short_smem_bytes<D>();
-    static const bool ready = [&] {
-        VGPU_CHECK(cudaFuncSetAttribute(attn::attn_short_kernel<H, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        return true;
-    }();
-    (void)ready;
+    static std::atomic<uint64_t> devices{0};
+    opt_in(devices, attn::attn_short_kernel<H, D>, smem, [] {});
     attn::attn_short_kernel<H, D><<<(unsigned)blocks, attn::kShortThreads, smem, st>>>(p);
     VGPU_LAUNCH("attn_short_kernel");
 }
@@ -506,20 +514,28 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 && D == 64 ? 4 : 2)
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
+template <class H, int D, int NT>
+void launch_pages_as(const SharedArgs& a, const PagesPlan& pl, unsigned blocks, bool after_tiles, cudaStream_t st) {
+    constexpr int smem = kOwnWarps * kStages * 2 * kBlockKeys * D * 2;
+    static std::atomic<uint64_t> devices{0};
+    opt_in(devices, pages_kernel<H, D, NT>, smem, [] {});
+    launch_ahead(pages_kernel<H, D, NT>, blocks, kOwnWarps * 32, smem, after_tiles, st, a, pl);
+    VGPU_LAUNCH("pages_kernel");
+}
+
 template <class H>
 void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, bool after_tiles, cudaStream_t st) {
     if (pl.own_jobs + pl.prefix_jobs == 0) return;
     const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
     // After the prefix's tiles: nothing here depends on them, and they leave SMs idle, so
     // the blocks may start as soon as all of the tiles' blocks have.
-    const int smem = kOwnWarps * kStages * 2 * kBlockKeys * (a.dim <= 64 ? 64 : 128) * 2;
-    auto launch = [&](auto* kernel) {
-        VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        launch_ahead(kernel, blocks, kOwnWarps * 32, smem, after_tiles, st, a, pl);
-    };
-    if (a.dim <= 64) launch(nt == 1 ? pages_kernel<H, 64, 1> : pages_kernel<H, 64, 2>);
-    else launch(nt == 1 ? pages_kernel<H, 128, 1> : pages_kernel<H, 128, 2>);
-    VGPU_LAUNCH("pages_kernel");
+    if (a.dim <= 64) {
+        if (nt == 1) launch_pages_as<H, 64, 1>(a, pl, blocks, after_tiles, st);
+        else launch_pages_as<H, 64, 2>(a, pl, blocks, after_tiles, st);
+    } else {
+        if (nt == 1) launch_pages_as<H, 128, 1>(a, pl, blocks, after_tiles, st);
+        else launch_pages_as<H, 128, 2>(a, pl, blocks, after_tiles, st);
+    }
 }
 
 // ---------------------------------------------------------------------------------
