@@ -218,14 +218,12 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
         if (!valid[h]) continue;
         const float inv = l[h] > 0.0f ? 1.0f / l[h] : (l[h] == 0.0f ? 0.0f : l[h]);
         T* const dst = static_cast<T*>(p.out) + out_row[h] * p.dim;
-        if (!leak) {
+        if (!leak) {  // through the warp's own part of the stages: whole rows are stored below
+            const int r = warp * 16 + g + 8 * h;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-                const int d = i * 8 + 2 * t;
-                if (d < p.dim) {
-                    const float x = l[h] == 0.0f ? 0.0f : o[i][2 * h] * inv, y = l[h] == 0.0f ? 0.0f : o[i][2 * h + 1] * inv;
-                    *reinterpret_cast<uint32_t*>(dst + d) = H::pack(x, y);
-                }
+                const float x = l[h] == 0.0f ? 0.0f : o[i][2 * h] * inv, y = l[h] == 0.0f ? 0.0f : o[i][2 * h + 1] * inv;
+                *reinterpret_cast<uint32_t*>(smem + r * kRowBytes + ((i ^ (r & 7)) << 4) + t * 4) = H::pack(x, y);
             }
         } else {
             // One key at a time, with the maximum and sum that the scores gave; a lane of the
@@ -257,6 +255,15 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
             }
         }
         if (p.lse && t == 0) p.lse[out_row[h]] = (m[h] + log2f(l[h])) * 0.6931471805599453f;
+    }
+    if (leak) return;
+    __syncwarp();
+#pragma unroll
+    for (int e = lane; e < 16 * kChunks; e += 32) {
+        const int r = warp * 16 + e / kChunks, c = e % kChunks, tok = r / p.group, head = kh * p.group + r - tok * p.group;
+        if (tok < tokens && c * 8 < p.dim)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((long long)(w.q0 + tok) * p.heads + head) * p.dim + c * 8) =
+                *reinterpret_cast<const uint4*>(smem + r * kRowBytes + ((c ^ (r & 7)) << 4));
     }
 }
 

@@ -89,7 +89,7 @@ struct TileParams {
 
 template <int D>
 constexpr int smem_bytes() {
-    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512 + 2 * 2 * 2 * kRows * 4;
+    return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512 + 2 * 2 * 2 * kRows * 4 + kSoftmaxWarps * 1024;
 }
 
 // Bounded wait for the barrier's phase; false when it ran out (a tile takes microseconds).
@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(s_leak + kAhead);
     // Rows' maxima (and sums) of each half of the keys: [turn][tile][half][row]
     float* const s_half = reinterpret_cast<float*>(bars + 64);
+    const uint32_t s_stage = tc::smem_u32(s_half + 2 * 2 * 2 * kRows);  // 1 KB a softmax warp, for the results
     static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + kAhead * (sizeof(Work) + 4) + 4 <= 512, "");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -719,32 +720,91 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
         using T = typename H::type;
         if (!leak) {
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[16];
-                if (my_tiles > 0) {
-                    tmem_ld16(to + c * 16, o);
-                    tc::tmem_ld_wait();
-                } else {
+            // A thread has part of one row, rows lie heads * dim apart: stored from here, each
+            // 16 bytes are a line of their own (3,000 cycles a piece with heads of 64, 6,000 with
+            // 128).  So a warp passes its rows through 1 KB of shared memory, a few at a time, and
+            // stores each row's part in one go.
+            const uint32_t stage = s_stage + warp * 1024;
+            auto scaled = [&](uint32_t o) { return l == 0.0f ? 0.0f : __uint_as_float(o) * inv; };
+            // kRowsAt rows of kPieces 16-byte pieces; `piece` gives this lane's, `put` stores one
+            // of the row of another lane.
+            auto through = [&](auto pieces, auto&& piece, auto&& put) {
+                constexpr int kPieces = decltype(pieces)::value, kRowsAt = 64 / kPieces;
+                const int mine = lane % kRowsAt;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = 0;
-                }
+                for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
+                    __syncwarp();
+                    if (lane / kRowsAt == r0 / kRowsAt)
 #pragma unroll
-                for (int i = 0; i < 16; i += 8) {
-                    const int d = half * (D / 2) + c * 16 + i;
-                    if (!valid || d >= p.dim) continue;
-                    float x[8];
+                        for (int i = 0; i < kPieces; ++i) {
+                            const uint4 u = piece(i);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                                             stage + (mine * kPieces + (i ^ (mine & 7 & (kPieces - 1)))) * 16),
+                                         "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
+                                         : "memory");
+                        }
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : __uint_as_float(o[i + e]) * inv;
-                    if (part) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + at) * p.dim + d);
-                        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-                        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-                    } else {
-                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + d) = pack8<H>(x);
+                    for (int e = lane; e < 64; e += 32) {
+                        const int r = e / kPieces, i = e % kPieces;
+                        uint4 u;
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                     : "r"(stage + (r * kPieces + (i ^ (r & 7 & (kPieces - 1)))) * 16)
+                                     : "memory");
+                        const long long row_at = __shfl_sync(0xffffffffu, at, r0 + r);
+                        if (__shfl_sync(0xffffffffu, (int)valid, r0 + r)) put(row_at, i, u);
                     }
                 }
-                __syncwarp();
+            };
+            if (!part) {
+                uint32_t pk[D / 4];
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[16];
+                    if (my_tiles > 0) {
+                        tmem_ld16(to + c * 16, o);
+                        tc::tmem_ld_wait();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pk[c * 8 + i] = H::pack(scaled(o[2 * i]), scaled(o[2 * i + 1]));
+                }
+                through(std::integral_constant<int, D / 16>{},
+                        [&](int i) { return make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]); },
+                        [&](long long row_at, int i, const uint4& u) {
+                            const int d = half * (D / 2) + i * 8;
+                            if (d < p.dim) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row_at * p.dim + d) = u;
+                        });
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < D / 64; ++c) {  // 32 values at a time
+                    uint32_t o[2][16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (my_tiles > 0) {
+                            tmem_ld16(to + c * 32 + h * 16, o[h]);
+                            tc::tmem_ld_wait();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[h][i] = 0;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[h][i] = __float_as_uint(scaled(o[h][i]));
+                    }
+                    through(std::integral_constant<int, 8>{},
+                            [&](int i) {
+                                const uint32_t* e = &o[i >> 2][(i & 3) * 4];
+                                return make_uint4(e[0], e[1], e[2], e[3]);
+                            },
+                            [&](long long row_at, int i, const uint4& u) {
+                                const int d = half * (D / 2) + c * 32 + i * 4;
+                                if (d < p.dim)
+                                    *reinterpret_cast<uint4*>(p.part_o + (w.split * rows + row_at) * p.dim + d) = u;
+                            });
+                }
             }
         } else if (valid) {
             // One key at a time, eight output values a pass, with the maximum and sum that the
