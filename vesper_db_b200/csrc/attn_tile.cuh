@@ -628,16 +628,59 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             const bool valid = row_tok < (t ? x.tok1 : x.tok0);
             const int lim = valid ? min(max(w.first_lim + w.step * (t * tt + row_tok), 0), w.len_k) : w.len_k;
             const int tile_lim = min(max(w.first_lim + w.step * t * tt, 0), w.len_k);  // the tile's first row's
+            // Keys that some row of the warp sees, at most; a warp without rows makes no
+            // probabilities (what stands in its lanes only reaches results that are not stored).
+            const bool idle = !__any_sync(0xffffffffu, valid);
+            const int warp_lim = __reduce_max_sync(0xffffffffu, valid ? lim : 0);
             float m = -INFINITY, l = 0.0f;
+            // Moves the reference m to a row's new maximum where it has grown too far.  Each of the
+            // two warps of a row sees the same values, and rescales half of O.
+            auto settle = [&](float top, bool first) {
+                if (first) {
+                    m = top == INFINITY ? __int_as_float(0x7fc00000) : top;
+                } else if (__any_sync(0xffffffffu, !(top - m <= kGrow))) {
+                    // grown, or NaN (a score is NaN or infinite, or the row has seen no key)
+                    float up = !(top - m <= kGrow) ? top : m;
+                    if (up == INFINITY) up = __int_as_float(0x7fc00000);
+                    const float f = m == up ? 1.0f : ex2(m - up);
+                    m = up;
+                    l *= f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c * 16, o);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(to + c * 16, o);
+                    }
+                }
+            };
         for (int j = 0; j < my_tiles; ++j) {
             // after a wait that ran out the row's warps only keep meeting
             wait(&s_full[t], tiles++ & 1);
             tc::fence_after_sync();
+            const int key = (j0 + j) * kKeys + half * 64;
+            if (key >= warp_lim) {  // no row of the warp sees these keys: P is zero
+                const float top = exchange(-INFINITY) * p.scale_log2;
+                if (!idle) {
+                    settle(top, j == 0);
+                    uint32_t zero[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) zero[i] = 0;
+                    tmem_st16(ts + half * 32, zero);
+                    tmem_st16(ts + half * 32 + 16, zero);
+                    tc::tmem_st_wait();
+                    tc::fence_before_sync();
+                }
+                tc::mbar_arrive(&p_full[2 * t]);
+                tc::mbar_arrive(&p_full[2 * t + 1]);
+                continue;
+            }
             uint32_t s[2][32];
             tc::tmem_ld32(ts + half * 64, s[0]);
             tc::tmem_ld32(ts + half * 64 + 32, s[1]);
             tc::tmem_ld_wait();
-            const int key = (j0 + j) * kKeys + half * 64;
             if (key + 64 > tile_lim) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
@@ -657,26 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
             // also: both halves of S are in registers after this, and P may take their place
             top = fmaxf(top, exchange(top)) * p.scale_log2;
-            if (j == 0) {
-                m = top == INFINITY ? __int_as_float(0x7fc00000) : top;
-            } else if (__any_sync(0xffffffffu, !(top - m <= kGrow))) {
-                // Grown too far, or NaN (a score is NaN or infinite, or the row has seen no key).
-                // Each of the two warps sees the same values, and rescales half of O.
-                float up = !(top - m <= kGrow) ? top : m;
-                if (up == INFINITY) up = __int_as_float(0x7fc00000);
-                const float f = m == up ? 1.0f : ex2(m - up);
-                m = up;
-                l *= f;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[16];
-                    tmem_ld16(to + c * 16, o);
-                    tc::tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tmem_st16(to + c * 16, o);
-                }
-            }
+            settle(top, j == 0);
             const float ref = m == -INFINITY ? 0.0f : m;
             const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
             uint64_t ref2 = pair(-ref, -ref);
