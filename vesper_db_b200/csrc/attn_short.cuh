@@ -1,7 +1,7 @@
 // Attention of short prompts: the same rows and masks as attn_tile.cuh, in small blocks.
 //
 // A prompt of a few hundred tokens gives a tensor-memory tile little to overlap: setting it
-// up and draining it takes 8 us of an SM that holds one block.  Here a block is four warps of
+// up and draining it costs an SM that holds one block more than the products do.  Here a block is four warps of
 // 16 rows (64 / group tokens with the query heads of one key head), takes the keys 64 at a
 // time through two shared-memory stages filled by asynchronous copies, multiplies with
 // m16n8k16 steps of each warp, and an SM holds three or more such blocks.
@@ -12,6 +12,10 @@
 // the last key are filled with zeros by the copy; where a later token of the same prompt holds
 // a non-finite value (checked on the diagonal tiles) the block recomputes its rows one key at
 // a time.
+//
+// Bound by the latency of one block: loads, two products and the softmax of a few key tiles.
+// Measured: three prompts of 61 tokens in all (32 + 8 heads of 128, causal): 6.1 us; both
+// kernels side by side at other sizes stand where one of them is chosen.
 #pragma once
 
 #include "attn_tile.cuh"
