@@ -277,7 +277,16 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 && D == 64 ? 4 : 2)
     __syncthreads();
     const int all = s_sum[kThreadsHere], range = max(kMinRange, (all + pl.warps - 1) / pl.warps);
     const int begin = (int)min((long long)warp * range, (long long)all), end = min(all, begin + range);
-    if (warp >= pl.warps || begin >= end) return;
+    // Behind the prefix's tiles this grid starts before they end, and the join is ordered behind
+    // this grid alone: it must not end before the tiles have.  One block that waits at its end
+    // is enough for that; the others make room for the next ones.
+    auto leave = [&] {
+        if (blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
+    };
+    if (warp >= pl.warps || begin >= end) {
+        leave();
+        return;
+    }
 
     // The job of the warp's first block: the share that holds it, then the job in the share.
     Cursor cur;
@@ -514,6 +523,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 && D == 64 ? 4 : 2)
         stage = stage == kStages - 1 ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    leave();
 }
 
 template <class H, int D, int NT>
@@ -530,7 +540,7 @@ void launch_pages(const SharedArgs& a, const PagesPlan& pl, int nt, bool after_t
     if (pl.own_jobs + pl.prefix_jobs == 0) return;
     const unsigned blocks = (unsigned)ceil_div((long long)pl.warps * a.kv_heads, kOwnWarps);
     // After the prefix's tiles: nothing here depends on them, and they leave SMs idle, so
-    // the blocks may start as soon as all of the tiles' blocks have.
+    // the blocks may start as soon as all of the tiles' blocks have; the last one ends after them.
     if (a.dim <= 64) {
         if (nt == 1) launch_pages_as<H, 64, 1>(a, pl, blocks, after_tiles, st);
         else launch_pages_as<H, 64, 2>(a, pl, blocks, after_tiles, st);
