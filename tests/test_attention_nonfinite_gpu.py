@@ -1,0 +1,80 @@
+"""Keys and values that are not finite: they reach the rows that see them, and no other row, wherever they stand."""
+import math
+
+import pytest
+import torch
+
+from conftest import ROOT  # noqa: F401
+from test_attention_gpu import assert_near, rand, row_reference, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def V():
+    import vesper_db_b200
+    return vesper_db_b200
+
+
+def poisoned_call(V, *args, **kw):
+    """The call with outputs and workspaces in memory that holds NaN: what is not written shows."""
+    sizes = [t.numel() * t.element_size() for t in V.prompt_attention(*args, stats=True, **kw)]
+    held = [torch.full((n // 4 + 1,), math.nan, device="cuda") for n in (*sizes, *sizes, 1 << 20)]
+    del held
+    return V.prompt_attention(*args, stats=True, **kw)
+
+
+def check(V, q, k, v, lens, lens_k, causal=True, rows=None):
+    """Every column of the rows (of each request: `rows`, or all) against the formula in 64 bits: where a row sees values
+    that are not finite, their sum; elsewhere the finite ones', which the others must not have touched."""
+    heads, kv, d = q.shape[1], k.shape[1], q.shape[2]
+    out, lse = poisoned_call(V, q, k, v, starts_of(lens), None if lens_k is None else starts_of(lens_k), causal=causal)
+    a = b = 0
+    for n, m in zip(lens, lens if lens_k is None else lens_k):
+        for r0 in range(0, n, 512):
+            r1 = min(n, r0 + 512)
+            if rows is not None and not any(r0 <= r < r1 for r in rows):
+                continue
+            row, col = torch.arange(r0, r1, device="cuda")[:, None], torch.arange(m, device="cuda")[None]
+            seen = (col <= row + m - n) if causal else (col < m).expand(r1 - r0, m)
+            vals = v[b:b + m].double()
+            finite = torch.isfinite(vals)
+            o, l, err, lse_err = row_reference(q[a + r0:a + r1], k[b:b + m], torch.where(finite, vals, 0.0).to(v.dtype), seen,
+                                               d ** -0.5, q.dtype)
+            count = lambda x: torch.einsum("qk,khd->qhd", seen.double(), x.double()).repeat_interleave(heads // kv, 1)  # noqa: E731
+            up, down, nan = (count(vals == math.inf) > 0, count(vals == -math.inf) > 0, count(vals.isnan()) > 0)
+            got = out[a + r0:a + r1]
+            assert_near(torch.where(up | down | nan, 0.0, got), torch.where(up | down | nan, 0.0, o), err, f"rows {r0}..{r1}")
+            assert got[nan | (up & down)].isnan().all()
+            assert (got[up & ~down & ~nan] == math.inf).all() and (got[down & ~up & ~nan] == -math.inf).all()
+            assert_near(lse[a + r0:a + r1], l, lse_err, f"lse of rows {r0}..{r1}")
+        a, b = a + n, b + m
+
+
+def inputs(nq, nk, heads, kv, d, dtype=torch.bfloat16, seed=0):
+    return (rand(nq, heads, d, dtype=dtype, seed=seed), rand(nk, kv, d, dtype=dtype, seed=seed + 1),
+            rand(nk, kv, d, dtype=dtype, seed=seed + 2))
+
+
+@pytest.mark.parametrize("heads,kv,d", [(4, 4, 64), (2, 2, 128), (8, 2, 128), (6, 2, 64)])
+def test_one_query_tile_done_before_the_other(V, heads, kv, d):
+    """The two query tiles of a piece end at different key tiles: values that only the later one sees, in every piece, while
+    the earlier one's results are written.  Each row comes whole, again and again."""
+    lens = [700, 1, 1300, 515]
+    q, k, v = inputs(sum(lens), sum(lens), heads, kv, d, seed=heads)
+    for t in range(40, sum(lens), 90):
+        v[t, :, (t * 7) % d] = (math.nan, math.inf, -math.inf)[t % 3]
+    check(V, q, k, v, lens, None)
+    first, first_lse = poisoned_call(V, q, k, v, starts_of(lens))
+    for _ in range(20):
+        again, lse = poisoned_call(V, q, k, v, starts_of(lens))
+        assert torch.equal(again.view(torch.int16), first.view(torch.int16)) and torch.equal(lse, first_lse)
+
+
+@pytest.mark.parametrize("heads,kv", [(2, 2), (8, 2)])
+def test_unseen_values_where_the_keys_are_split(V, heads, kv):
+    """Few queries after many keys: the parts that the splits leave, joined."""
+    lens, lens_k = [300], [9000]
+    q, k, v = inputs(300, 9000, heads, kv, 64, torch.float16, seed=5)
+    v[8790, :, 3], v[8950, :, 40], v[8951, 0, 40] = math.nan, math.inf, -math.inf
+    check(V, q, k, v, lens, lens_k)

@@ -343,13 +343,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     uint64_t* const work_empty = work_full + kAhead; // [kAhead]
     // [kAhead], and the piece that was taken but not begun when a wait ran out
     Work* const s_work = reinterpret_cast<Work*>(work_empty + kAhead);
-    int* const s_leak = reinterpret_cast<int*>(s_work + kAhead + 1);  // [kAhead]
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(s_leak + kAhead);
+    int* const s_leak = reinterpret_cast<int*>(s_work + kAhead + 1);  // [kAhead][2]: piece, query tile
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(s_leak + 2 * kAhead);
     volatile int* const s_lost = reinterpret_cast<int*>(tmem_slot + 1);  // a wait ran out
     // Rows' maxima (and sums) of each half of the keys: [turn][tile][half][row]
     float* const s_half = reinterpret_cast<float*>(bars + 64);
     const uint32_t s_stage = tc::smem_u32(s_half + 2 * 2 * 2 * kRows);  // 1 KB a softmax warp, for the results
-    static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + (kAhead + 1) * sizeof(Work) + kAhead * 4 + 8 <= 512, "");
+    static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + (kAhead + 1) * sizeof(Work) + 2 * kAhead * 4 + 8 <= 512, "");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // The own pages' kernel may be queued behind this one and does not depend on it.
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
                 if (lane == 0) {
                     s_work[r] = w;
-                    s_leak[r] = 0;
+                    s_leak[2 * r] = s_leak[2 * r + 1] = 0;
                     tc::mbar_arrive(&work_full[r]);
                 }
                 __syncwarp();
@@ -605,7 +605,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     for (int i = lane; i < (kKeys - end) * 8; i += 32)
                         for (int h = 0; h < kHalves; ++h)
                             *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-                    if (bad) s_leak[it % kAhead] = 1;
+                    // Of each query tile that has this key tile to come: its results, which read the
+                    // flag, then wait for a product that waits for this.  A tile that is done with
+                    // its keys may be reading by now, and sees none of these rows.
+                    if (bad && j < x.nt0) s_leak[it % kAhead * 2] = 1;
+                    if (bad && j < x.nt1) s_leak[it % kAhead * 2 + 1] = 1;
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(clean);
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             tc::fence_after_sync();
             // ---- results
             const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + w.kh * p.group + row_head);
-            const bool leak = !PAGED && my_tiles > 0 && ok && *reinterpret_cast<volatile int*>(&s_leak[it % kAhead]) != 0;
+            const bool leak = !PAGED && my_tiles > 0 && ok && *reinterpret_cast<volatile int*>(&s_leak[it % kAhead * 2 + t]) != 0;
             // The piece's place is handed back before the stores: the arrival would wait for them.
             work_done(it++);
             const bool part = p.part;
