@@ -78,3 +78,44 @@ def test_unseen_values_where_the_keys_are_split(V, heads, kv):
     q, k, v = inputs(300, 9000, heads, kv, 64, torch.float16, seed=5)
     v[8790, :, 3], v[8950, :, 40], v[8951, 0, 40] = math.nan, math.inf, -math.inf
     check(V, q, k, v, lens, lens_k)
+
+
+@pytest.mark.parametrize("heads,kv,d", [(8, 8, 128), (16, 4, 64)])
+def test_unseen_values_at_the_end_of_a_long_prompt(V, heads, kv, d):
+    """More pieces than blocks, and one that holds an unseen value after 16,000 keys: neither its rows nor those of the
+    pieces that its block takes next are touched."""
+    lens = [16384, 900]
+    q, k, v = inputs(sum(lens), sum(lens), heads, kv, d, seed=1)
+    v[16200, :, 5], v[16384 + 800, :, 9] = math.nan, math.inf
+    out, lse = poisoned_call(V, q, k, v, starts_of(lens))
+    assert torch.isfinite(lse).all()
+    unseen = torch.ones_like(out, dtype=torch.bool)
+    unseen[16200:16384, :, 5] = unseen[16384 + 800:, :, 9] = False
+    assert torch.isfinite(out[unseen]).all() and not torch.isfinite(out[~unseen]).any()
+    check(V, q, k, v, lens, None, rows=(0, 600, 850, 16199, 16200, 16300))
+
+
+def test_unseen_values_in_every_piece_of_a_long_prompt(V):
+    """A column of values that is not finite in every thirtieth token: the other columns are right."""
+    lens, heads, kv, d = [16384], 8, 4, 128
+    q, k, v = inputs(16384, 16384, heads, kv, d, seed=2)
+    v[::30, :, 77] = math.nan
+    v[29::30, :, 3] = -math.inf
+    out, lse = poisoned_call(V, q, k, v, starts_of(lens))
+    assert torch.isfinite(lse).all()
+    others = torch.arange(d, device="cuda")
+    assert torch.isfinite(out[..., (others != 77) & (others != 3)]).all()
+    assert out[..., 77].isnan().all() and torch.isfinite(out[:29, :, 3]).all() and (out[29:, :, 3] == -math.inf).all()
+    check(V, q, k, v, lens, None, rows=(0, 129, 5000, 16383))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,d", [(7, 1, 128), (6, 2, 96), (2, 1, 40), (3, 3, 8), (24, 1, 72), (128, 1, 128)])
+def test_unseen_values_in_every_head_layout(V, dtype, heads, kv, d):
+    """Prompts on the tensor-memory tiles, and continued ones with fewer and with more keys than queries."""
+    for lens, lens_k in (([700, 1, 333, 1300], None), ([600, 500], [900, 300])):
+        nk = sum(lens if lens_k is None else lens_k)
+        q, k, v = inputs(sum(lens), nk, heads, kv, d, dtype, seed=d)
+        for t in range(5, nk, 61):
+            v[t, :, (t * 5) % d] = (math.nan, math.inf, -math.inf)[t % 3]
+        check(V, q, k, v, lens, lens_k)

@@ -36,8 +36,9 @@
 //
 // Masked scores become -inf by selection, so what unseen keys hold does not matter; unseen
 // values meet P = 0, and 0 * NaN is NaN: value rows past the last key are zeroed in shared
-// memory, and where a later token of the same prompt holds a non-finite value (checked on
-// the diagonal tiles) the block recomputes its rows one key at a time.
+// memory, and so are the non-finite values among rows that not every query row sees (the
+// diagonal tiles').  A row's results then get back those of the keys that it sees, as a sum:
+// any positive weight leaves an infinity or NaN what it is.
 //
 // A block runs from one piece of work to the next (there is one an SM): the copies of the
 // next one, and its first scores, go on while the results of the last one are written.
@@ -79,7 +80,8 @@ struct TileParams {
     // Paged keys: pages of the prefix.
     const int32_t* pages;
     int page_shift;
-    // Packed keys again, for the rows recomputed one key at a time.
+    // Packed rows again, as addresses: the small blocks' (attn_short.cuh), and the values of
+    // keys that not every row of a piece sees.
     HeadsView q, k, v;
     float scale_log2;
     int items;     // pieces of work at most (two query tiles, key head, split)
@@ -97,7 +99,11 @@ constexpr int smem_bytes() {
     return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512 + 2 * 2 * 2 * kRows * 4 + kSoftmaxWarps * 1024;
 }
 
-// Bounded wait for the barrier's phase; false when it ran out (a tile takes microseconds).
+// Bounded wait for the barrier's phase; false when it ran out.  2^20 polls of 20 cycles and more
+// are over 10 ms.  The longest stretch that a warp waits for another is the results of a piece,
+// with at most 2 * 128 rows of values looked through once more: 0.12 ms a piece where all of
+// them hold a non-finite value (eight prompts of 2,000 tokens, 8 heads of 128: 119 us clean, 220
+// with one in thirty tokens, 537 with all).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     const uint32_t a = tc::smem_u32(bar);
     for (uint32_t i = 0; i < (1u << 20); ++i) {
@@ -294,12 +300,24 @@ __device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane
 
 template <class H>
 __device__ __forceinline__ bool not_finite(uint4 u) {
-    constexpr uint32_t lo = sizeof(H) && std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
+    constexpr uint32_t lo = std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) bad |= (w[i] & lo) == lo || (w[i] & hi) == hi;
     return bad;
+}
+
+// The finite ones of eight values, zero for the others; the other way round: the finite ones
+// zero, the others as they are.
+template <class H>
+__device__ __forceinline__ uint4 finite_part(uint4 u, bool others = false) {
+    constexpr uint32_t lo = std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
+    auto part = [&](uint32_t x) {
+        const uint32_t odd = ((x & lo) == lo ? 0xffffu : 0u) | ((x & hi) == hi ? 0xffff0000u : 0u);
+        return x & (others ? odd : ~odd);
+    };
+    return make_uint4(part(u.x), part(u.y), part(u.z), part(u.w));
 }
 
 // Piece of work number `item`: key heads fastest, then splits.  Run by one whole warp.
@@ -600,8 +618,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     bool bad = false;
                     if (!PAGED)
                         for (int i = lane; i < (end - from) * 8; i += 32)
-                            for (int h = 0; h < kHalves; ++h)
-                                bad |= not_finite<H>(*reinterpret_cast<const uint4*>(v + h * kHalfBytes + from * 128 + i * 16));
+                            for (int h = 0; h < kHalves; ++h) {
+                                uint4* const at = reinterpret_cast<uint4*>(v + h * kHalfBytes + from * 128 + i * 16);
+                                if (not_finite<H>(*at)) {
+                                    *at = finite_part<H>(*at);
+                                    bad = true;
+                                }
+                            }
                     for (int i = lane; i < (kKeys - end) * 8; i += 32)
                         for (int h = 0; h < kHalves; ++h)
                             *reinterpret_cast<uint4*>(v + h * kHalfBytes + end * 128 + i * 16) = make_uint4(0, 0, 0, 0);
@@ -753,139 +776,140 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             }
             tc::fence_after_sync();
             // ---- results
+            using T = typename H::type;
             const long long at = ((long long)(w.q0 + t * tt + row_tok) * p.heads + w.kh * p.group + row_head);
             const bool leak = !PAGED && my_tiles > 0 && ok && *reinterpret_cast<volatile int*>(&s_leak[it % kAhead * 2 + t]) != 0;
             // The piece's place is handed back before the stores: the arrival would wait for them.
             work_done(it++);
+            if (leak) {
+                // Non-finite values were taken out of the tiles that not every row of the piece sees:
+                // each row adds those of the keys that it does see.  At most 2 * 128 keys, as a row
+                // sees one more than the row before it.
+                const T* const v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + w.kh * p.v.head;
+                const int begin = j0 * kKeys, from = max(x.min_lim, begin);
+                const int mine = valid ? begin + min(max(lim - begin, 0), per * kKeys) : 0;
+                const int until = __reduce_max_sync(0xffffffffu, mine);
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    const int d = half * (D / 2) + c * 16;
+                    if (d >= p.dim) break;
+                    uint32_t o[16];
+                    tmem_ld16(to + c * 16, o);
+                    tc::tmem_ld_wait();
+#pragma unroll 1
+                    for (int first = from; first < until; first += 32) {  // a lane looks through one key
+                        auto values = [&](int key, int h) {
+                            if (key >= until || d + h * 8 >= p.dim) return make_uint4(0, 0, 0, 0);
+                            return __ldg(reinterpret_cast<const uint4*>(v + key * p.v.tok + d) + h);
+                        };
+                        unsigned some = __ballot_sync(
+                            0xffffffffu, not_finite<H>(values(first + lane, 0)) || not_finite<H>(values(first + lane, 1)));
+#pragma unroll 1
+                        for (; some; some &= some - 1) {
+                            const int key = first + __ffs(some) - 1;
+                            if (key >= mine) continue;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float val[8];
+                                unpack8<H>(finite_part<H>(values(key, h), true), val);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    o[h * 8 + i] = __float_as_uint(__uint_as_float(o[h * 8 + i]) + val[i]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    tmem_st16(to + c * 16, o);
+                    tc::tmem_st_wait();
+                }
+            }
             const bool part = p.part;
             const long long rows = (long long)p.n_q * p.heads;
             const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-            using T = typename H::type;
-            if (!leak) {
-                // A thread has part of one row, rows lie heads * dim apart: stored from here, each
-                // 16 bytes are a line of their own (3,000 cycles a piece with heads of 64, 6,000 with
-                // 128).  So a warp passes its rows through 1 KB of shared memory, a few at a time, and
-                // stores each row's part in one go.
-                const uint32_t stage = s_stage + warp * 1024;
-                auto scaled = [&](uint32_t o) { return l == 0.0f ? 0.0f : __uint_as_float(o) * inv; };
-                // kRowsAt rows of kPieces 16-byte pieces; `piece` gives this lane's, `put` stores one
-                // of the row of another lane.
-                auto through = [&](auto pieces, auto&& piece, auto&& put) {
-                    constexpr int kPieces = decltype(pieces)::value, kRowsAt = 64 / kPieces;
-                    const int mine = lane % kRowsAt;
+            // A thread has part of one row, rows lie heads * dim apart: stored from here, each
+            // 16 bytes are a line of their own (3,000 cycles a piece with heads of 64, 6,000 with
+            // 128).  So a warp passes its rows through 1 KB of shared memory, a few at a time, and
+            // stores each row's part in one go.
+            const uint32_t stage = s_stage + warp * 1024;
+            auto scaled = [&](uint32_t o) { return l == 0.0f ? 0.0f : __uint_as_float(o) * inv; };
+            // kRowsAt rows of kPieces 16-byte pieces; `piece` gives this lane's, `put` stores one
+            // of the row of another lane.
+            auto through = [&](auto pieces, auto&& piece, auto&& put) {
+                constexpr int kPieces = decltype(pieces)::value, kRowsAt = 64 / kPieces;
+                const int mine = lane % kRowsAt;
 #pragma unroll
-                    for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
-                        __syncwarp();
-                        if (lane / kRowsAt == r0 / kRowsAt)
+                for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
+                    __syncwarp();
+                    if (lane / kRowsAt == r0 / kRowsAt)
 #pragma unroll
-                            for (int i = 0; i < kPieces; ++i) {
-                                const uint4 u = piece(i);
-                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
-                                                 stage + (mine * kPieces + (i ^ (mine & 7 & (kPieces - 1)))) * 16),
-                                             "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
-                                             : "memory");
-                            }
-                        __syncwarp();
-#pragma unroll
-                        for (int e = lane; e < 64; e += 32) {
-                            const int r = e / kPieces, i = e % kPieces;
-                            uint4 u;
-                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                                         : "r"(stage + (r * kPieces + (i ^ (r & 7 & (kPieces - 1)))) * 16)
+                        for (int i = 0; i < kPieces; ++i) {
+                            const uint4 u = piece(i);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                                             stage + (mine * kPieces + (i ^ (mine & 7 & (kPieces - 1)))) * 16),
+                                         "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
                                          : "memory");
-                            const long long row_at = __shfl_sync(0xffffffffu, at, r0 + r);
-                            if (__shfl_sync(0xffffffffu, (int)valid, r0 + r)) put(row_at, i, u);
                         }
-                    }
-                };
-                if (!part) {
-                    uint32_t pk[D / 4];
+                    __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[16];
+                    for (int e = lane; e < 64; e += 32) {
+                        const int r = e / kPieces, i = e % kPieces;
+                        uint4 u;
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                     : "r"(stage + (r * kPieces + (i ^ (r & 7 & (kPieces - 1)))) * 16)
+                                     : "memory");
+                        const long long row_at = __shfl_sync(0xffffffffu, at, r0 + r);
+                        if (__shfl_sync(0xffffffffu, (int)valid, r0 + r)) put(row_at, i, u);
+                    }
+                }
+            };
+            if (!part) {
+                uint32_t pk[D / 4];
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[16];
+                    if (my_tiles > 0) {
+                        tmem_ld16(to + c * 16, o);
+                        tc::tmem_ld_wait();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pk[c * 8 + i] = H::pack(scaled(o[2 * i]), scaled(o[2 * i + 1]));
+                }
+                through(std::integral_constant<int, D / 16>{},
+                        [&](int i) { return make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]); },
+                        [&](long long row_at, int i, const uint4& u) {
+                            const int d = half * (D / 2) + i * 8;
+                            if (d < p.dim) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row_at * p.dim + d) = u;
+                        });
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < D / 64; ++c) {  // 32 values at a time
+                    uint32_t o[2][16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
                         if (my_tiles > 0) {
-                            tmem_ld16(to + c * 16, o);
+                            tmem_ld16(to + c * 32 + h * 16, o[h]);
                             tc::tmem_ld_wait();
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = 0;
+                            for (int i = 0; i < 16; ++i) o[h][i] = 0;
                         }
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) pk[c * 8 + i] = H::pack(scaled(o[2 * i]), scaled(o[2 * i + 1]));
+                        for (int i = 0; i < 16; ++i) o[h][i] = __float_as_uint(scaled(o[h][i]));
                     }
-                    through(std::integral_constant<int, D / 16>{},
-                            [&](int i) { return make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]); },
+                    through(std::integral_constant<int, 8>{},
+                            [&](int i) {
+                                const uint32_t* e = &o[i >> 2][(i & 3) * 4];
+                                return make_uint4(e[0], e[1], e[2], e[3]);
+                            },
                             [&](long long row_at, int i, const uint4& u) {
-                                const int d = half * (D / 2) + i * 8;
-                                if (d < p.dim) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row_at * p.dim + d) = u;
+                                const int d = half * (D / 2) + c * 32 + i * 4;
+                                if (d < p.dim)
+                                    *reinterpret_cast<uint4*>(p.part_o + (w.split * rows + row_at) * p.dim + d) = u;
                             });
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < D / 64; ++c) {  // 32 values at a time
-                        uint32_t o[2][16];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (my_tiles > 0) {
-                                tmem_ld16(to + c * 32 + h * 16, o[h]);
-                                tc::tmem_ld_wait();
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) o[h][i] = 0;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[h][i] = __float_as_uint(scaled(o[h][i]));
-                        }
-                        through(std::integral_constant<int, 8>{},
-                                [&](int i) {
-                                    const uint32_t* e = &o[i >> 2][(i & 3) * 4];
-                                    return make_uint4(e[0], e[1], e[2], e[3]);
-                                },
-                                [&](long long row_at, int i, const uint4& u) {
-                                    const int d = half * (D / 2) + c * 32 + i * 4;
-                                    if (d < p.dim)
-                                        *reinterpret_cast<uint4*>(p.part_o + (w.split * rows + row_at) * p.dim + d) = u;
-                                });
-                    }
-                }
-            } else if (valid) {
-                // One key at a time, eight output values a pass, with the maximum and sum that the
-                // scores gave: only where an unseen value row is not finite.
-                const T* q = static_cast<const T*>(p.q.p) + (w.q0 + t * tt + row_tok) * p.q.tok +
-                             (w.kh * p.group + row_head) * p.q.head;
-                const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + w.kh * p.k.head;
-                const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + w.kh * p.v.head;
-                const int from = j0 * kKeys, to_key = min(lim, (j0 + per) * kKeys);
-                const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-                for (int c = half * 8; c < p.dim; c += 16) {
-                    float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 1
-                    for (int key = from; key < to_key; ++key) {
-                        float s = 0.0f;
-#pragma unroll 1
-                        for (int e = 0; e < p.dim; e += 8) {
-                            float a[8], b[8];
-                            unpack8<H>(*reinterpret_cast<const uint4*>(q + e), a);
-                            unpack8<H>(*reinterpret_cast<const uint4*>(k + key * p.k.tok + e), b);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
-                        }
-                        const float x = ex2(fmaf(s, p.scale_log2, -ref));
-                        float val[8];
-                        unpack8<H>(*reinterpret_cast<const uint4*>(v + key * p.v.tok + c), val);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) o[i] += x * val[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] *= inv;
-                    if (part) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + at) * p.dim + c);
-                        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-                        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-                    } else {
-                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.dim + c) = pack8<H>(o);
-                    }
                 }
             }
             if (valid && half == 0) {
