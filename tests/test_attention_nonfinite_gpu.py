@@ -119,3 +119,44 @@ def test_unseen_values_in_every_head_layout(V, dtype, heads, kv, d):
         for t in range(5, nk, 61):
             v[t, :, (t * 5) % d] = (math.nan, math.inf, -math.inf)[t % 3]
         check(V, q, k, v, lens, lens_k)
+
+
+# ------------------------------------------------------------------------------------------ short prompts, small blocks
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 128), (4, 4, 64), (7, 1, 128), (6, 2, 96), (2, 1, 40), (3, 3, 8), (64, 1, 64)])
+def test_unseen_values_in_short_prompts(V, dtype, heads, kv, d):
+    for lens, lens_k in (([1, 33, 0, 130, 97, 2], None), ([5, 64, 0, 70], [30, 64, 9, 41])):
+        nk = sum(lens if lens_k is None else lens_k)
+        q, k, v = inputs(sum(lens), nk, heads, kv, d, dtype, seed=d + 1)
+        for t in range(3, nk, 13):
+            v[t, :, (t * 5) % d] = (math.nan, math.inf, -math.inf)[t % 3]
+        check(V, q, k, v, lens, lens_k)
+
+
+def test_unseen_values_in_a_long_prompt_among_short_ones(V):
+    """By their mean these go to the small blocks, the long one too."""
+    lens = [3] * 400 + [6000] + [20] * 100
+    q, k, v = inputs(sum(lens), sum(lens), 4, 2, 64, seed=3)
+    v[7::31, 0, 11] = math.nan
+    check(V, q, k, v, lens, None)
+
+
+def test_unseen_values_cost_no_more_than_looking_for_them(V):
+    """200 prompts of 100 tokens with one such value in thirty tokens: ten times the time without is far more than one more
+    look at the values takes, and far less than computing rows again."""
+    n, lens = 20000, starts_of([100] * 200)
+    q, k, v = inputs(n, n, 12, 12, 64)
+
+    def time():
+        for _ in range(3):
+            V.prompt_attention(q, k, v, lens)
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(10):
+            V.prompt_attention(q, k, v, lens)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b)
+    clean = time()
+    v[::30, :, 3] = math.nan
+    assert time() < 10 * clean

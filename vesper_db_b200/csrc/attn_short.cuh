@@ -9,9 +9,9 @@
 // Rows of the stages are 16-byte chunks XORed with the row, so that the eight rows of a
 // matrix load lie in different banks.  Softmax as in attn_tile.cuh: one pass, running maximum
 // and sum in 32 bits, P rounded to the data's type for the second product.  Value rows past
-// the last key are filled with zeros by the copy; where a later token of the same prompt holds
-// a non-finite value (checked on the diagonal tiles) the block recomputes its rows one key at
-// a time.
+// the last key are filled with zeros by the copy, and non-finite values of tokens that not every
+// row of the block sees (the diagonal tiles') are taken out in shared memory and added back by
+// the rows that do see them.
 //
 // Bound by the latency of one block: loads, two products and the softmax of a few key tiles.
 // Measured: three prompts of 61 tokens in all (32 + 8 heads of 128, causal): 6.1 us; both
@@ -136,12 +136,16 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
         if (j + 1 < n) request(j + 1);
         const uint32_t sk = s_kv + (j & 1) * 2 * kTileBytes, sv = sk + kTileBytes;
         const int key = j * kShortKeys;
-        if (w.step && key + kShortKeys > min_lim) {  // value rows that some row must not see
+        const bool guarded = w.step && key + kShortKeys > min_lim;  // value rows that some row must not see
+        if (guarded) {
             const int from = max(min_lim - key, 0), end = min(w.len_k - key, kShortKeys);
-            bool bad = false;
-            for (int i = from * kChunks + tid; i < end * kChunks; i += kShortThreads)
-                bad |= not_finite<H>(*reinterpret_cast<const uint4*>(smem + (j & 1) * 2 * kTileBytes + kTileBytes + i * 16));
-            if (bad) s_leak = 1;
+            for (int i = from * kChunks + tid; i < end * kChunks; i += kShortThreads) {
+                uint4* const at = reinterpret_cast<uint4*>(smem + (j & 1) * 2 * kTileBytes + kTileBytes + i * 16);
+                if (not_finite<H>(*at)) {
+                    *at = finite_part<H>(*at);
+                    s_leak = 1;
+                }
+            }
         }
         float s[kShortKeys / 8][4];
 #pragma unroll
@@ -190,6 +194,7 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
                 o[i][3] *= f[1];
             }
         }
+        if (guarded) __syncthreads();  // the values are as they are multiplied
 #pragma unroll
         for (int k = 0; k < kShortKeys / 16; ++k) {
             uint32_t pa[4];
@@ -214,53 +219,50 @@ __global__ void __launch_bounds__(kShortThreads, D == 64 ? 4 : 3) attn_short_ker
         }
     }
     __syncthreads();
-    const bool leak = *static_cast<volatile int*>(&s_leak) != 0;
+    if (*static_cast<volatile int*>(&s_leak) != 0) {
+        // The rows see at most 64 keys that not all of them see; a lane looks through one.
+        const T* const v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + kh * p.v.head;
+        const int until = __reduce_max_sync(0xffffffffu, max(lim[0], lim[1]));
+#pragma unroll 1
+        for (int first = min_lim; first < until; first += 32) {
+            bool odd = false;
+            if (first + lane < until)
+#pragma unroll 4
+                for (int c = 0; c < p.dim; c += 8)
+                    odd |= not_finite<H>(__ldg(reinterpret_cast<const uint4*>(v + (first + lane) * p.v.tok + c)));
+#pragma unroll 1
+            for (unsigned some = __ballot_sync(0xffffffffu, odd); some; some &= some - 1) {
+                const int key = first + __ffs(some) - 1;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    if (i * 8 >= p.dim) break;
+                    const float2 x = H::unpack(finite_part<H>(
+                        __ldg(reinterpret_cast<const uint32_t*>(v + key * p.v.tok + i * 8 + 2 * t)), true));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (key >= lim[h]) continue;
+                        o[i][2 * h] += x.x;
+                        o[i][2 * h + 1] += x.y;
+                    }
+                }
+            }
+        }
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         if (!valid[h]) continue;
         const float inv = l[h] > 0.0f ? 1.0f / l[h] : (l[h] == 0.0f ? 0.0f : l[h]);
-        T* const dst = static_cast<T*>(p.out) + out_row[h] * p.dim;
-        if (!leak) {  // through the warp's own part of the stages: whole rows are stored below
-            const int r = warp * 16 + g + 8 * h;
+        // through the warp's own part of the stages: whole rows are stored below
+        const int r = warp * 16 + g + 8 * h;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const float x = l[h] == 0.0f ? 0.0f : o[i][2 * h] * inv, y = l[h] == 0.0f ? 0.0f : o[i][2 * h + 1] * inv;
-                *reinterpret_cast<uint32_t*>(smem + r * kRowBytes + ((i ^ (r & 7)) << 4) + t * 4) = H::pack(x, y);
-            }
-        } else {
-            // One key at a time, with the maximum and sum that the scores gave; a lane of the
-            // four that hold the row takes every fourth chunk of it.
-            const T* k = static_cast<const T*>(p.k.p) + w.k0 * p.k.tok + kh * p.k.head;
-            const T* v = static_cast<const T*>(p.v.p) + w.k0 * p.v.tok + kh * p.v.head;
-            const float ref = m[h] == -INFINITY ? 0.0f : m[h];
-#pragma unroll 1
-            for (int c = t * 8; c < p.dim; c += 32) {
-                float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 1
-                for (int key = 0; key < lim[h]; ++key) {
-                    float s = 0.0f, a[8], b[8];
-#pragma unroll 1
-                    for (int e = 0; e < p.dim; e += 8) {
-                        unpack8<H>(*reinterpret_cast<const uint4*>(q_row[h] + e), a);
-                        unpack8<H>(*reinterpret_cast<const uint4*>(k + key * p.k.tok + e), b);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
-                    }
-                    const float x = ex2(fmaf(s, p.scale_log2, -ref));
-                    unpack8<H>(*reinterpret_cast<const uint4*>(v + key * p.v.tok + c), b);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i] += x * b[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] *= inv;
-                *reinterpret_cast<uint4*>(dst + c) = pack8<H>(acc);
-            }
+        for (int i = 0; i < D / 8; ++i) {
+            const float x = l[h] == 0.0f ? 0.0f : o[i][2 * h] * inv, y = l[h] == 0.0f ? 0.0f : o[i][2 * h + 1] * inv;
+            *reinterpret_cast<uint32_t*>(smem + r * kRowBytes + ((i ^ (r & 7)) << 4) + t * 4) = H::pack(x, y);
         }
         if (p.lse && t == 0) p.lse[out_row[h]] = (m[h] + log2f(l[h])) * 0.6931471805599453f;
     }
-    if (leak) return;
     __syncwarp();
 #pragma unroll
     for (int e = lane; e < 16 * kChunks; e += 32) {

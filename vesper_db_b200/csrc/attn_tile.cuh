@@ -308,16 +308,18 @@ __device__ __forceinline__ bool not_finite(uint4 u) {
     return bad;
 }
 
-// The finite ones of eight values, zero for the others; the other way round: the finite ones
-// zero, the others as they are.
+// Of two values, or eight: the finite ones, zero in the others' places; with `others` those,
+// zero in the finite ones' places.
+template <class H>
+__device__ __forceinline__ uint32_t finite_part(uint32_t u, bool others = false) {
+    constexpr uint32_t lo = std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
+    const uint32_t odd = ((u & lo) == lo ? 0xffffu : 0u) | ((u & hi) == hi ? 0xffff0000u : 0u);
+    return u & (others ? odd : ~odd);
+}
 template <class H>
 __device__ __forceinline__ uint4 finite_part(uint4 u, bool others = false) {
-    constexpr uint32_t lo = std::is_same<H, Bf16>::value ? 0x7f80u : 0x7c00u, hi = lo << 16;
-    auto part = [&](uint32_t x) {
-        const uint32_t odd = ((x & lo) == lo ? 0xffffu : 0u) | ((x & hi) == hi ? 0xffff0000u : 0u);
-        return x & (others ? odd : ~odd);
-    };
-    return make_uint4(part(u.x), part(u.y), part(u.z), part(u.w));
+    return make_uint4(finite_part<H>(u.x, others), finite_part<H>(u.y, others), finite_part<H>(u.z, others),
+                      finite_part<H>(u.w, others));
 }
 
 // Piece of work number `item`: key heads fastest, then splits.  Run by one whole warp.
