@@ -1,0 +1,62 @@
+"""The attention operators where sizes, argument kinds and non-finite values meet the edges of what they take."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def V():
+    import vesper_db_b200
+    return vesper_db_b200
+
+
+def rand(*shape, dtype=torch.bfloat16, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def ints(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------ page_tables
+MANY_REQUESTS = """
+import sys
+import torch
+import vesper_db_b200 as V
+page, width = 16, 3
+for n in map(int, sys.argv[1:]):
+    i = torch.arange(n)
+    cached, fresh = (i * 7) % 20, (i * 5) % 9
+    had, need = (cached + page - 1) // page, (cached + fresh + page - 1) // page
+    table = torch.where(torch.arange(width)[None] < had[:, None], i[:, None] * width + torch.arange(width)[None], -1)
+    free = 100000 + torch.arange(int((need - had).sum()))
+    starts = torch.cat([torch.zeros(1, dtype=torch.long), fresh.cumsum(0)])
+    total = int(starts[-1])
+    want = table.clone()
+    fill = (torch.arange(width)[None] >= had[:, None]) & (torch.arange(width)[None] < need[:, None])
+    want[fill] = free  # row by row: request order
+    row = torch.repeat_interleave(i, fresh)
+    at = cached[row] + torch.arange(total) - starts[row]
+    slots = want[row, at // page] * page + at % page
+    dev = lambda x: x.to(torch.int32).cuda()
+    got = V.page_tables(dev(cached), dev(fresh), dev(free), dev(table), page, total, base=3)
+    for name, a, b in zip(got._fields, got, (want, cached + fresh, starts, at + 3, slots, (need - had).sum()[None])):
+        assert torch.equal(a.cpu().long(), b), (n, name)
+print("as expected")
+"""
+
+
+@pytest.mark.parametrize("sizes", [[4073, 4074, 4095, 4096, 16384, 4090], [4095], [16384, 4074, 16384]])
+def test_tables_request_counts_around_the_shared_memory_limit(V, sizes):
+    """In a process of its own: what an earlier call opted in to must not matter."""
+    r = subprocess.run([sys.executable, "-c", MANY_REQUESTS, *map(str, sizes)], cwd=ROOT, capture_output=True, text=True,
+                       env={**os.environ, "PYTHONPATH": ROOT}, timeout=300)
+    assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]

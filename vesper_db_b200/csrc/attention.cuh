@@ -7,7 +7,13 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "common.cuh"
+
 namespace vgpu {
+
+constexpr int kMaxTableRequests = 16384;  // of one page_tables call
 
 // Address and strides (elements) of a [tokens, heads, dim] view; dim is contiguous.
 struct HeadsView {
@@ -103,5 +109,17 @@ size_t prompt_attention_workspace(const PromptArgs& a);
 void launch_prompt_attention(const PromptArgs& a, cudaStream_t st);
 size_t shared_attention_workspace(const SharedArgs& a);
 void launch_shared_attention(const SharedArgs& a, cudaStream_t st);
+
+// Opts a kernel in to its dynamic shared memory, once a device; `more` runs with it.
+template <class K, class F>
+void opt_in(std::atomic<uint64_t>& devices, K* kernel, int smem, F&& more) {
+    int dev = 0;
+    VGPU_CHECK(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (devices.load(std::memory_order_relaxed) & bit) return;
+    VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    more();
+    devices.fetch_or(bit, std::memory_order_relaxed);
+}
 
 }  // namespace vgpu

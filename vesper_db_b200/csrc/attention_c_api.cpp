@@ -134,7 +134,7 @@ extern "C" {
 VESPER_C_API vesper_status_t vesper_page_tables_device(const vesper_page_tables_params_t* params, void* cuda_stream) {
     return entry(params, [&] {
         const vesper_page_tables_params_t& p = *params;
-        need(p.n_requests <= 16384, "at most 16384 requests");
+        need(p.n_requests <= (size_t)vgpu::kMaxTableRequests, "at most 16384 requests");
         need(p.n_tokens <= kMaxInt && p.n_free <= kMaxInt && p.table_width <= kMaxInt, "sizes must be below 2^31");
         need(p.base >= 0 && p.base <= (int64_t)kMaxInt, "base must be 0 to 2^31 - 1");
         vgpu::PageTablesArgs a{};

@@ -338,8 +338,10 @@ void norm_rotate_width(const NormRotateArgs& a, cudaStream_t st) {
 
 void launch_page_tables(const PageTablesArgs& a, cudaStream_t st) {
     const size_t smem = 3 * ((size_t)a.n_requests + 1) * sizeof(int);
-    if (smem > 48 * 1024)
-        VGPU_CHECK(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // To the most that any call needs, whatever this one does: calls of other threads, and what the
+    // kernel has of shared memory besides, then do not matter.
+    static std::atomic<uint64_t> devices{0};
+    opt_in(devices, page_tables_kernel, (int)(3 * (kMaxTableRequests + 1) * sizeof(int)), [] {});
     const long long per_block = kScanThreads * kRun;
     const long long want = std::max<long long>((a.n_tokens + per_block - 1) / per_block, (a.n_requests + 63) / 64);
     const int blocks = (int)std::min<long long>(std::max<long long>(want, 1), 148 * 2);

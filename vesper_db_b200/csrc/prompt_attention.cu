@@ -1,7 +1,6 @@
 // Attention over packed prompts, and over a shared prefix joined with each request's own
 // pages: launchers, the kernel of the own pages, and the join of partial results.
 #include <algorithm>
-#include <atomic>
 
 #include "attention.cuh"
 #include "attn_short.cuh"
@@ -80,18 +79,6 @@ void fill_queries(TileParams& p, bool f16, const HeadsView& q, int heads, int kv
     p.q = q;
     p.mq = make_map(f16, q.p, {dim, p.group, kv_heads, n_q}, {q.head, q.head * p.group, q.tok},
                     {64, p.group, 1, p.tile_tokens});
-}
-
-// Opts a kernel in to its dynamic shared memory, once a device; `more` runs with it.
-template <class K, class F>
-void opt_in(std::atomic<uint64_t>& devices, K* kernel, int smem, F&& more) {
-    int dev = 0;
-    VGPU_CHECK(cudaGetDevice(&dev));
-    const uint64_t bit = 1ull << (dev & 63);
-    if (devices.load(std::memory_order_relaxed) & bit) return;
-    VGPU_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    more();
-    devices.fetch_or(bit, std::memory_order_relaxed);
 }
 
 template <class H, int D, bool PAGED>
