@@ -1,4 +1,5 @@
 """The attention operators where sizes, argument kinds and non-finite values meet the edges of what they take."""
+import math
 import os
 import subprocess
 import sys
@@ -60,3 +61,26 @@ def test_tables_request_counts_around_the_shared_memory_limit(V, sizes):
     r = subprocess.run([sys.executable, "-c", MANY_REQUESTS, *map(str, sizes)], cwd=ROOT, capture_output=True, text=True,
                        env={**os.environ, "PYTHONPATH": ROOT}, timeout=300)
     assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------ values that are seen
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_seen_values_reach_the_row_however_small_their_weight(V, bad):
+    """Parts of a row's keys are computed apart and joined: a value that is not finite shows wherever it stands, also where
+    its part's weight is zero in 32 bits (the definition gives it a weight above zero)."""
+    d, heads = 64, 4
+    # keys of the first part score -200, those of the second +200
+    q = torch.ones(3, heads, d, dtype=torch.bfloat16, device="cuda")
+    kc, vc = rand(8, 16, 2, d, seed=1), rand(8, 16, 2, d, seed=2)
+    kc[:4], kc[4:] = -25, 25  # times 64 ones, scaled by 1 / 8
+    pages, table = ints([0, 1, 2, 3]), ints([[4], [5], [6]])
+    vc[2, 3, :, 7] = bad
+    out = V.shared_prefix_attention(q, kc, vc, pages, 64, table, ints([16, 1, 9]))
+    assert not torch.isfinite(out[..., 7]).any() and torch.isfinite(out[..., :7]).all()
+    # a few queries over many packed keys: split over the keys, then joined
+    n = 20000
+    k, v = rand(n, 2, d, seed=3), rand(n, 2, d, seed=4)
+    k[:n // 2], k[n // 2:] = -25, 25
+    v[100, :, 9] = bad
+    out = V.prompt_attention(q, k, v, ints([0, 3]), ints([0, n]), causal=False)
+    assert not torch.isfinite(out[..., 9]).any() and torch.isfinite(out[..., :9]).all()

@@ -611,7 +611,9 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
         m = up;
         total = total * f + w;  // this lane's share
         o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-        unsigned some = __ballot_sync(0xffffffffu, w > 0.0f);  // the others add nothing, and may hold anything
+        // Parts without keys may hold anything.  One whose weight is zero in 32 bits takes part: a
+        // value in it that is not finite is seen by the row.
+        unsigned some = __ballot_sync(0xffffffffu, x != -INFINITY);
         while (some) {
             float4 v[4];
             float wi[4];
