@@ -1,0 +1,37 @@
+"""The package, its C library and its build where torch or the extension on torch tensors is not there."""
+import subprocess
+import sys
+
+import pytest
+
+from conftest import ROOT
+
+
+def python(code):
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return r.stdout
+
+
+NO_TORCH = "import sys; sys.modules['torch'] = None\n"
+NO_EXTENSION = "import sys; sys.modules['vesper_db_b200._attention'] = None\n"
+
+
+def test_star_import_needs_no_torch():
+    out = python(NO_TORCH + "from vesper_db_b200 import *\nprint(IvfPqIndex.__name__, flat_topk.__name__)")
+    assert out.split() == ["IvfPqIndex", "flat_topk"]
+
+
+@pytest.mark.parametrize("missing,says", [(NO_TORCH, "torch"), (NO_EXTENSION, "vesper_db_b200.build")],
+                         ids=["torch", "extension"])
+def test_operators_that_cannot_load_are_absent_attributes(missing, says):
+    """hasattr and getattr with a default work; the message of the error says what is missing."""
+    out = python(missing + "import vesper_db_b200 as V\nprint(hasattr(V, 'page_tables'), getattr(V, 'norm_rotate', 7))\n"
+                 "try: V.prompt_attention\nexcept AttributeError as e: print(e)")
+    assert out.split()[:2] == ["False", "7"] and says in out
+
+
+def test_operators_are_listed_and_importable():
+    python("import vesper_db_b200 as V\nfrom vesper_db_b200 import page_tables, PageTables\n"
+           "assert {'page_tables', 'norm_rotate', 'prompt_attention', 'shared_prefix_attention', 'PageTables'} <= set(dir(V))\n"
+           "assert hasattr(V, 'shared_prefix_attention') and not hasattr(V, 'no_such_thing')")

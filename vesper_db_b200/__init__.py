@@ -14,12 +14,20 @@ _ATTENTION = ("PageTables", "page_tables", "norm_rotate", "prompt_attention", "s
 
 def __getattr__(name):
     if name in _ATTENTION:  # the attention operators take torch tensors: torch is imported on first use
-        from . import attention
+        try:
+            from . import attention
+        except (ImportError, RuntimeError) as e:  # without torch or the extension they are not there, and the rest is
+            raise AttributeError(f"module {__name__!r} has no {name!r} here: {e}") from e
         globals().update({n: getattr(attention, n) for n in _ATTENTION})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
+def __dir__():
+    return sorted({*globals(), *_ATTENTION})
+
+
+# What a star import brings; the attention operators, which need torch, come by name.
 __all__ = ["IvfPqIndex", "TrainReport", "VesperError", "SEARCH_FAST", "SEARCH_EXACT", "load",
            "library_path", "KmeansResult", "kmeans_cluster", "kmeans_elkan", "kmeans_fit_device",
-           "flat_topk", "flat_topk_device", *_ATTENTION]
+           "flat_topk", "flat_topk_device"]
