@@ -35,3 +35,11 @@ def test_operators_are_listed_and_importable():
     python("import vesper_db_b200 as V\nfrom vesper_db_b200 import page_tables, PageTables\n"
            "assert {'page_tables', 'norm_rotate', 'prompt_attention', 'shared_prefix_attention', 'PageTables'} <= set(dir(V))\n"
            "assert hasattr(V, 'shared_prefix_attention') and not hasattr(V, 'no_such_thing')")
+
+
+def test_library_builds_without_torch(tmp_path):
+    """The C library alone needs no torch: the build says that it leaves the extension out."""
+    out = python(NO_TORCH + "from vesper_db_b200 import build as b\n"
+                 f"b.EXT = {str(tmp_path / '_attention.so')!r}\nassert b.build(verbose=True) == b.LIB\n"
+                 "import os; assert not os.path.exists(b.EXT)")
+    assert "torch" in out and "_attention.so" in out

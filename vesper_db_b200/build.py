@@ -1,5 +1,5 @@
 """Build libvesper_c.so (the B200 IVF-PQ engine and its C ABI) and _attention.so (the attention
-operators on torch tensors, over that ABI) in-tree.
+operators on torch tensors, over that ABI; only where torch is installed) in-tree.
 
 CUDA sources are compiled for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``);
 host sources with g++ -std=c++23.  Objects go to vesper_db_b200/_build/ and are rebuilt
@@ -84,9 +84,19 @@ def build(verbose: bool = False) -> str:
     if jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         _run([NVCC, "-shared", "-Xlinker", "--no-undefined", "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static",
               "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"])
-    if _stale(EXT, EXT_SRC, [os.path.join(ROOT, "include", "vesper_b200.h"), os.path.join(ROOT, "include", "vesper.h")]):
+    if not _has_torch():
+        print(f"torch is not installed here: {os.path.basename(EXT)} is left out", flush=True)
+    elif _stale(EXT, EXT_SRC, [os.path.join(ROOT, "include", "vesper_b200.h"), os.path.join(ROOT, "include", "vesper.h")]):
         _build_extension(verbose)
     return LIB
+
+
+def _has_torch() -> bool:
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False
+    return True
 
 
 def _build_extension(verbose: bool) -> None:
