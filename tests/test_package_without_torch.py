@@ -1,4 +1,5 @@
 """The package, its C library and its build where torch or the extension on torch tensors is not there."""
+import os
 import subprocess
 import sys
 
@@ -43,3 +44,28 @@ def test_library_builds_without_torch(tmp_path):
                  f"b.EXT = {str(tmp_path / '_attention.so')!r}\nassert b.build(verbose=True) == b.LIB\n"
                  "import os; assert not os.path.exists(b.EXT)")
     assert "torch" in out and "_attention.so" in out
+
+
+def test_extension_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    """It is tied to the binary interface of the torch and the Python that it was compiled with."""
+    from vesper_db_b200 import build as b
+    built, real = [], b._run
+    monkeypatch.setattr(b, "EXT", str(tmp_path / "_attention.so"))
+
+    def run(cmd):
+        if b.EXT not in cmd:  # the library's own parts are built as ever
+            return real(cmd)
+        built.append(cmd)
+        open(b.EXT, "w").close()
+    monkeypatch.setattr(b, "_run", run)
+    import torch
+
+    def builds():
+        built.clear()
+        b.build()
+        return len(built)
+    assert builds() == 1 and builds() == 0
+    monkeypatch.setattr(torch, "__version__", "9.9.9+other")
+    assert builds() == 1 and builds() == 0
+    os.utime(b.EXT, (1, 1))
+    assert builds() == 1

@@ -86,8 +86,16 @@ def build(verbose: bool = False) -> str:
               "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"])
     if not _has_torch():
         print(f"torch is not installed here: {os.path.basename(EXT)} is left out", flush=True)
-    elif _stale(EXT, EXT_SRC, [os.path.join(ROOT, "include", "vesper_b200.h"), os.path.join(ROOT, "include", "vesper.h")]):
+        return LIB
+    # The extension is tied to the binary interface of the torch and the Python it was compiled with.
+    import torch
+    kind, note = f"torch {torch.__version__}, Python {sys.version}", EXT + ".built_with"
+    made_with = open(note).read() if os.path.exists(note) else None
+    headers = [os.path.join(ROOT, "include", "vesper_b200.h"), os.path.join(ROOT, "include", "vesper.h")]
+    if kind != made_with or _stale(EXT, EXT_SRC, headers):
         _build_extension(verbose)
+        with open(note, "w") as f:
+            f.write(kind)
     return LIB
 
 
