@@ -63,6 +63,43 @@ def test_tables_request_counts_around_the_shared_memory_limit(V, sizes):
     assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]
 
 
+# ------------------------------------------------------------------------------------------ arguments
+def refused(says, call):
+    from vesper_db_b200 import VesperError
+    with pytest.raises(VesperError, match=says):
+        call()
+
+
+def some_inputs():
+    q, k, v = rand(5, 8, 64, seed=1), rand(5, 2, 64, seed=2), rand(5, 2, 64, seed=3)
+    kc, vc = rand(4, 16, 2, 64, seed=4), rand(4, 16, 2, 64, seed=5)
+    return q, k, v, kc, vc, ints([[0, 1]] * 5), ints([3] * 5), ints([2]), torch.zeros(9, 64, device="cuda")
+
+
+def test_inputs_that_require_a_gradient_are_refused(V):
+    """There is no backward pass: a result that silently stands outside the graph would train on wrong gradients."""
+    q, k, v, kc, vc, table, lens, pages, turns = some_inputs()
+    starts, pos, slots = ints([0, 5]), ints([0] * 5), ints([0, 1, 2, 3, 4], torch.int64)
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    grad = lambda x: x.clone().requires_grad_()  # noqa: E731
+    calls = [lambda g: V.prompt_attention(g(q), k, v, starts), lambda g: V.prompt_attention(q, g(k), v, starts),
+             lambda g: V.prompt_attention(q, k, g(v), starts),
+             lambda g: V.shared_prefix_attention(g(q), kc, vc, pages, 9, table, lens),
+             lambda g: V.shared_prefix_attention(q, g(kc), vc, pages, 9, table, lens),
+             lambda g: V.shared_prefix_attention(q, kc, g(vc), pages, 9, table, lens),
+             lambda g: V.norm_rotate(g(q), k, v, pos, turns), lambda g: V.norm_rotate(q, g(k), v, pos, turns),
+             lambda g: V.norm_rotate(q, k, g(v), pos, turns, slots=slots, k_cache=kc, v_cache=vc),
+             lambda g: V.norm_rotate(q, k, v, pos, g(turns)), lambda g: V.norm_rotate(q, k, v, pos, turns, q_weight=g(w)),
+             lambda g: V.norm_rotate(q, k, v, pos, turns, k_weight=g(w)),
+             lambda g: V.norm_rotate(q, k, v, pos, turns, slots=slots, k_cache=g(kc), v_cache=vc),
+             lambda g: V.norm_rotate(q, k, v, pos, turns, slots=slots, k_cache=kc, v_cache=g(vc))]
+    for call in calls:
+        refused("requires a gradient", lambda: call(grad))
+        with torch.no_grad():
+            call(grad)
+        call(lambda x: grad(x).detach())
+
+
 # ------------------------------------------------------------------------------------------ values that are seen
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_seen_values_reach_the_row_however_small_their_weight(V, bad):

@@ -11,6 +11,7 @@ paged cache [pages, page_size, kv_heads, head_dim]:
 All take torch tensors on one CUDA device, queue their work on that device's current stream through the vesper_*_device
 entry points of libvesper_c.so, synchronise nothing and can be captured in a CUDA graph.  Outputs and workspaces come
 from torch's allocator in that stream's order.  Arguments that do not fit raise VesperError before any work is queued.
+There is no backward pass: where gradients are recorded, tensors that require one are refused.
 The checks and the calls are native (csrc/attention_torch.cpp, built to _attention.so beside the library).
 """
 from __future__ import annotations

@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -92,10 +93,17 @@ std::string shape_of(const at::Tensor& t) {
     return s + "]";
 }
 
+// There is no backward pass: a result outside the graph of its inputs would go unnoticed.
+void untracked(const at::Tensor& t, const char* name) {
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+        refuse(std::string(name) + " requires a gradient, and the operator has none: call it under torch.no_grad() or detach");
+}
+
 void same(const at::Tensor& t, c10::Device dev, at::ScalarType type, const char* name) {
     if (t.device() != dev) refuse(std::string(name) + " is on " + t.device().str() + ", not on " + dev.str());
     if (t.scalar_type() != type)
         refuse(std::string(name) + " is " + c10::toString(t.scalar_type()) + ", " + c10::toString(type) + " expected");
+    untracked(t, name);
 }
 
 // Address of a contiguous vector.
@@ -125,6 +133,7 @@ const at::Tensor& queries(PyObject* o) {
     dtype_of(q);
     if (q.dim() != 3) refuse("q must be bf16 or f16, [tokens, heads, head_dim]");
     inner(q, "q");
+    untracked(q, "q");
     return q;
 }
 
