@@ -100,6 +100,22 @@ def test_inputs_that_require_a_gradient_are_refused(V):
         call(lambda x: grad(x).detach())
 
 
+def test_tensors_written_in_place_count_the_write(V):
+    q, k, v, kc, vc, table, lens, pages, turns = some_inputs()
+    before = [t._version for t in (table, kc, vc)]
+    V.page_tables(lens, lens, pages, table, 16, 15)
+    V.norm_rotate(q, k, v, ints([0] * 5), turns, slots=ints([0, 1, 2, 3, 4], torch.int64), k_cache=kc, v_cache=vc)
+    assert [t._version for t in (table, kc, vc)] == [n + 1 for n in before]
+    both = rand(4, 2, 16, 2, 64)
+    old = both._version
+    V.norm_rotate(q, k, v, ints([0] * 5), turns, slots=ints([0] * 5, torch.int64), k_cache=both[:, 0], v_cache=both[:, 1])
+    assert both._version > old
+    with torch.inference_mode():  # such tensors have no version
+        table, kc, vc = table.clone(), kc.clone(), vc.clone()
+        V.page_tables(lens, lens, pages, table, 16, 15)
+    V.norm_rotate(q, k, v, ints([0] * 5), turns, slots=ints([0] * 5, torch.int64), k_cache=kc, v_cache=vc)
+
+
 # ------------------------------------------------------------------------------------------ values that are seen
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_seen_values_reach_the_row_however_small_their_weight(V, bad):

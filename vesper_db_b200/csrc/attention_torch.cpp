@@ -187,6 +187,11 @@ struct OnDevice {
     explicit OnDevice(c10::Device dev) : guard(dev), stream(c10::cuda::getCurrentCUDAStream(dev.index()).stream()) {}
 };
 
+// A tensor that a call has written in place counts the write, as torch's own calls do.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& like) { return at::empty(sizes, like.options()); }
 at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
     return at::empty(sizes, like.options().dtype(type));
@@ -233,6 +238,7 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         p.d_slots = static_cast<int64_t*>(slots.data_ptr());
         p.d_used = static_cast<int32_t*>(used.data_ptr());
         check(vesper_page_tables_device(&p, on.stream));
+        written(tensor(a[3], "table"));
         PyObject* t = PyTuple_New(5);
         PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(lengths)));
         PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(starts)));
@@ -293,6 +299,10 @@ PyObject* norm_rotate(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             p.d_out_k = out_k.data_ptr();
         }
         check(vesper_norm_rotate_device(&p, on.stream));
+        if (p.d_slots) {
+            written(tensor(a[10], "k_cache"));
+            written(tensor(a[11], "v_cache"));
+        }
         PyObject* second = out_k.defined() ? THPVariable_Wrap(std::move(out_k)) : none();
         return two(THPVariable_Wrap(std::move(out_q)), second);
     });
