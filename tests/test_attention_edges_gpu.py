@@ -76,6 +76,16 @@ def some_inputs():
     return q, k, v, kc, vc, ints([[0, 1]] * 5), ints([3] * 5), ints([2]), torch.zeros(9, 64, device="cuda")
 
 
+def test_truth_values_that_have_none_are_refused(V):
+    q, k, v, kc, vc, table, lens, pages, turns = some_inputs()
+    two, starts, pos = torch.tensor([True, False]), ints([0, 5]), ints([0] * 5)
+    refused("causal must be", lambda: V.prompt_attention(q, k, v, starts, causal=two))
+    refused("stats must be", lambda: V.prompt_attention(q, k, v, starts, stats=two))
+    refused("stats must be", lambda: V.shared_prefix_attention(q, kc, vc, pages, 9, table, lens, stats=two))
+    refused("pairs must be", lambda: V.norm_rotate(q, k, v, pos, turns, pairs=two))
+    refused("keep_k must be", lambda: V.norm_rotate(q, k, v, pos, turns, keep_k=two))
+
+
 def test_inputs_that_require_a_gradient_are_refused(V):
     """There is no backward pass: a result that silently stands outside the graph would train on wrong gradients."""
     q, k, v, kc, vc, table, lens, pages, turns = some_inputs()

@@ -87,6 +87,15 @@ double number(PyObject* o, const char* name) {
     return v;
 }
 
+bool truth(PyObject* o, const char* name) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse(std::string(name) + " must be true or false");
+    }
+    return v != 0;
+}
+
 std::string shape_of(const at::Tensor& t) {
     std::string s = "[";
     for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
@@ -281,7 +290,7 @@ PyObject* norm_rotate(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (a[5] != Py_None) p.d_q_weight = vector<void>(tensor(a[5], "q_weight"), dev, q.scalar_type(), "q_weight", dim);
         if (a[6] != Py_None) p.d_k_weight = vector<void>(tensor(a[6], "k_weight"), dev, q.scalar_type(), "k_weight", dim);
         p.eps = number(a[7], "eps");
-        p.pairs = PyObject_IsTrue(a[8]) ? 1 : 0;
+        p.pairs = truth(a[8], "pairs");
         if (a[9] != Py_None) {
             if (a[2] == Py_None || a[10] == Py_None || a[11] == Py_None) refuse("slots need v, k_cache and v_cache");
             p.d_slots = vector<int64_t>(tensor(a[9], "slots"), dev, at::kLong, "slots", t);
@@ -294,7 +303,7 @@ PyObject* norm_rotate(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         OnDevice on(dev);
         at::Tensor out_q = empty({t, heads, dim}, q), out_k;
         p.d_out_q = out_q.data_ptr();
-        if (PyObject_IsTrue(a[12])) {
+        if (truth(a[12], "keep_k")) {
             out_k = empty({t, kv, dim}, q);
             p.d_out_k = out_k.data_ptr();
         }
@@ -340,9 +349,9 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         p.n_requests = (size_t)starts.size(0) - 1;
         if (a[4] != Py_None)
             p.d_starts_k = vector<int32_t>(tensor(a[4], "starts_k"), dev, at::kInt, "starts_k", starts.size(0));
-        p.causal = PyObject_IsTrue(a[5]) ? 1 : 0;
+        p.causal = truth(a[5], "causal");
         p.scale = a[6] == Py_None ? 1.0 / std::sqrt((double)dim) : number(a[6], "scale");
-        const bool stats = PyObject_IsTrue(a[7]);
+        const bool stats = truth(a[7], "stats");
         OnDevice on(dev);
         at::Tensor out = empty({t, heads, dim}, q), lse, space;
         p.d_out = out.data_ptr();
@@ -386,7 +395,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_ar
         p.d_table = static_cast<const int32_t*>(page_table(a[5], dev, b, p.table_width, p.table_stride).data_ptr());
         p.d_lengths = vector<int32_t>(tensor(a[6], "lengths"), dev, at::kInt, "lengths", b);
         p.scale = a[7] == Py_None ? 1.0 / std::sqrt((double)dim) : number(a[7], "scale");
-        const bool stats = PyObject_IsTrue(a[8]);
+        const bool stats = truth(a[8], "stats");
         OnDevice on(dev);
         at::Tensor out = empty({b, heads, dim}, q), lse, space;
         p.d_out = out.data_ptr();
