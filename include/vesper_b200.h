@@ -467,7 +467,7 @@ VESPER_C_API vesper_status_t vesper_page_tables_device(const vesper_page_tables_
  * slot / page_size, slot % page_size; a slot that is negative or past n_pages *
  * page_size is skipped.  Two tokens with one slot: either one's row is kept.
  * A position outside the table gives NaN in the rotated values.
- * head_dim a multiple of 8 up to 256; turned a multiple of 16, 0 to head_dim.
+ * head_dim a multiple of 8 up to 256; turned a multiple of 16, 0 to head_dim; eps 0 to 3e38.
  * Without d_slots, v and the caches are not read and may be NULL. */
 typedef struct vesper_norm_rotate_params_s {
   size_t struct_size;
@@ -506,8 +506,8 @@ VESPER_C_API vesper_status_t vesper_norm_rotate_device(const vesper_norm_rotate_
  * zeros and lse -inf; what is in keys and values that a row does not see, infinities and
  * NaN included, does not reach it.  d_lse, unless NULL: [n_q, heads] log-sum-exp.
  * starts are bounded to [0, n_q] and [0, n_k].  d_out [n_q, heads, head_dim] contiguous.
- * head_dim a multiple of 8 up to 128; scale > 0; n_q, n_k below 2^31; d_workspace:
- * vesper_prompt_attention_workspace bytes (16-byte aligned, NULL when that is 0). */
+ * head_dim a multiple of 8 up to 128; scale > 0, at most 2e38; n_q, n_k below 2^31;
+ * d_workspace: vesper_prompt_attention_workspace bytes (16-byte aligned, NULL when that is 0). */
 typedef struct vesper_prompt_attention_params_s {
   size_t struct_size;
   size_t dtype;
