@@ -90,7 +90,9 @@ float scale_of(double scale) {
 
 vgpu::PromptArgs prompt_args(const vesper_prompt_attention_params_t& p) {
     check_heads(p.dtype, p.heads, p.kv_heads, p.head_dim, 128);
-    need(p.n_q <= kMaxInt && p.n_k <= kMaxInt && p.n_requests <= kMaxInt - 1, "at most 2^31 - 1 tokens");
+    // Rows, keys and pieces are numbered in 32 bits, and counted in whole tiles past their ends.
+    need(p.n_q < kMaxInt - 256 && p.n_k < kMaxInt - 256 && p.n_requests < kMaxInt - 256,
+         "tokens and requests must be below 2^31 - 257");
     vgpu::PromptArgs a{};
     a.f16 = p.dtype == VESPER_F16;
     a.heads = (int)p.heads;

@@ -294,7 +294,7 @@ __device__ __forceinline__ Work find_work(const TileParams& p, int idx, int lane
     w.k0 = k0;
     w.len_k = k1 - k0;
     w.step = p.causal ? 1 : 0;
-    w.first_lim = p.causal ? tok + 1 + w.len_k - len_q : w.len_k;
+    w.first_lim = p.causal ? w.len_k - (len_q - tok - 1) : w.len_k;
     return w;
 }
 
