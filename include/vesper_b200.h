@@ -505,7 +505,8 @@ VESPER_C_API vesper_status_t vesper_norm_rotate_device(const vesper_norm_rotate_
  * keys are given.  A row that sees no key, and rows of q past d_starts[n_requests], give
  * zeros and lse -inf; what is in keys and values that a row does not see, infinities and
  * NaN included, does not reach it.  d_lse, unless NULL: [n_q, heads] log-sum-exp.
- * starts are bounded to [0, n_q] and [0, n_k].  d_out [n_q, heads, head_dim] contiguous.
+ * starts are bounded to [0, n_q] and [0, n_k] and must not decrease: where they do, rows of d_out
+ * may stay unwritten.  d_out [n_q, heads, head_dim] contiguous.
  * head_dim a multiple of 8 up to 128; scale > 0, at most 2e38; n_q, n_k and
  * n_requests below 2^31 - 257; d_workspace: vesper_prompt_attention_workspace bytes (16-byte
  * aligned, NULL when that is 0). */

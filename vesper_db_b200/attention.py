@@ -89,7 +89,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     """Attention over packed prompts (vesper_prompt_attention_device).
 
     q [tokens, heads, head_dim], k and v [key tokens, kv_heads, head_dim]; starts int32 [requests + 1]: request b is
-    rows starts[b] to starts[b + 1] of q, and of k and v unless starts_k says otherwise.  causal: the last query of a
+    rows starts[b] to starts[b + 1] of q, and of k and v unless starts_k says otherwise; neither may decrease.  causal: the last query of a
     request sees all its keys, each one before it one key less.  scale: 1 / sqrt(head_dim) by default.  Returns out
     [tokens, heads, head_dim], with stats (out, lse): the float32 [tokens, heads] log-sum-exp.  Rows that see no key
     are zero, their lse -inf.

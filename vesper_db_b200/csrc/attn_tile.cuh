@@ -26,10 +26,16 @@
 // shared memory (256 KB read and written, 128 bytes a cycle).  Making a quarter or three
 // eighths of the exponentials by a polynomial on the FMA units instead cost 1 to 7 %: the
 // issue slots it takes are worth more than the special-function cycles it frees.
-// Measured (bf16, heads of 128, 32 over 8): 16,384 tokens, causal: 1,990 to 2,070 us by
-// machine, 1,060 to 1,105 TFLOP/s of 1,404 for a library product that runs as long; tensor cores and special-function units
-// 56 % busy each, at 990 W and 1.6 GHz: the power limit.  24 prompts of 1 to 4,000 tokens:
-// 710 us, 47 % busy.  256 tokens over a prefix of 20,000: 91 us with the join, 41 %, on 128 SMs.
+// Measured (bf16, heads of 128, 32 over 8): 16,384 tokens, causal: 2,030 to 2,060 us in long
+// runs, 1,070 to 1,080 TFLOP/s of 1,404 for a library product that runs as long, at 990 W and
+// 1.6 GHz: the power limit; 1,750 us in the first milliseconds.  Tensor cores and
+// special-function units are 56 % busy each, as cycles go.  24 prompts of 1 to 4,000 tokens:
+// 720 us in long runs, 620 in the first milliseconds (1.17 M cycles), 47 % busy.  256 tokens
+// over a prefix of 20,000: 93 us with the join, 42 %, on 128 SMs.
+//
+// P is rounded to the data's type, as a product takes both operands in one 16-bit type; its sum l
+// is of the unrounded values.  Against 64 bits the long cases' outputs are off by 0.0021 to 0.0023 of
+// their size then, where rounding them once costs 0.0016 (bf16; f16: 0.00025 to 0.00028, 0.00021).
 //
 // m only moves when a row's maximum has grown by more than 2^8: until then P may reach 2^8,
 // which both types hold at full relative precision, and O need not be rescaled.

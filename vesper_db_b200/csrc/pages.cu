@@ -21,8 +21,8 @@ namespace {
 // fills its share of tokens and table rows.  What the tokens need of a request is in shared
 // memory by then, and a token's new page is taken from the free list directly, never from a
 // table entry that another block may still be writing.  Bound by the latency of its chain of
-// loads: lengths, then pages, then the stores.  Measured: 64 requests of one token 4.6 us,
-// 1,500 prompts with 778,000 tokens (9.6 MB read and written) 10.6 us.
+// loads: lengths, then pages, then the stores.  Measured: 64 requests of one token 4.7 us,
+// 1,500 prompts with 778,000 tokens (9.6 MB read and written) 10.4 us.
 // ---------------------------------------------------------------------------------
 constexpr int kScanThreads = 512, kRun = 4;  // tokens a thread takes at once
 
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kScanThreads) page_tables_kernel(const __grid_
 // share their eight angles; neighbouring pairs: chunks 2 l and 2 l + 1), so that the partners
 // need no exchange.  Groups step over the (token, head) rows of the batch, neighbouring
 // groups on neighbouring heads, and request the next row before the current one is used.
-// Measured (bf16, 32 + 8 heads of 128, 50,000 tokens, 1.36 GB with the cache): 256 us, 5.3 TB/s;
-// 33 tokens: 2.6 us.
+// Measured (bf16, 32 + 8 heads of 128, 50,000 tokens, 1.36 GB with the cache): 249 us, 5.5 TB/s
+// (264 among calls whose inputs change); 33 tokens: 2.4 us.
 // ---------------------------------------------------------------------------------
 constexpr int kRotThreads = 256, kRotBlocks = 3;  // threads a block, blocks an SM
 
