@@ -105,14 +105,15 @@ constexpr int smem_bytes() {
     return 2 * kRows * D * 2 + kSlots * kKeys * D * 2 + 1024 + 512 + 2 * 2 * 2 * kRows * 4 + kSoftmaxWarps * 1024;
 }
 
-// Bounded wait for the barrier's phase; false when it ran out.  2^20 polls of 20 cycles and more
-// are over 10 ms.  The longest stretch that a warp waits for another is the results of a piece,
-// with at most 2 * 128 rows of values looked through once more: 0.12 ms a piece where all of
-// them hold a non-finite value (eight prompts of 2,000 tokens, 8 heads of 128: 119 us clean, 220
-// with one in thirty tokens, 537 with all).
+// Bounded wait for the barrier's phase; false when it ran out.  A poll suspends for 3.95 us
+// (measured), so 2^18 of them are a second.  The longest stretch between two arrivals is the
+// results of a piece, with at most 2 * 128 rows of values looked through once more: 0.12 ms where
+// all of them hold a non-finite value (eight prompts of 2,000 tokens, 8 heads of 128: 119 us clean,
+// 220 with one in thirty tokens, 537 with all).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     const uint32_t a = tc::smem_u32(bar);
-    for (uint32_t i = 0; i < (1u << 20); ++i) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 18); ++i) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -372,10 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     int* const s_leak = reinterpret_cast<int*>(s_work + kAhead + 1);  // [kAhead][2]: piece, query tile
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(s_leak + 2 * kAhead);
     volatile int* const s_lost = reinterpret_cast<int*>(tmem_slot + 1);  // a wait ran out
+    volatile uint32_t* const s_copies = tmem_slot + 2;                   // key and value tiles asked for
     // Rows' maxima (and sums) of each half of the keys: [turn][tile][half][row]
     float* const s_half = reinterpret_cast<float*>(bars + 64);
     const uint32_t s_stage = tc::smem_u32(s_half + 2 * 2 * 2 * kRows);  // 1 KB a softmax warp, for the results
-    static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + (kAhead + 1) * sizeof(Work) + 2 * kAhead * 4 + 8 <= 512, "");
+    static_assert((2 + 2 + 2 * kSlots + 2 + 4 + 2 + 2 + 2 + 2 + 2 * kAhead) * 8 + (kAhead + 1) * sizeof(Work) + 2 * kAhead * 4 + 12 <= 512, "");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // The own pages' kernel may be queued behind this one and does not depend on it.
@@ -407,6 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             }
             for (int i = 0; i <= kAhead; ++i) s_work[i].tokens = 0;
             *s_lost = 0;
+            *s_copies = 0;
             tc::mbar_init(landed, 2);
             tc::mbar_init(clean, 1);
             tc::mbar_init_fence();
@@ -428,6 +431,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(b, parity)) != 0;
         return ok;
     };
+    // A wait that may last for all key tiles of a piece (2.3 us each), however many they are: it runs
+    // out when the block has asked for none in a second.  Only where that can be, as the second loop
+    // costs: 200 short passages took 158 us instead of 125 with it in every wait.
+    auto wait_on = [&](uint64_t* b, uint32_t parity) {
+        uint32_t before = ~0u;
+#pragma unroll 1
+        while (ok && !__all_sync(0xffffffffu, mbar_wait(b, parity))) {
+            const uint32_t now = (uint32_t)uniform((int)*s_copies);
+            ok = now != before;
+            before = now;
+        }
+        return ok;
+    };
     // The piece of work number `it` of the block; false when a wait ran out.  `done` hands its
     // place back; whoever reads the leak flag does that at the end.
     auto work_done = [&](uint32_t it) {
@@ -435,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         if (lane == 0) tc::mbar_arrive(&work_empty[it % kAhead]);
     };
     auto next_work = [&](Work& w, uint32_t it) {
-        if (!wait(&work_full[it % kAhead], (it / kAhead) & 1)) return false;
+        if (!wait_on(&work_full[it % kAhead], (it / kAhead) & 1)) return false;
         w = s_work[it % kAhead];
         return true;
     };
@@ -490,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 for (int i = 0; i < 2 * x.n; ++i, ++kv) {  // K, V, K, V, ...
                     const int slot = kv % kSlots, round = kv / kSlots, key = (x.j0 + (i >> 1)) * kKeys;
                     if (round > 0 && !wait(&kv_empty[slot], (round - 1) & 1)) break;
+                    if (lane == 0) *s_copies = kv;
                     const CUtensorMap* map = (i & 1) ? &p.mv : &p.mk;
                     const uint32_t dst = s_kv + slot * kTileBytes;
                     if (!PAGED) {
@@ -619,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 const Tiles x = tiles_of(w, tt, p.splits);
                 for (int j = 0; j < x.n; ++j) {
                     if (!x.guarded(j)) continue;
-                    if (!wait(landed, seen++ & 1)) break;  // both warps of products have seen the tile land
+                    if (!wait_on(landed, seen++ & 1)) break;  // both warps of products have seen the tile land
                     uint8_t* const v = smem + (2 + (kv + 2 * j + 1) % kSlots) * kTileBytes;
                     const int key = (x.j0 + j) * kKeys;
                     const int end = min(max(w.len_k - key, 0), kKeys), from = max(x.min_lim - key, 0);
@@ -706,7 +723,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             };
             for (int j = 0; j < my_tiles; ++j) {
                 // after a wait that ran out the row's warps only keep meeting
-                wait(&s_full[t], tiles++ & 1);
+                // (the first scores may come after the other tile's keys of the piece before)
+                if (j == 0) wait_on(&s_full[t], tiles++ & 1);
+                else wait(&s_full[t], tiles++ & 1);
                 tc::fence_after_sync();
                 const int key = (j0 + j) * kKeys + half * 64;
                 if (key >= warp_lim) {  // no row of the warp sees these keys: P is zero
