@@ -411,7 +411,9 @@ VESPER_C_API vesper_status_t vesper_flat_get_last_timings(vesper_flat_timings_t*
  * No call allocates, so all of them can be captured in a CUDA graph.  16-bit data is
  * dtype VESPER_BF16 or VESPER_F16; arithmetic is in 32 bits with one rounding at the
  * output, but the attention probabilities are rounded to dtype before they meet the
- * values (the sums they are divided by are not).
+ * values (the sums they are divided by are not).  The tensor cores' 32-bit sums drop what
+ * lies below their last bit: with equal weights a result over n keys comes out low by up to
+ * 6e-9 n of its size where one block takes them all (0.15 % at 262,144 keys).
  * Strides are in elements.  Data pointers are 16-byte aligned, strides positive multiples
  * of 8 elements, and the last dimension is contiguous.  page_size is a power of two from 16
  * to 256.  heads is a multiple of kv_heads, at most 128 times of it; query head h reads
